@@ -22,7 +22,10 @@ OBJ_DIR = os.path.join(HERE, "lib", "obj" + (f"_{_TAG}" if _TAG else ""))
 LIB = os.path.join(OUT_DIR, f"libnbx_{_TAG}.so" if _TAG else "libnbx.so")
 ARCH = os.environ.get("NBX_OFFLOAD_ARCH", "gfx950")
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-result",
-         "-munsafe-fp-atomics", "-save-temps=obj"]
+         "-munsafe-fp-atomics", "-save-temps=obj",
+         # no packed fp32 VALU forms (v_pk_fma_f32 and kin): some have given wrong results now and then
+         # on these machines (the host pass warns that it does not know the feature; harmless)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-file extra flags: the split-precision MFMA kernels' VALU work (operand splits, the message
 # kernel's edge combination) runs beside MFMAs, where packed fp32 VALU costs extra cycles; with
 # SLP vectorisation off these files run 1.8 % more steps/s (measured, C2).
