@@ -12,7 +12,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("NBX_LIB") or os.path.join(_HERE, "lib", "libnbx.so")  # NBX_LIB: A/B builds only
-ABI_VERSION = 19
+ABI_VERSION = 20
 COMM_ID_BYTES = 128
 ROLLOUT_ABSOLUTE = 1   # NBX_ROLLOUT_ABSOLUTE
 GEMM_TRANS_A, GEMM_TRANS_B, GEMM_B_ONES, GEMM_ONES_TAIL = 1, 2, 4, 8
@@ -21,6 +21,7 @@ MAX_LAYERS = 64
 
 c_i64, c_i32, c_f, c_d, c_p, c_sz = (ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_double,
                                      ctypes.c_void_p, ctypes.c_size_t)
+c_u32 = ctypes.c_uint32
 
 
 class SegnnLayer(ctypes.Structure):
@@ -111,6 +112,32 @@ class Eqv2Weights(ctypes.Structure):
                            "vel_b")] + [
         ("edge_degree", Eqv2Radial), ("norm_w", c_p), ("norm_b", c_p), ("force", Eqv2Attn),
         ("blocks", Eqv2Block * EQV2_MAX_LAYERS)]
+
+
+F32, BF16, F16 = 0, 1, 2                     # NBX_F32 / NBX_BF16 / NBX_F16
+DROP_ELEMENT, DROP_GROUP, DROP_CHANNEL = 0, 1, 2
+
+
+class ResidualNormArgs(ctypes.Structure):
+    _fields_ = [(n, c_i64) for n in ("rows", "C", "ldx", "ldy", "gate_groups", "group")] + [
+        (n, c_i32) for n in ("x_dtype", "y_dtype", "param_dtype", "norm")] + [
+        ("eps", c_f), ("scale", c_f), ("threshold", c_u32), ("call", c_u32)] + [(n, c_p) for n in (
+            "rng", "used", "x", "y", "gate", "post_w", "post_b", "pre_w", "pre_b", "h", "z", "stats", "dh", "dz", "dx",
+            "dy", "dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b", "workspace")] + [("workspace_bytes", c_sz)]
+
+
+class ShResidualNormArgs(ctypes.Structure):
+    _fields_ = [("V", c_i64), ("path_group", c_i64)] + [(n, c_i32) for n in ("lmax", "C", "dtype", "param_dtype")] + [
+        ("eps", c_f), ("path_threshold", c_u32), ("channel_threshold", c_u32), ("call", c_u32)] + [(n, c_p) for n in (
+            "rng", "used", "x", "y", "weight", "bias", "h", "z", "stats", "dh", "dz", "dx", "dy", "dweight", "dbias",
+            "workspace")] + [("workspace_bytes", c_sz)]
+
+
+class SegmentAttentionArgs(ctypes.Structure):
+    _fields_ = [(n, c_i64) for n in ("V", "E", "K")] + [(n, c_i32) for n in ("H", "D", "v_dtype", "l_dtype")] + [
+        ("threshold", c_u32), ("call", c_u32)] + [(n, c_p) for n in (
+            "rng", "used", "ptr", "eid", "values", "logits", "out", "stats", "dout", "dvalues", "dlogits",
+            "workspace")] + [("workspace_bytes", c_sz)]
 
 
 _SIGNATURES = {
@@ -232,6 +259,19 @@ _SIGNATURES = {
                                               c_d * 8, ctypes.POINTER(c_f)]),
     "nbx_eqv2_rollout": (ctypes.c_int, [ctypes.POINTER(Eqv2Weights), c_p, c_p, c_p, c_i64, c_i64, c_i64, c_i32,
                                         ctypes.c_uint64, c_p, c_p, c_p, c_sz, c_p]),
+    "nbx_dropout": (ctypes.c_int, [c_i32, c_i32, c_i64, c_i64, c_i64, c_i64, c_u32, c_p, c_u32, c_p, c_p, c_p, c_p]),
+    "nbx_residual_norm": (ctypes.c_int, [ctypes.POINTER(ResidualNormArgs), c_p]),
+    "nbx_residual_norm_backward_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(ResidualNormArgs),
+                                                                  ctypes.POINTER(c_sz)]),
+    "nbx_residual_norm_backward": (ctypes.c_int, [ctypes.POINTER(ResidualNormArgs), c_p]),
+    "nbx_sh_residual_norm": (ctypes.c_int, [ctypes.POINTER(ShResidualNormArgs), c_p]),
+    "nbx_sh_residual_norm_backward_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(ShResidualNormArgs),
+                                                                     ctypes.POINTER(c_sz)]),
+    "nbx_sh_residual_norm_backward": (ctypes.c_int, [ctypes.POINTER(ShResidualNormArgs), c_p]),
+    "nbx_segment_attention_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(SegmentAttentionArgs), c_i32,
+                                                             ctypes.POINTER(c_sz)]),
+    "nbx_segment_attention": (ctypes.c_int, [ctypes.POINTER(SegmentAttentionArgs), c_p]),
+    "nbx_segment_attention_backward": (ctypes.c_int, [ctypes.POINTER(SegmentAttentionArgs), c_p]),
 }
 
 _lib = None

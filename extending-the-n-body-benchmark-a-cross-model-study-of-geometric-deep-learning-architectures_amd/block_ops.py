@@ -1,0 +1,489 @@
+"""Operators around a training block's products (include/nbx.h "Block operators", csrc/block_ops.hip and
+csrc/segment_attention.hip), each an autograd operator on the caller's stream:
+
+* :func:`dropout` — dropout of elements, of whole groups of rows (stochastic depth) or of channels, whose
+  mask is never stored: forward and backward draw it from a counter;
+* :func:`residual_norm` — the residual add of a block's output with its gate (layer scale), dropout and the
+  LayerNorm or RMS norm before and after it, in one pass;
+* :func:`sh_residual_norm` — the same with EquiformerV2's norm over spherical-harmonics coefficients;
+* :func:`segment_attention` — softmax over the edges into a node, dropout of the weights and the weighted sum
+  of the edges' values in one pass.
+
+Activations are float32, bfloat16 or float16; sums, statistics and draws' factors are float32 and each
+result is rounded once.  Every reduction has a fixed order: the same call gives the same bits.
+
+Random numbers: ``rng`` is a :class:`CounterRNG`, or its state tensor with an explicit ``call``.  A draw is a
+function of (seed, step, call, index) alone (Philox4x32-10), so a step can be repeated, captured into a graph
+(the step is read on the device: ``rng.advance()`` between or inside replays gives new draws) and its
+backward pass needs no mask.  The drop rate is resolved to 2^-16 and the scale is that of the resolved rate,
+so the mean is exact.  A dropped element is 0 whatever it held.
+
+Like the framework's other operators these run on the HIP device only.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_f32 = torch.float32
+_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_PER = {"element": _lib.DROP_ELEMENT, "group": _lib.DROP_GROUP, "channel": _lib.DROP_CHANNEL}
+_NORM = {"layer": 0, "rms": 1}
+
+
+class CounterRNG:
+    """The state of the counter-based draws: a device tensor ``state`` (seed, step) and the number of the next
+    call of this step.  Call :meth:`advance` once per training step; ``seed`` is any 64-bit integer."""
+
+    def __init__(self, seed=0, device="cuda", step=0):
+        seed = int(seed) & (2 ** 64 - 1)
+        self.state = torch.tensor([seed - 2 ** 64 if seed >= 2 ** 63 else seed, int(step)], dtype=torch.int64,
+                                  device=device)
+        self._next = 0
+
+    def take(self, calls=1):
+        """The number of the step's next call (of ``calls`` consecutive ones)."""
+        c = self._next
+        self._next += calls
+        return c
+
+    def advance(self, steps=1):
+        """The next step, on the device (may be captured), with its calls counted from 0 again."""
+        self.state[1:].add_(steps)
+        self._next = 0
+
+    def state_dict(self):
+        return {"state": self.state.clone(), "next": self._next}
+
+    def load_state_dict(self, d):
+        self.state.copy_(d["state"])
+        self._next = int(d["next"])
+
+
+def _threshold(p):
+    """The 16-bit threshold of a drop rate."""
+    p = float(p)
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"the drop rate must be in [0, 1), got {p}")
+    t = int(65536 * p + 0.5)
+    if (t == 0 and p > 0.0) or t >= 65536:
+        raise ValueError(f"drop rates are resolved to 2^-16: {p} cannot be told from {0 if t == 0 else 1}")
+    return t
+
+
+def _draws(rng, call, calls, device):
+    """(state tensor, number of the first of ``calls`` calls)."""
+    if isinstance(rng, CounterRNG):
+        state = rng.state
+        call = rng.take(calls) if call is None else call
+    elif isinstance(rng, torch.Tensor):
+        state = rng
+        if call is None:
+            raise ValueError("a state tensor needs an explicit call")
+    else:
+        raise TypeError("a drop rate needs rng, a CounterRNG or its state tensor")
+    if state.dtype != torch.int64 or state.shape != (2,) or state.device != device:
+        raise ValueError(f"the state must be int64 [2] on {device}, got {state.dtype} {list(state.shape)} on {state.device}")
+    call = int(call)
+    if not 0 <= call <= 2 ** 32 - calls:
+        raise ValueError(f"call must be in [0, 2^32), got {call}")
+    return state.contiguous(), call
+
+
+def _device(*tensors):
+    """The HIP device of the tensors (None entries are skipped); raises unless all are on it."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None:
+            if not t.is_cuda:
+                raise _lib.NbxError("nbx ops run on the HIP device only; got a CPU tensor")
+            if t.device != dev:
+                raise ValueError(f"tensors on {dev} and on {t.device}")
+    return dev
+
+
+def _dtype(t, what):
+    code = _CODE.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+_SAME = contextlib.nullcontext()
+
+
+def _on(dev):
+    """Launches go to the tensors' device, whichever is current."""
+    return _SAME if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _call(name, *args):
+    _lib.check(getattr(_lib.lib(), name)(*args), name)
+
+
+def _workspace(name, args, dev, *more):
+    n = _lib.c_sz()
+    _call(name, ctypes.byref(args), *more, ctypes.byref(n))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
+    args.workspace, args.workspace_bytes = _ptr(ws), n.value
+    return ws
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _dense(g):
+    return None if g is None else g.contiguous()
+
+
+# ---------------------------------------------------------------------------------------------- dropout
+def _dropout(x, mode, dims, threshold, state, call, used):
+    y = torch.empty_like(x)
+    dev = x.device
+    with _on(dev):
+        _call("nbx_dropout", _CODE[x.dtype], mode, *dims, threshold, state.data_ptr(), call, _ptr(used), x.data_ptr(),
+              y.data_ptr(), _lib.stream_ptr(dev))
+    return y
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, mode, dims, threshold, state, call):
+        used = torch.empty(2, dtype=torch.int64, device=x.device)
+        y = _dropout(x, mode, dims, threshold, state, call, used)
+        ctx.save_for_backward(used)
+        ctx.how = (mode, dims, threshold, call)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        mode, dims, threshold, call = ctx.how
+        (used,) = ctx.saved_tensors
+        return _dropout(dy.contiguous(), mode, dims, threshold, used, call, None), None, None, None, None, None
+
+
+def dropout(x, p, rng=None, *, call=None, per="element", group=1):
+    """``x`` with a share ``p`` of it set to 0 and the rest scaled by 1 / (1 - p).
+
+    per="element": every element on its own.  per="group": ``group`` consecutive entries of the first axis share
+    a draw (stochastic depth of a system's nodes).  per="channel": x [n, ..., C], one draw for each (entry,
+    channel), shared by the axes between.  p = 0 returns ``x``."""
+    threshold = _threshold(p)
+    if per not in _PER:
+        raise ValueError(f'per must be "element", "group" or "channel", got {per!r}')
+    if int(group) < 1:
+        raise ValueError(f"group must be at least 1, got {group}")
+    _dtype(x, "x")
+    if per != "element" and x.dim() < (1 if per == "group" else 2):
+        raise ValueError(f"per={per!r} needs more axes than {list(x.shape)} has")
+    dev = _device(x)
+    if threshold == 0:
+        return x
+    state, call = _draws(rng, call, 1, dev)
+    x = x.contiguous()
+    n = x.shape[0] if x.dim() and per != "element" else 1
+    C = x.shape[-1] if per == "channel" else 1
+    dims = (n, x.numel() // max(n * C, 1), C, int(group))
+    if _wants_grad(x):
+        return _DropoutFn.apply(x, _PER[per], dims, threshold, state, call)
+    return _dropout(x, _PER[per], dims, threshold, state, call, None)
+
+
+# ---------------------------------------------------------------------------------------------- residual + norms
+def _rows(t, C):
+    """(tensor, elements between its rows): strided rows are read in place, anything else is copied."""
+    if t.dim() == 2 and t.shape[0] > 1 and t.stride(1) == 1 and t.stride(0) >= C:
+        return t, t.stride(0)
+    return t.contiguous(), C
+
+
+def _residual_args(how, x, y, gate, post_w, post_b, pre_w, pre_b):
+    rows, C, ldx, ldy, codes, norm, eps, scale, threshold, group, call = how
+    a = _lib.ResidualNormArgs(rows, C, ldx, ldy, gate.numel() // C if gate is not None else 0, group, *codes, norm, eps,
+                              scale, threshold, call)
+    a.x, a.y, a.gate = _ptr(x), _ptr(y), _ptr(gate)
+    a.post_w, a.post_b, a.pre_w, a.pre_b = _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(pre_b)
+    return a
+
+
+def _residual_forward(how, x, y, gate, post_w, post_b, pre_w, pre_b, state, used, stats):
+    dev = x.device
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    z = torch.empty(y.shape, dtype=y.dtype, device=dev) if pre_w is not None else None
+    a = _residual_args(how, x, y, gate, post_w, post_b, pre_w, pre_b)
+    a.rng, a.used, a.h, a.z, a.stats = _ptr(state), _ptr(used), h.data_ptr(), _ptr(z), _ptr(stats)
+    with _on(dev):
+        _call("nbx_residual_norm", ctypes.byref(a), _lib.stream_ptr(dev))
+    return h, z
+
+
+class _ResidualNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, how, state, x, y, gate, post_w, post_b, pre_w, pre_b):
+        dev, rows = x.device, how[0]
+        used = torch.empty(2, dtype=torch.int64, device=dev) if state is not None else None
+        norms = post_w is not None or pre_w is not None
+        stats = torch.empty(4, rows, dtype=_f32, device=dev) if norms else None
+        h, z = _residual_forward(how, x, y, gate, post_w, post_b, pre_w, pre_b, state, used, stats)
+        # y is read again for its norm and the gate's gradient only, h for the norm behind it
+        keep_y = y if post_w is not None or (gate is not None and ctx.needs_input_grad[4]) else None
+        ctx.save_for_backward(keep_y, h if pre_w is not None else None, gate, post_w, post_b, pre_w, pre_b, used, stats)
+        ctx.how = how
+        ctx.shapes = (x.shape, x.dtype, y.shape, y.dtype)
+        ctx.set_materialize_grads(False)
+        return (h, z) if z is not None else h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, dz=None):
+        if dh is None and dz is None:
+            return (None,) * 9
+        y, h, gate, post_w, post_b, pre_w, pre_b, used, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        xs, xt, ys, yt = ctx.shapes
+        dh, dz = _dense(dh), _dense(dz)
+        dev = (dh if dh is not None else dz).device
+        a = _residual_args(ctx.how, None, y, gate, post_w, post_b, pre_w, pre_b)
+        grads = [torch.empty(xs, dtype=xt, device=dev) if need[2] else None,
+                 torch.empty(ys, dtype=yt, device=dev) if need[3] else None]
+        # without dz nothing reaches the norm behind the sum: its parameters' gradients are 0
+        grads += [torch.empty_like(t) if need[4 + i] and t is not None else None
+                  for i, t in enumerate((gate, post_w, post_b, pre_w, pre_b))]
+        a.rng, a.h, a.stats, a.dh, a.dz = _ptr(used), _ptr(h), _ptr(stats), _ptr(dh), _ptr(dz)
+        a.dx, a.dy, a.dgate, a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = (_ptr(g) for g in grads)
+        with _on(dev):
+            ws = _workspace("nbx_residual_norm_backward_workspace_bytes", a, dev)
+            _call("nbx_residual_norm_backward", ctypes.byref(a), _lib.stream_ptr(dev))
+        del ws
+        return (None, None, *grads)
+
+
+def residual_norm(x, y, *, gate=None, scale=1.0, post=None, pre=None, norm="rms", eps=1e-5, p=0.0, group=0, rng=None,
+                  call=None):
+    """The residual stream after a block: ``h = x + scale * dropout(gate * u)`` with ``u = y`` or, with ``post``
+    (weight, bias or None), the norm of y; and with ``pre`` (weight, bias or None) the norm of h that the next
+    block reads.  Returns (h, z); z is None without ``pre``.
+
+    x (the stream) and y (the block's output) [..., C] of one shape, C <= 8192; y of x's type, or of 16 bits
+    under a float32 stream.  norm = "rms" or "layer" (biased variance), for both places.  gate: [C] (layer
+    scale), [G, C] (one row for each rows / G consecutive rows) or y's shape.  gate and the norms' parameters
+    are all float32 or all of y's type; their gradients are column sums in float32, rounded once.  p: drop rate
+    of every element, or with group > 0 of whole groups of that many consecutive rows."""
+    if norm not in _NORM:
+        raise ValueError(f'norm must be "rms" or "layer", got {norm!r}')
+    threshold = _threshold(p)
+    post_w, post_b = post if post is not None else (None, None)
+    pre_w, pre_b = pre if pre is not None else (None, None)
+    if (post is not None and post_w is None) or (pre is not None and pre_w is None):
+        raise ValueError("a norm needs its weight")
+    params = [t for t in (gate, post_w, post_b, pre_w, pre_b) if t is not None]
+    if x.shape != y.shape or x.dim() < 1:
+        raise ValueError(f"x {list(x.shape)} and y {list(y.shape)} must have one shape [..., C]")
+    cx, cy = _dtype(x, "x"), _dtype(y, "y")
+    if cx != cy and cx != _lib.F32:
+        raise TypeError(f"y must have x's type, or x be float32: got {x.dtype} and {y.dtype}")
+    C = x.shape[-1]
+    if not 1 <= C <= 8192:
+        raise ValueError(f"need 1 <= C <= 8192, got {C}")
+    rows = x.numel() // C
+    cp = _dtype(params[0], "gate and norm parameters") if params else _lib.F32
+    if any(t.dtype != params[0].dtype for t in params) or cp not in (_lib.F32, cy):
+        raise TypeError(f"gate and norm parameters must all be float32 or all {y.dtype}")
+    for t in (post_w, post_b, pre_w, pre_b):
+        if t is not None and t.shape != (C,):
+            raise ValueError(f"a norm's parameters must be [{C}], got {list(t.shape)}")
+    if gate is not None and (gate.dim() < 1 or gate.shape[-1] != C or (rows and gate.numel() == 0)
+                             or rows % max(gate.numel() // C, 1)):
+        raise ValueError(f"gate {list(gate.shape)} must be [C], [G, C] with G dividing the {rows} rows, or y's shape")
+    if int(group) < 0:
+        raise ValueError(f"group must be at least 0, got {group}")
+    dev = _device(x, y, *params)
+    state = None
+    if threshold:
+        state, call = _draws(rng, call, 1, dev)
+    if rows == 0:
+        return x.clone(), (y.clone() if pre_w is not None else None)
+    x, ldx = _rows(x, C)
+    y, ldy = _rows(y, C)
+    params = [None if t is None else t.contiguous() for t in (gate, post_w, post_b, pre_w, pre_b)]
+    how = (rows, C, ldx, ldy, (cx, cy, cp), _NORM[norm], float(eps), float(scale), threshold, int(group), call or 0)
+    if _wants_grad(x, y, *params):
+        out = _ResidualNormFn.apply(how, state, x, y, *params)
+        return out if pre_w is not None else (out, None)
+    return _residual_forward(how, x, y, *params, state, None, None)
+
+
+# ---------------------------------------------------------------------------------------------- spherical harmonics
+def _sh_args(how, weight, bias):
+    V, path_group, lmax, C, code, cp, eps, t1, t2, call = how
+    a = _lib.ShResidualNormArgs(V, path_group, lmax, C, code, cp, eps, t1, t2, call)
+    a.weight, a.bias = _ptr(weight), _ptr(bias)
+    return a
+
+
+def _sh_forward(how, x, y, weight, bias, state, used, stats):
+    dev = x.device
+    h, z = torch.empty_like(x), torch.empty_like(x)
+    a = _sh_args(how, weight, bias)
+    a.rng, a.used, a.x, a.y, a.h, a.z, a.stats = (_ptr(state), _ptr(used), x.data_ptr(), y.data_ptr(), h.data_ptr(),
+                                                  z.data_ptr(), _ptr(stats))
+    with _on(dev):
+        _call("nbx_sh_residual_norm", ctypes.byref(a), _lib.stream_ptr(dev))
+    return h, z
+
+
+class _ShResidualNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, how, state, x, y, weight, bias):
+        dev = x.device
+        used = torch.empty(2, dtype=torch.int64, device=dev) if state is not None else None
+        stats = torch.empty(2, x.shape[0], dtype=_f32, device=dev)
+        h, z = _sh_forward(how, x, y, weight, bias, state, used, stats)
+        ctx.save_for_backward(h, weight, bias, used, stats)
+        ctx.how = how
+        ctx.set_materialize_grads(False)
+        return h, z
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, dz):
+        if dh is None and dz is None:
+            return (None,) * 6
+        h, weight, bias, used, stats = ctx.saved_tensors
+        dev, need = h.device, ctx.needs_input_grad
+        dh, dz = _dense(dh), _dense(dz)
+        a = _sh_args(ctx.how, weight, bias)
+        grads = [torch.empty_like(t) if n else None for t, n in zip((h, h, weight, bias), need[2:])]
+        a.rng, a.h, a.stats, a.dh, a.dz = _ptr(used), h.data_ptr(), stats.data_ptr(), _ptr(dh), _ptr(dz)
+        a.dx, a.dy, a.dweight, a.dbias = (_ptr(g) for g in grads)
+        with _on(dev):
+            ws = _workspace("nbx_sh_residual_norm_backward_workspace_bytes", a, dev)
+            _call("nbx_sh_residual_norm_backward", ctypes.byref(a), _lib.stream_ptr(dev))
+        del ws
+        return (None, None, *grads)
+
+
+def sh_residual_norm(x, y, weight, bias, *, eps=1e-5, path_p=0.0, path_group=1, channel_p=0.0, rng=None, call=None):
+    """The residual add of an EquiformerV2 block with the norm behind it: ``h = x + dropout(y)`` and z, the
+    equivariant RMS norm of h (degree-balanced mean square over coefficients and channels, the l = 0 row
+    centred over the channels, ``weight`` [lmax + 1, C] per degree, ``bias`` [C] on l = 0).  Returns (h, z).
+
+    x, y [V, (lmax + 1)^2, C] of one type, lmax <= 6, C <= 512.  path_p: one draw for each ``path_group``
+    consecutive nodes (the nodes of a system); channel_p: one for each (node, channel), shared by the
+    coefficients.  With a rate the call takes two call numbers, ``call`` and ``call`` + 1."""
+    t1, t2 = _threshold(path_p), _threshold(channel_p)
+    code = _dtype(x, "x")
+    if x.dim() != 3 or x.shape != y.shape or x.dtype != y.dtype:
+        raise ValueError(f"x {x.dtype} {list(x.shape)} and y {y.dtype} {list(y.shape)} must be one [V, (lmax + 1)^2, C]")
+    V, S, C = x.shape
+    lmax = round(max(S, 1) ** 0.5) - 1
+    if (lmax + 1) ** 2 != S or lmax > 6 or not 1 <= C <= 512:
+        raise ValueError(f"need (lmax + 1)^2 coefficients with lmax <= 6 and 1 <= C <= 512, got {S} and {C}")
+    if weight.shape != (lmax + 1, C) or bias.shape != (C,):
+        raise ValueError(f"weight must be [{lmax + 1}, {C}] and bias [{C}], got {list(weight.shape)} and {list(bias.shape)}")
+    cp = _dtype(weight, "weight")
+    if bias.dtype != weight.dtype or cp not in (_lib.F32, code):
+        raise TypeError(f"weight and bias must both be float32 or both {x.dtype}")
+    if int(path_group) < 1:
+        raise ValueError(f"path_group must be at least 1, got {path_group}")
+    dev = _device(x, y, weight, bias)
+    state = None
+    if t1 or t2:
+        state, call = _draws(rng, call, 2, dev)
+    if V == 0:
+        return x.clone(), y.clone()
+    x, y, weight, bias = x.contiguous(), y.contiguous(), weight.contiguous(), bias.contiguous()
+    how = (V, int(path_group), lmax, C, code, cp, float(eps), t1, t2, call or 0)
+    if _wants_grad(x, y, weight, bias):
+        return _ShResidualNormFn.apply(how, state, x, y, weight, bias)
+    return _sh_forward(how, x, y, weight, bias, state, None, None)
+
+
+# ---------------------------------------------------------------------------------------------- segment attention
+def _attention_args(how, ptr, eid, values, logits):
+    V, E, K, H, D, cv, cl, threshold, call = how
+    a = _lib.SegmentAttentionArgs(V, E, K, H, D, cv, cl, threshold, call)
+    a.ptr, a.eid, a.values, a.logits = _ptr(ptr), _ptr(eid), _ptr(values), _ptr(logits)
+    return a
+
+
+def _attention_forward(how, values, logits, ptr, eid, state, used, stats):
+    dev = values.device
+    V, _, K, H, D = how[:5]
+    out = torch.empty(V, K, H, D, dtype=values.dtype, device=dev)
+    a = _attention_args(how, ptr, eid, values, logits)
+    a.rng, a.used, a.out, a.stats = _ptr(state), _ptr(used), out.data_ptr(), _ptr(stats)
+    with _on(dev):
+        ws = _workspace("nbx_segment_attention_workspace_bytes", a, dev, 0)
+        _call("nbx_segment_attention", ctypes.byref(a), _lib.stream_ptr(dev))
+    del ws
+    return out
+
+
+class _SegmentAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, how, state, values, logits, ptr, eid):
+        dev = values.device
+        used = torch.empty(2, dtype=torch.int64, device=dev) if state is not None else None
+        stats = torch.empty(2, how[0], how[3], dtype=_f32, device=dev)
+        out = _attention_forward(how, values, logits, ptr, eid, state, used, stats)
+        ctx.save_for_backward(values, logits, ptr, eid, used, stats)
+        ctx.how = how
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        values, logits, ptr, eid, used, stats = ctx.saved_tensors
+        dev = values.device
+        dout = dout.contiguous()
+        a = _attention_args(ctx.how, ptr, eid, values, logits)
+        dv = torch.empty_like(values) if ctx.needs_input_grad[2] else None
+        dl = torch.empty_like(logits) if ctx.needs_input_grad[3] else None
+        a.rng, a.stats, a.dout, a.dvalues, a.dlogits = _ptr(used), stats.data_ptr(), dout.data_ptr(), _ptr(dv), _ptr(dl)
+        with _on(dev):
+            ws = _workspace("nbx_segment_attention_workspace_bytes", a, dev, 1)
+            _call("nbx_segment_attention_backward", ctypes.byref(a), _lib.stream_ptr(dev))
+        del ws
+        return None, None, dv, dl, None, None
+
+
+def segment_attention(values, logits, ptr, eid, *, p=0.0, rng=None, call=None):
+    """Attention over the edges into each node: ``out[v] = sum over v's edges of dropout(a[e, h]) values[e, :, h]``
+    with a the softmax of the edges' ``logits`` over v's list.  Returns [V, K, H, D].
+
+    values [E, K, H, D] (K rows per edge that share the heads' weights), logits [E, H] float32 or of values'
+    type; ptr int32 [V + 1] and eid int32 [E]: the edges by destination, eid a permutation of the edges
+    (``segnn_train.Graph``'s dptr / deid).  A node without edges, or whose logits are all -inf, gets 0; edges
+    in no list (positions from ptr[V] on) get gradients of 0.  A weight that is exactly 0 reads nothing of its
+    value.  H <= 64 and H D <= 4096 (1024 if D is no multiple of 4)."""
+    threshold = _threshold(p)
+    cv, cl = _dtype(values, "values"), _dtype(logits, "logits")
+    if values.dim() != 4 or logits.shape != (values.shape[0], values.shape[2]):
+        raise ValueError(f"values must be [E, K, H, D] and logits [E, H], got {list(values.shape)} and {list(logits.shape)}")
+    E, K, H, D = values.shape
+    if cl not in (_lib.F32, cv):
+        raise TypeError(f"logits must be float32 or {values.dtype}, got {logits.dtype}")
+    if ptr.dtype != torch.int32 or eid.dtype != torch.int32 or ptr.dim() != 1 or ptr.numel() < 1 or eid.shape != (E,):
+        raise ValueError(f"ptr must be int32 [V + 1] and eid int32 [{E}], got {ptr.dtype} {list(ptr.shape)} and "
+                         f"{eid.dtype} {list(eid.shape)}")
+    dev = _device(values, logits, ptr, eid)
+    state = None
+    if threshold:
+        state, call = _draws(rng, call, 1, dev)
+    how = (ptr.numel() - 1, E, K, H, D, cv, cl, threshold, call or 0)
+    values, logits, ptr, eid = values.contiguous(), logits.contiguous(), ptr.contiguous(), eid.contiguous()
+    if _wants_grad(values, logits):
+        return _SegmentAttentionFn.apply(how, state, values, logits, ptr, eid)
+    return _attention_forward(how, values, logits, ptr, eid, state, None, None)

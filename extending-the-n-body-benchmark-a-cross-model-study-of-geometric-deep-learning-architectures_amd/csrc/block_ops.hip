@@ -1,0 +1,888 @@
+// Block operators (include/nbx.h "Block operators"): what surrounds the products of a training block —
+//   * dropout whose mask is never stored (drawn again from the counter in the backward pass);
+//   * the residual add with the norms before and after it, the gate (layer scale) and dropout;
+//   * the same with EquiformerV2's spherical-harmonics norm.
+// All three are bound by HBM: each element is read and written once per direction, everything else
+// (statistics, draws, gate) happens in registers between the two.  A row lives in the registers of the 16
+// or 64 lanes or of the block that owns it, eight consecutive columns per lane, so the norm's two passes
+// (mean, then squares around it) cost no second read.  Column sums (parameter gradients) stay in registers
+// over a block's rows, then one partial row per block is summed by a second launch in a fixed order.
+#include <algorithm>
+
+#include "nbx_internal.h"
+#include "philox.h"
+#include "typed_io.h"
+
+namespace {
+
+using namespace nbx;
+
+bool dtype_ok(int32_t d) { return d == NBX_F32 || d == NBX_BF16 || d == NBX_F16; }
+
+// a launch's threads along x fit 32 bits
+bool grid_ok(int64_t blocks, int threads) { return blocks * threads < ((int64_t)1 << 32); }
+
+// f(T{}) with T the storage type of a dtype code
+template <typename F>
+int with_type(int32_t d, F&& f) {
+    if (d == NBX_F32) return f(float{});
+    if (d == NBX_BF16) return f(bf16{});
+    return f(f16{});
+}
+
+__device__ __forceinline__ void note_used(int64_t* used, const int64_t* rng) {
+    if (used && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+        used[0] = rng[0];
+        used[1] = rng[1];
+    }
+}
+
+// ======================================================================== dropout
+// Flat form: thread t owns elements 8 t .. 8 t + 7, which are exactly one Philox block's draws.
+template <typename T>
+__global__ __launch_bounds__(256) void dropout_flat_kernel(int64_t total, uint32_t threshold, float scale,
+                                                           const int64_t* __restrict__ rng, uint32_t call,
+                                                           int64_t* __restrict__ used, const T* __restrict__ X,
+                                                           T* __restrict__ Y) {
+    note_used(used, rng);
+    const int64_t q = blockIdx.x * (int64_t)256 + threadIdx.x;
+    if (8 * q >= total) return;
+    const int n = (int)std::min<int64_t>(8, total - 8 * q);
+    float v[8];
+    load8n(X + 8 * q, n, v);
+    const uint32_t m = keep_bits(draw_key(rng, call), (uint64_t)q, threshold);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (m >> i & 1) ? v[i] * scale : 0.f;
+    store8n(Y + 8 * q, n, v);
+}
+
+// Row form (entries of S C elements sharing draws): a block takes 256 chunks of eight elements, of one
+// entry or of several.  CHANNEL keeps the entry's mask as bits in LDS, one Philox block for eight channels,
+// shared by the S rows.
+template <typename T, bool CHANNEL>
+__global__ __launch_bounds__(256) void dropout_rows_kernel(int64_t n, int64_t RS, int64_t C, int64_t group, int cpr,
+                                                           int rpb, int64_t segs, uint32_t threshold, float scale,
+                                                           const int64_t* __restrict__ rng, uint32_t call,
+                                                           int64_t* __restrict__ used, const T* __restrict__ X,
+                                                           T* __restrict__ Y) {
+    extern __shared__ uint8_t mask[];
+    note_used(used, rng);
+    const DrawKey key = draw_key(rng, call);
+    const int64_t row0 = blockIdx.x / segs * rpb, seg = blockIdx.x % segs;
+    const int64_t Cq = (C + 7) >> 3;
+    if (CHANNEL) {
+        const int64_t rows = std::min<int64_t>(rpb, n - row0);
+        for (int64_t k = threadIdx.x; k < rows * Cq; k += 256)
+            mask[k] = (uint8_t)keep_bits(key, (uint64_t)(row0 * Cq + k), threshold);
+        __syncthreads();
+    }
+    const int lr = rpb > 1 ? (int)threadIdx.x / cpr : 0;
+    const int64_t row = row0 + lr, f0 = 8 * (rpb > 1 ? (int64_t)(threadIdx.x - lr * cpr) : seg * 256 + threadIdx.x);
+    if (lr >= rpb || row >= n || f0 >= RS) return;
+    const int cnt = (int)std::min<int64_t>(8, RS - f0);
+    const int64_t at = row * RS + f0;
+    float v[8];
+    load8n(X + at, cnt, v);
+    if (CHANNEL) {
+        const uint8_t* mk = mask + lr * Cq;
+        int64_t c = f0 % C;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] = (mk[c >> 3] >> (c & 7) & 1) ? v[i] * scale : 0.f;
+            c = c + 1 == C ? 0 : c + 1;
+        }
+    } else {
+        const bool keep = keep_one(key, (uint64_t)(row / group), threshold);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = keep ? v[i] * scale : 0.f;
+    }
+    store8n(Y + at, cnt, v);
+}
+
+// ======================================================================== residual add, norms, gate
+// Sum over the threads of a row: 16 or 64 lanes, or (W = 0) the whole block through LDS.  `slot` alternates
+// over four places so that one barrier per sum is enough.
+template <int W>
+__device__ __forceinline__ float row_sum(float x, float (*red)[16], int& slot) {
+    if constexpr (W != 0) {
+        return lanes_sum<W>(x);
+    } else {
+        x = lanes_sum<64>(x);
+        float* r = red[slot];
+        slot = (slot + 1) & 3;
+        if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = x;
+        __syncthreads();
+        float s = 0.f;
+        for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += r[i];
+        return s;
+    }
+}
+
+// mean (0 for the RMS norm) and 1/sqrt(mean square around it + eps) of the row's n of eight columns here
+template <int W>
+__device__ __forceinline__ void row_stats(const float (&v)[8], int n, int C, int rms, float eps, float& mu, float& rs,
+                                          float (*red)[16], int& slot) {
+    mu = 0.f;
+    if (!rms) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[i];   // columns past the row are 0
+        mu = row_sum<W>(s, red, slot) / (float)C;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float d = i < n ? v[i] - mu : 0.f;
+        q += d * d;
+    }
+    rs = 1.0f / sqrtf(row_sum<W>(q, red, slot) / (float)C + eps);
+}
+
+struct Draws {
+    DrawKey key;
+    uint32_t threshold;
+    int64_t group, Cq;
+    float scale;
+};
+
+// the keep bits of a row's eight columns at 8 lane
+__device__ __forceinline__ uint32_t row_keep(const Draws& d, int64_t row, int lane) {
+    if (d.threshold == 0) return 0xFFu;
+    if (d.group) return keep_one(d.key, (uint64_t)(row / d.group), d.threshold) ? 0xFFu : 0u;
+    return keep_bits(d.key, (uint64_t)(row * d.Cq + lane), d.threshold);
+}
+
+// Forward: one row per 16 / 64 lanes or per block.
+template <typename TX, typename TY, int W>
+__global__ __launch_bounds__(W ? 256 : 1024) void residual_norm_kernel(nbx_residual_norm_args a, float keep) {
+    __shared__ float red[4][16];
+    int slot = 0;
+    if (a.threshold) note_used(a.used, a.rng);
+    const int lane = W ? (int)threadIdx.x % (W ? W : 1) : (int)threadIdx.x;
+    const int64_t r = W ? blockIdx.x * (int64_t)(256 / (W ? W : 1)) + threadIdx.x / (W ? W : 1) : blockIdx.x;
+    if (r >= a.rows) return;   // W = 0: never (one block per row); else whole lane groups
+    const int C = (int)a.C, c0 = 8 * lane, n = std::max(0, std::min(8, C - c0));
+    Draws d = {{0, 0, 0, 0}, a.threshold, a.group, (a.C + 7) >> 3, keep};
+    if (a.threshold) d.key = draw_key(a.rng, a.call);
+    float x[8], u[8], w[8], b[8];
+    load8n((const TX*)a.x + r * a.ldx + c0, n, x);
+    load8n((const TY*)a.y + r * a.ldy + c0, n, u);
+    const uint32_t m = row_keep(d, r, lane);
+    if (a.post_w) {
+        float mu, rs;
+        row_stats<W>(u, n, C, a.norm, a.eps, mu, rs, red, slot);
+        load8p(a.post_w, a.param_dtype, c0, n, w);
+        if (a.post_b) load8p(a.post_b, a.param_dtype, c0, n, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = (u[i] - mu) * rs * w[i] + (a.post_b ? b[i] : 0.f);
+        if (a.stats && lane == 0) {
+            a.stats[r] = mu;
+            a.stats[a.rows + r] = rs;
+        }
+    }
+    if (a.gate) {
+        load8p(a.gate, a.param_dtype, (a.gate_groups == a.rows ? r : r / (a.rows / a.gate_groups)) * a.C + c0, n, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] *= w[i];
+    }
+    const float s = a.scale * keep;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] += (m >> i & 1) ? s * u[i] : 0.f;
+    store8n((TX*)a.h + r * a.C + c0, n, x);
+    if (a.pre_w) {
+        // z is the norm of the sum before h is rounded to its type: one rounding per result
+        float mu, rs;
+        row_stats<W>(x, n, C, a.norm, a.eps, mu, rs, red, slot);
+        load8p(a.pre_w, a.param_dtype, c0, n, w);
+        if (a.pre_b) load8p(a.pre_b, a.param_dtype, c0, n, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (x[i] - mu) * rs * w[i] + (a.pre_b ? b[i] : 0.f);
+        store8n((TY*)a.z + r * a.C + c0, n, x);
+        if (a.stats && lane == 0) {
+            a.stats[2 * a.rows + r] = mu;
+            a.stats[3 * a.rows + r] = rs;
+        }
+    }
+}
+
+// Which rows a block of the backward pass owns.  ALIGNED: rows [g rpg + k cs, ..) of gate group g, k = block
+// % cpg: a group's gate gradient is the sum of its cpg partial rows.  WHOLE (groups shorter than a block's
+// share): every row slot owns gps whole groups and writes their gate gradients itself.
+struct RowPlan {
+    int64_t rpg, cs, cpg, gps, nblocks;
+    int whole, W, rpb, threads;
+};
+
+RowPlan row_plan(int64_t rows, int64_t C, int64_t gate_groups) {
+    RowPlan p = {};
+    p.W = C <= 128 ? 16 : C <= 512 ? 64 : 0;
+    p.threads = p.W ? 256 : (int)(ceil_div(C, 512) * 64);
+    p.rpb = p.W ? 256 / p.W : 1;
+    const int64_t groups = gate_groups > 0 && gate_groups < rows ? gate_groups : 1;
+    p.rpg = rows / groups;
+    const int64_t chunk = std::max<int64_t>(4 * p.rpb, ceil_div(rows, 1024));
+    p.whole = p.rpg < chunk && groups > 1;
+    if (p.whole) {
+        p.gps = std::max<int64_t>(1, chunk / p.rpb / p.rpg);
+        p.nblocks = ceil_div(ceil_div(groups, p.gps), p.rpb);
+        p.cpg = 1;
+    } else {
+        p.cpg = ceil_div(p.rpg, chunk);
+        p.cs = ceil_div(p.rpg, p.cpg);
+        p.nblocks = groups * p.cpg;
+    }
+    return p;
+}
+
+enum { SUM_POST_W, SUM_POST_B, SUM_PRE_W, SUM_PRE_B, SUM_GATE, SUMS };
+
+template <typename TX, typename TY, int W>
+__global__ __launch_bounds__(W ? 256 : 1024) void residual_norm_bwd_kernel(nbx_residual_norm_args a, RowPlan p,
+                                                                           float keep, float* __restrict__ part) {
+    __shared__ float red[4][16];
+    __shared__ float comb[W ? 2048 : 1];
+    int slot = 0;
+    constexpr int RPB = W ? 256 / (W ? W : 1) : 1;
+    const int lane = W ? (int)threadIdx.x % (W ? W : 1) : (int)threadIdx.x;
+    const int mine = W ? (int)threadIdx.x / (W ? W : 1) : 0;
+    const int C = (int)a.C, c0 = 8 * lane, n = std::max(0, std::min(8, C - c0));
+    Draws d = {{0, 0, 0, 0}, a.threshold, a.group, (a.C + 7) >> 3, keep};
+    if (a.threshold) d.key = draw_key(a.rng, a.call);
+    const float s = a.scale * keep, invC = 1.0f / (float)C;
+    const bool rowgate = a.gate && a.gate_groups == a.rows && a.rows > 1;
+    const bool gsum = a.dgate && !rowgate;
+    float acc[SUMS][8] = {};
+    float pw[8], pb[8] = {}, qw[8], gt[8];
+    if (a.post_w) load8p(a.post_w, a.param_dtype, c0, n, pw);
+    if (a.post_b) load8p(a.post_b, a.param_dtype, c0, n, pb);
+    if (a.pre_w) load8p(a.pre_w, a.param_dtype, c0, n, qw);
+    int64_t g0, g1, r0, r1, step;
+    const int64_t groups = a.gate && !rowgate ? a.gate_groups : 1;
+    if (p.whole) {
+        const int64_t unit = blockIdx.x * (int64_t)RPB + mine;
+        g0 = std::min(unit * p.gps, groups);
+        g1 = std::min(g0 + p.gps, groups);
+        r0 = 0;
+        r1 = p.rpg;
+        step = 1;
+    } else {
+        g0 = blockIdx.x / p.cpg;
+        g1 = g0 + 1;
+        r0 = blockIdx.x % p.cpg * p.cs;
+        r1 = std::min(r0 + p.cs, p.rpg);
+        r0 += mine;
+        step = RPB;
+    }
+    for (int64_t g = g0; g < g1; ++g) {
+        if (a.gate && !rowgate) load8p(a.gate, a.param_dtype, g * a.C + c0, n, gt);
+        for (int64_t rr = r0; rr < r1; rr += step) {
+            const int64_t r = g * p.rpg + rr;
+            float t[8], v[8], e[8];
+            if (a.dh) load8n((const TX*)a.dh + r * a.C + c0, n, t);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] = 0.f;
+            if (a.pre_w && a.dz) {
+                load8n((const TY*)a.dz + r * a.C + c0, n, e);
+                load8n((const TX*)a.h + r * a.C + c0, n, v);
+                const float mu = a.stats[2 * a.rows + r], rs = a.stats[3 * a.rows + r];
+                float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    v[i] = (v[i] - mu) * rs;   // from h as it is stored
+                    acc[SUM_PRE_W][i] += e[i] * v[i];
+                    acc[SUM_PRE_B][i] += e[i];
+                    e[i] = i < n ? e[i] * qw[i] : 0.f;
+                    s1 += e[i];
+                    s2 += e[i] * v[i];
+                }
+                s1 = a.norm ? 0.f : row_sum<W>(s1, red, slot) * invC;
+                s2 = row_sum<W>(s2, red, slot) * invC;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] += rs * (e[i] - s1 - v[i] * s2);
+            }
+            if (a.dx) store8n((TX*)a.dx + r * a.C + c0, n, t);
+            const uint32_t m = row_keep(d, r, lane);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = (m >> i & 1) ? s * t[i] : 0.f;
+            float mu = 0.f, rs = 1.f;
+            if (a.post_w || a.dgate) {
+                load8n((const TY*)a.y + r * a.ldy + c0, n, v);
+                if (a.post_w) {
+                    mu = a.stats[r];
+                    rs = a.stats[a.rows + r];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = (v[i] - mu) * rs;
+            }
+            if (a.gate) {
+                if (rowgate) load8p(a.gate, a.param_dtype, r * a.C + c0, n, gt);
+                if (a.dgate) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float u = a.post_w ? v[i] * pw[i] + pb[i] : v[i];
+                        e[i] = (m >> i & 1) ? t[i] * u : 0.f;   // a dropped place counts 0 whatever it held
+                        acc[SUM_GATE][i] += e[i];
+                    }
+                    if (rowgate) store8p(a.dgate, a.param_dtype, r * a.C + c0, n, e);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] *= gt[i];
+            }
+            if (a.post_w) {
+                float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    acc[SUM_POST_W][i] += t[i] * v[i];
+                    acc[SUM_POST_B][i] += t[i];
+                    t[i] = i < n ? t[i] * pw[i] : 0.f;
+                    s1 += t[i];
+                    s2 += t[i] * v[i];
+                }
+                s1 = a.norm ? 0.f : row_sum<W>(s1, red, slot) * invC;
+                s2 = row_sum<W>(s2, red, slot) * invC;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] = rs * (t[i] - s1 - v[i] * s2);
+            }
+            if (a.dy) store8n((TY*)a.dy + r * a.C + c0, n, t);
+        }
+        if (gsum && p.whole) {
+            store8p(a.dgate, a.param_dtype, g * a.C + c0, n, acc[SUM_GATE]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[SUM_GATE][i] = 0.f;
+        }
+    }
+    // one partial row per block and sum: part[sum][block][C]
+#pragma unroll
+    for (int k = 0; k < SUMS; ++k) {
+        const bool want = k == SUM_POST_W ? a.dpost_w != nullptr : k == SUM_POST_B ? a.dpost_b != nullptr
+                        : k == SUM_PRE_W ? a.dpre_w != nullptr : k == SUM_PRE_B ? a.dpre_b != nullptr
+                        : gsum && !p.whole;
+        if (!want) continue;
+        float* to = part + ((int64_t)k * p.nblocks + blockIdx.x) * a.C;
+        if constexpr (W == 0) {
+            store8n(to + c0, n, acc[k]);
+        } else {
+            __syncthreads();
+            store8(comb + mine * 8 * W + c0, acc[k]);
+            __syncthreads();
+            for (int c = threadIdx.x; c < C; c += 256) {
+                float t = 0.f;
+#pragma unroll 4
+                for (int q = 0; q < RPB; ++q) t += comb[q * 8 * W + c];
+                to[c] = t;
+            }
+        }
+    }
+}
+
+// Column sums of the partial rows: job j < 4: a parameter gradient over all blocks; job 4 + g: gate group g
+// over its cpg blocks.  64 columns x 16 waves, each wave every 16th row, combined in order.
+struct FinalSums {
+    void* out[SUMS];
+    int dtype, jobs;
+    int job[SUMS];
+};
+
+__global__ __launch_bounds__(1024) void residual_norm_sums_kernel(FinalSums f, int64_t nblocks, int64_t cpg, int64_t C,
+                                                                  const float* __restrict__ part) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t c = blockIdx.x * (int64_t)64 + lane;
+    const int k = (int)blockIdx.y < f.jobs ? f.job[blockIdx.y] : SUM_GATE;
+    const int64_t g = (int)blockIdx.y < f.jobs ? 0 : blockIdx.y - f.jobs;
+    const int64_t b0 = k == SUM_GATE ? g * cpg : 0, nb = k == SUM_GATE ? cpg : nblocks;
+    const float* p = part + ((int64_t)k * nblocks + b0) * C + c;
+    float s = 0.f;
+    if (c < C)
+        for (int64_t b = w; b < nb; b += 16) s += p[b * C];
+    red[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && c < C) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += red[i][lane];
+        store1p(f.out[k], f.dtype, g * C + c, t);
+    }
+}
+
+int residual_check(const nbx_residual_norm_args* a, const char* who) {
+    NBX_CHECK_ARG(a, "%s: null arguments", who);
+    NBX_CHECK_ARG(a->rows >= 0 && a->rows < ((int64_t)1 << 31), "%s: need 0 <= rows < 2^31", who);
+    NBX_CHECK_ARG(a->C >= 1 && a->C <= 8192, "%s: need 1 <= C <= 8192", who);
+    NBX_CHECK_ARG(dtype_ok(a->x_dtype) && dtype_ok(a->y_dtype) && (a->x_dtype == a->y_dtype || a->x_dtype == NBX_F32),
+                  "%s: x_dtype must be y_dtype or fp32", who);
+    NBX_CHECK_ARG(a->param_dtype == NBX_F32 || a->param_dtype == a->y_dtype, "%s: param_dtype must be fp32 or y_dtype",
+                  who);
+    NBX_CHECK_ARG(a->norm == 0 || a->norm == 1, "%s: unknown norm %d", who, a->norm);
+    NBX_CHECK_ARG(a->threshold < 65536 && a->group >= 0, "%s: need threshold < 65536, group >= 0", who);
+    NBX_CHECK_ARG(!a->threshold || a->rng, "%s: a drop rate needs rng", who);
+    NBX_CHECK_ARG(!a->gate || (a->gate_groups >= 1 && (a->rows == 0 || a->rows % a->gate_groups == 0)),
+                  "%s: gate_groups must divide rows", who);
+    NBX_CHECK_ARG(a->ldy >= a->C && a->ldx >= a->C, "%s: row strides are shorter than the rows", who);
+    NBX_CHECK_ARG((!a->post_b || a->post_w) && (!a->pre_b || a->pre_w), "%s: a norm's bias needs its weight", who);
+    return NBX_OK;
+}
+
+// f(TX{}, TY{}) for the storage types
+template <typename F>
+int with_types(const nbx_residual_norm_args& a, F&& f) {
+    return with_type(a.y_dtype, [&](auto y) {
+        using TY = decltype(y);
+        if (a.x_dtype == a.y_dtype) return f(TY{}, TY{});
+        return f(float{}, TY{});
+    });
+}
+
+// ======================================================================== residual add, spherical-harmonics norm
+// A node's (lmax+1)^2 C values sit in the registers of TPN threads: 64 (four nodes per block) or the block;
+// thread t keeps chunks t, t + TPN, .. of eight consecutive values (NJ of them).
+constexpr int SH_MAXC = 512;
+
+struct ShPlan {
+    int S, RL, tpn, nj, npb, threads;   // npb: nodes in flight per block
+};
+
+ShPlan sh_plan(int lmax, int C) {
+    ShPlan p = {};
+    p.S = (lmax + 1) * (lmax + 1);
+    p.RL = p.S * C;
+    const int chunks = (p.RL + 7) / 8;
+    if (chunks <= 128) {
+        p.tpn = 64;
+        p.nj = chunks <= 64 ? 1 : 2;
+        p.npb = 4;
+        p.threads = 256;
+    } else {
+        p.nj = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : 4;
+        p.tpn = p.threads = (int)ceil_div(ceil_div(chunks, p.nj), 64) * 64;
+        p.npb = 1;
+    }
+    return p;
+}
+
+__device__ __forceinline__ int degree_of(int i) {
+    return (i >= 1) + (i >= 4) + (i >= 9) + (i >= 16) + (i >= 25) + (i >= 36);
+}
+
+// coefficient and channel of eight consecutive values starting at f0
+struct ShAt {
+    int i[8], c[8];
+};
+__device__ __forceinline__ ShAt sh_at(int f0, int C) {
+    ShAt s;
+    int i = f0 / C, c = f0 - i * C;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        s.i[e] = i;
+        s.c[e] = c;
+        if (++c == C) {
+            c = 0;
+            ++i;
+        }
+    }
+    return s;
+}
+
+template <bool SUB>
+__device__ __forceinline__ float node_sum(float x, float (*red)[16], int& slot) {
+    return row_sum<SUB ? 64 : 0>(x, red, slot);
+}
+
+// the factors of a node's dropout: path (whole node) and the channel bits in LDS
+__device__ __forceinline__ void sh_channel_bits(const nbx_sh_residual_norm_args& a, int64_t node, bool live, int t,
+                                                int tpn, uint8_t* bits) {
+    if (!a.channel_threshold) return;
+    const int Cq = (a.C + 7) >> 3;
+    const DrawKey key = draw_key(a.rng, a.call + 1);
+    if (live)
+        for (int k = t; k < Cq; k += tpn) bits[k] = (uint8_t)keep_bits(key, (uint64_t)(node * Cq + k), a.channel_threshold);
+}
+
+template <typename T, int NJ, bool SUB>
+__global__ __launch_bounds__(SUB ? 256 : 1024) void sh_residual_norm_kernel(nbx_sh_residual_norm_args a, ShPlan p,
+                                                                            float k1, float k2) {
+    __shared__ float red[4][16];
+    __shared__ uint8_t bits[SUB ? 4 : 1][SH_MAXC / 8];
+    int slot = 0;
+    if (a.path_threshold | a.channel_threshold) note_used(a.used, a.rng);
+    const int t = SUB ? (int)threadIdx.x & 63 : (int)threadIdx.x, sub = SUB ? (int)threadIdx.x >> 6 : 0;
+    const int64_t v = SUB ? blockIdx.x * (int64_t)4 + sub : blockIdx.x;
+    const bool live = v < a.V;
+    sh_channel_bits(a, v, live, t, p.tpn, bits[sub]);
+    __syncthreads();
+    if (!live) return;   // SUB: whole waves, no barrier below
+    const bool path = !a.path_threshold || keep_one(draw_key(a.rng, a.call), (uint64_t)(v / a.path_group), a.path_threshold);
+    const float k = (a.path_threshold ? k1 : 1.f) * (a.channel_threshold ? k2 : 1.f);
+    const int C = a.C;
+    float h[NJ][8];
+    float s0 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int f0 = 8 * (t + p.tpn * j), n = std::max(0, std::min(8, p.RL - f0));
+        const int64_t at = v * p.RL + f0;
+        float y[8];
+        load8n((const T*)a.x + at, n, h[j]);
+        load8n((const T*)a.y + at, n, y);
+        const ShAt q = sh_at(f0, C);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool on = path && (!a.channel_threshold || (e < n && (bits[sub][q.c[e] >> 3] >> (q.c[e] & 7) & 1)));
+            h[j][e] += on ? k * y[e] : 0.f;
+            if (f0 + e < C) s0 += h[j][e];
+        }
+        store8n((T*)a.h + at, n, h[j]);
+    }
+    const float m0 = node_sum<SUB>(s0, red, slot) / (float)C;
+    float qs = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int f0 = 8 * (t + p.tpn * j), n = std::max(0, std::min(8, p.RL - f0));
+        const ShAt q = sh_at(f0, C);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (f0 + e < C) h[j][e] -= m0;
+            const int l = degree_of(q.i[e]);
+            if (e < n) qs += h[j][e] * h[j][e] / (float)((2 * l + 1) * (a.lmax + 1));
+        }
+    }
+    const float rs = 1.0f / sqrtf(node_sum<SUB>(qs, red, slot) / (float)C + a.eps);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int f0 = 8 * (t + p.tpn * j), n = std::max(0, std::min(8, p.RL - f0));
+        const ShAt q = sh_at(f0, C);
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            z[e] = 0.f;
+            if (e < n) {
+                float w[8], b[8];
+                load8p(a.weight, a.param_dtype, degree_of(q.i[e]) * C + q.c[e], 1, w);
+                z[e] = h[j][e] * rs * w[0];
+                if (f0 + e < C) {
+                    load8p(a.bias, a.param_dtype, q.c[e], 1, b);
+                    z[e] += b[0];
+                }
+            }
+        }
+        store8n((T*)a.z + v * p.RL + f0, n, z);
+    }
+    if (a.stats && t == 0) {
+        a.stats[v] = m0;
+        a.stats[a.V + v] = rs;
+    }
+}
+
+// Backward over nodes [unit, unit + nunits, ..) with the column sums per coefficient and channel in
+// registers: part[unit][S C + C] = (sum over nodes of dz hc rs | of dz's l = 0 row).
+template <typename T, int NJ, bool SUB>
+__global__ __launch_bounds__(SUB ? 256 : 1024) void sh_residual_norm_bwd_kernel(nbx_sh_residual_norm_args a, ShPlan p,
+                                                                                float k1, float k2, int64_t nunits,
+                                                                                float* __restrict__ part) {
+    __shared__ float red[4][16];
+    __shared__ uint8_t bits[2][SUB ? 4 : 1][SH_MAXC / 8];
+    int slot = 0, flip = 0;
+    const int t = SUB ? (int)threadIdx.x & 63 : (int)threadIdx.x, sub = SUB ? (int)threadIdx.x >> 6 : 0;
+    const int64_t unit = SUB ? blockIdx.x * (int64_t)4 + sub : blockIdx.x;
+    const float k = (a.path_threshold ? k1 : 1.f) * (a.channel_threshold ? k2 : 1.f);
+    const int C = a.C;
+    float aw[NJ][8] = {}, ab[8] = {};
+    const int64_t iters = (a.V + nunits - 1) / nunits;
+    for (int64_t it = 0; it < iters; ++it) {
+        const int64_t v = it * nunits + unit;
+        const bool live = v < a.V;
+        sh_channel_bits(a, v, live, t, p.tpn, bits[flip][sub]);
+        __syncthreads();   // two copies of the bits: the next node's are written before this one's last read
+        const uint8_t* bt = bits[flip][sub];
+        flip ^= 1;
+        if (SUB && !live) continue;
+        if (!live) break;   // W = 0: the whole block
+        const bool path = !a.path_threshold || keep_one(draw_key(a.rng, a.call), (uint64_t)(v / a.path_group), a.path_threshold);
+        const float m0 = a.stats[v], rs = a.stats[a.V + v];
+        float g[NJ][8], hc[NJ][8];
+        float dot = 0.f, sg = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int f0 = 8 * (t + p.tpn * j), n = std::max(0, std::min(8, p.RL - f0));
+            const int64_t at = v * p.RL + f0;
+            const ShAt q = sh_at(f0, C);
+            if (a.dz) {
+                load8n((const T*)a.dz + at, n, g[j]);
+                load8n((const T*)a.h + at, n, hc[j]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[j][e] = hc[j][e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (f0 + e < C) {
+                    hc[j][e] -= m0;
+                    if (j == 0) ab[e] += g[j][e];
+                }
+                aw[j][e] += g[j][e] * hc[j][e] * rs;
+                if (e < n) {
+                    float w[8];
+                    load8p(a.weight, a.param_dtype, degree_of(q.i[e]) * C + q.c[e], 1, w);
+                    g[j][e] *= w[0];
+                    dot += g[j][e] * hc[j][e];
+                    if (f0 + e < C) sg += g[j][e];
+                }
+            }
+        }
+        dot = node_sum<SUB>(dot, red, slot);
+        sg = node_sum<SUB>(sg, red, slot);
+        const float coef = rs * rs * rs / (float)C * dot;
+        const float dm = rs * sg / (float)C;   // the centred row sums to 0, so only g is left of its mean
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int f0 = 8 * (t + p.tpn * j), n = std::max(0, std::min(8, p.RL - f0));
+            const int64_t at = v * p.RL + f0;
+            const ShAt q = sh_at(f0, C);
+            float dh[8];
+            if (a.dh) load8n((const T*)a.dh + at, n, dh);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float bal = 1.0f / (float)((2 * degree_of(q.i[e]) + 1) * (a.lmax + 1));
+                float d = rs * g[j][e] - coef * bal * hc[j][e] - (f0 + e < C ? dm : 0.f);
+                if (a.dh) d += dh[e];
+                g[j][e] = d;
+                const bool on = path && (!a.channel_threshold || (e < n && (bt[q.c[e] >> 3] >> (q.c[e] & 7) & 1)));
+                hc[j][e] = on ? k * d : 0.f;
+            }
+            if (a.dx) store8n((T*)a.dx + at, n, g[j]);
+            if (a.dy) store8n((T*)a.dy + at, n, hc[j]);
+        }
+    }
+    if (!part) return;
+    float* to = part + unit * (p.RL + C);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int f0 = 8 * (t + p.tpn * j);
+        store8n(to + f0, std::max(0, std::min(8, p.RL - f0)), aw[j]);
+        if (j == 0) store8n(to + p.RL + f0, std::max(0, std::min(8, C - f0)), ab);
+    }
+}
+
+// dweight [lmax+1][C] | dbias [C] from the units' partial sums: 64 columns x 16 waves in a fixed order
+__global__ __launch_bounds__(1024) void sh_residual_sums_kernel(nbx_sh_residual_norm_args a, int RL, int64_t nunits,
+                                                                const float* __restrict__ part) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int c = blockIdx.x * 64 + lane, l = blockIdx.y, C = a.C;   // l = lmax + 1: the bias
+    const int i0 = l <= a.lmax ? l * l : 0, ni = l <= a.lmax ? 2 * l + 1 : 1;
+    const int64_t ld = RL + C;
+    const float* p = part + (l <= a.lmax ? i0 * C : RL) + c;
+    float s = 0.f;
+    if (c < C)
+        for (int64_t u = w; u < nunits; u += 16)
+            for (int i = 0; i < ni; ++i) s += p[u * ld + i * C];
+    red[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && c < C) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += red[i][lane];
+        if (l <= a.lmax) {
+            if (a.dweight) store1p(a.dweight, a.param_dtype, (int64_t)l * C + c, t);
+        } else if (a.dbias) {
+            store1p(a.dbias, a.param_dtype, c, t);
+        }
+    }
+}
+
+// the units (nodes in flight) of the backward pass: its partial rows are read and written once more
+int64_t sh_units(const ShPlan& p, int64_t V) {
+    const int64_t most = 512 * (int64_t)p.npb;
+    return std::max<int64_t>(1, ceil_div(std::min(most, ceil_div(V, 4)), p.npb)) * p.npb;
+}
+
+int sh_check(const nbx_sh_residual_norm_args* a, const char* who) {
+    NBX_CHECK_ARG(a, "%s: null arguments", who);
+    NBX_CHECK_ARG(a->V >= 0 && a->V < ((int64_t)1 << 31) && a->lmax >= 0 && a->lmax <= 6 && a->C >= 1 && a->C <= SH_MAXC,
+                  "%s: need 0 <= V < 2^31, 0 <= lmax <= 6, 1 <= C <= %d", who, SH_MAXC);
+    NBX_CHECK_ARG(dtype_ok(a->dtype) && (a->param_dtype == NBX_F32 || a->param_dtype == a->dtype),
+                  "%s: param_dtype must be fp32 or dtype", who);
+    NBX_CHECK_ARG(a->path_threshold < 65536 && a->channel_threshold < 65536 && a->path_group >= 1,
+                  "%s: need thresholds < 65536, path_group >= 1", who);
+    NBX_CHECK_ARG(!(a->path_threshold | a->channel_threshold) || a->rng, "%s: a drop rate needs rng", who);
+    NBX_CHECK_ARG(a->V == 0 || a->weight, "%s: null weight", who);
+    return NBX_OK;
+}
+
+template <bool BWD, typename T>
+int sh_launch(const nbx_sh_residual_norm_args& a, const ShPlan& p, int64_t units, float* part, hipStream_t st) {
+    const float k1 = keep_scale(a.path_threshold), k2 = keep_scale(a.channel_threshold);
+    const unsigned blocks = (unsigned)ceil_div(BWD ? units : a.V, p.npb);
+    auto go = [&](auto fwd, auto bwd) {
+        if constexpr (BWD)
+            hipLaunchKernelGGL(bwd, dim3(blocks), dim3(p.threads), 0, st, a, p, k1, k2, units, part);
+        else
+            hipLaunchKernelGGL(fwd, dim3(blocks), dim3(p.threads), 0, st, a, p, k1, k2);
+    };
+    if (p.npb == 4) {
+        if (p.nj == 1) go(sh_residual_norm_kernel<T, 1, true>, sh_residual_norm_bwd_kernel<T, 1, true>);
+        else go(sh_residual_norm_kernel<T, 2, true>, sh_residual_norm_bwd_kernel<T, 2, true>);
+    } else {
+        if (p.nj == 1) go(sh_residual_norm_kernel<T, 1, false>, sh_residual_norm_bwd_kernel<T, 1, false>);
+        else if (p.nj == 2) go(sh_residual_norm_kernel<T, 2, false>, sh_residual_norm_bwd_kernel<T, 2, false>);
+        else go(sh_residual_norm_kernel<T, 4, false>, sh_residual_norm_bwd_kernel<T, 4, false>);
+    }
+    return NBX_OK;
+}
+
+}  // namespace
+
+// ======================================================================== C ABI (include/nbx.h)
+extern "C" int nbx_dropout(int32_t dtype, int32_t per, int64_t n, int64_t S, int64_t C, int64_t group,
+                           uint32_t threshold, const int64_t* rng, uint32_t call, int64_t* used, const void* X, void* Y,
+                           void* stream) {
+    NBX_CHECK_ARG(dtype_ok(dtype), "nbx_dropout: unknown dtype %d", dtype);
+    NBX_CHECK_ARG(per >= NBX_DROP_ELEMENT && per <= NBX_DROP_CHANNEL, "nbx_dropout: unknown mode %d", per);
+    NBX_CHECK_ARG(n >= 0 && S >= 0 && C >= 0 && group >= 1, "nbx_dropout: bad sizes");
+    NBX_CHECK_ARG(threshold < 65536, "nbx_dropout: need threshold < 65536");
+    if (n == 0 || S == 0 || C == 0) return NBX_OK;
+    const int64_t limit = (int64_t)1 << 40;
+    NBX_CHECK_ARG(n <= limit && S <= limit / n && C <= limit / (n * S), "nbx_dropout: need n S C <= 2^40");
+    NBX_CHECK_ARG(X && Y && rng, "nbx_dropout: null operand");
+    hipStream_t st = (hipStream_t)stream;
+    const float scale = keep_scale(threshold);
+    const int64_t total = n * S * C, RS = S * C;
+    return with_type(dtype, [&](auto tag) -> int {
+        using T = decltype(tag);
+        if (per == NBX_DROP_ELEMENT) {
+            const int64_t blocks = ceil_div(total, 2048);
+            NBX_CHECK_ARG(grid_ok(blocks, 256), "nbx_dropout: too many elements");
+            hipLaunchKernelGGL(dropout_flat_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, total, threshold, scale,
+                               rng, call, used, (const T*)X, (T*)Y);
+        } else {
+            const bool channel = per == NBX_DROP_CHANNEL;
+            const int64_t chunks = ceil_div(RS, 8), Cq = ceil_div(C, 8);
+            NBX_CHECK_ARG(!channel || Cq <= 65536, "nbx_dropout: need C <= 2^19 for one draw per channel");
+            int rpb = chunks <= 128 ? (int)(256 / chunks) : 1;
+            const int64_t segs = rpb > 1 ? 1 : ceil_div(chunks, 256), blocks = ceil_div(n, rpb) * segs;
+            NBX_CHECK_ARG(grid_ok(blocks, 256), "nbx_dropout: too many elements");
+            const int cpr = rpb > 1 ? (int)chunks : 256;
+            if (channel)
+                hipLaunchKernelGGL((dropout_rows_kernel<T, true>), dim3((unsigned)blocks), dim3(256),
+                                   (size_t)(rpb * Cq), st, n, RS, C, group, cpr, rpb, segs, threshold, scale, rng, call,
+                                   used, (const T*)X, (T*)Y);
+            else
+                hipLaunchKernelGGL((dropout_rows_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, st, n, RS, C,
+                                   group, cpr, rpb, segs, threshold, scale, rng, call, used, (const T*)X, (T*)Y);
+        }
+        NBX_LAUNCH_CHECK("dropout");
+        return NBX_OK;
+    });
+}
+
+extern "C" int nbx_residual_norm(const nbx_residual_norm_args* a, void* stream) {
+    if (int rc = residual_check(a, "nbx_residual_norm")) return rc;
+    if (a->rows == 0) return NBX_OK;
+    NBX_CHECK_ARG(a->x && a->y && a->h && (!a->pre_w || a->z), "nbx_residual_norm: null operand");
+    const RowPlan p = row_plan(a->rows, a->C, 0);
+    NBX_CHECK_ARG(grid_ok(ceil_div(a->rows, p.rpb), p.threads), "nbx_residual_norm: too many rows");
+    const unsigned blocks = (unsigned)ceil_div(a->rows, p.rpb);
+    const float keep = keep_scale(a->threshold);
+    return with_types(*a, [&](auto x, auto y) -> int {
+        using TX = decltype(x);
+        using TY = decltype(y);
+        auto k = p.W == 16 ? residual_norm_kernel<TX, TY, 16> : p.W == 64 ? residual_norm_kernel<TX, TY, 64>
+                                                                          : residual_norm_kernel<TX, TY, 0>;
+        hipLaunchKernelGGL(k, dim3(blocks), dim3(p.threads), 0, (hipStream_t)stream, *a, keep);
+        NBX_LAUNCH_CHECK("residual_norm");
+        return NBX_OK;
+    });
+}
+
+extern "C" int nbx_residual_norm_backward_workspace_bytes(const nbx_residual_norm_args* a, size_t* bytes) {
+    if (int rc = residual_check(a, "nbx_residual_norm_backward_workspace_bytes")) return rc;
+    NBX_CHECK_ARG(bytes, "nbx_residual_norm_backward_workspace_bytes: null result");
+    *bytes = a->rows ? (size_t)SUMS * row_plan(a->rows, a->C, a->gate ? a->gate_groups : 0).nblocks * a->C * sizeof(float)
+                     : 0;
+    return NBX_OK;
+}
+
+extern "C" int nbx_residual_norm_backward(const nbx_residual_norm_args* a, void* stream) {
+    if (int rc = residual_check(a, "nbx_residual_norm_backward")) return rc;
+    NBX_CHECK_ARG(a->rows >= 1, "nbx_residual_norm_backward: need a row");
+    NBX_CHECK_ARG((!a->post_w && !a->dgate) || a->y, "nbx_residual_norm_backward: null y");
+    NBX_CHECK_ARG(!a->pre_w || !a->dz || a->h, "nbx_residual_norm_backward: null h");
+    NBX_CHECK_ARG((!a->pre_w && !a->post_w) || a->stats, "nbx_residual_norm_backward: null stats");
+    NBX_CHECK_ARG((!a->dgate || a->gate) && ((!a->dpost_w && !a->dpost_b) || a->post_w) &&
+                      ((!a->dpre_w && !a->dpre_b) || a->pre_w),
+                  "nbx_residual_norm_backward: a gradient of a parameter that is not there");
+    const int64_t rows = a->rows, C = a->C;
+    const RowPlan p = row_plan(rows, C, a->gate ? a->gate_groups : 0);
+    const size_t need = (size_t)SUMS * p.nblocks * C * sizeof(float);
+    if (!(a->workspace && a->workspace_bytes >= need)) {
+        set_error("nbx_residual_norm_backward: workspace too small");
+        return NBX_E_WORKSPACE;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    const float keep = keep_scale(a->threshold);
+    float* part = (float*)a->workspace;
+    if (int rc = with_types(*a, [&](auto x, auto y) -> int {
+            using TX = decltype(x);
+            using TY = decltype(y);
+            auto k = p.W == 16 ? residual_norm_bwd_kernel<TX, TY, 16>
+                   : p.W == 64 ? residual_norm_bwd_kernel<TX, TY, 64> : residual_norm_bwd_kernel<TX, TY, 0>;
+            hipLaunchKernelGGL(k, dim3((unsigned)p.nblocks), dim3(p.threads), 0, st, *a, p, keep, part);
+            NBX_LAUNCH_CHECK("residual_norm_bwd");
+            return NBX_OK;
+        }))
+        return rc;
+    FinalSums f = {{a->dpost_w, a->dpost_b, a->dpre_w, a->dpre_b, a->dgate}, a->param_dtype, 0, {}};
+    for (int k = 0; k < SUM_GATE; ++k)
+        if (f.out[k]) f.job[f.jobs++] = k;
+    const bool rowgate = a->gate && a->gate_groups == rows && rows > 1;
+    const int64_t jobs = f.jobs + (a->dgate && !rowgate && !p.whole ? a->gate_groups : 0);
+    if (jobs) {
+        hipLaunchKernelGGL(residual_norm_sums_kernel, dim3((unsigned)ceil_div(C, 64), (unsigned)jobs), dim3(1024), 0, st,
+                           f, p.nblocks, p.cpg, C, part);
+        NBX_LAUNCH_CHECK("residual_norm_sums");
+    }
+    return NBX_OK;
+}
+
+extern "C" int nbx_sh_residual_norm(const nbx_sh_residual_norm_args* a, void* stream) {
+    if (int rc = sh_check(a, "nbx_sh_residual_norm")) return rc;
+    if (a->V == 0) return NBX_OK;
+    NBX_CHECK_ARG(a->x && a->y && a->bias && a->h && a->z, "nbx_sh_residual_norm: null operand");
+    const ShPlan p = sh_plan(a->lmax, a->C);
+    NBX_CHECK_ARG(grid_ok(ceil_div(a->V, p.npb), p.threads), "nbx_sh_residual_norm: too many nodes");
+    if (int rc = with_type(a->dtype, [&](auto t) { return sh_launch<false, decltype(t)>(*a, p, 0, nullptr, (hipStream_t)stream); }))
+        return rc;
+    NBX_LAUNCH_CHECK("sh_residual_norm");
+    return NBX_OK;
+}
+
+extern "C" int nbx_sh_residual_norm_backward_workspace_bytes(const nbx_sh_residual_norm_args* a, size_t* bytes) {
+    if (int rc = sh_check(a, "nbx_sh_residual_norm_backward_workspace_bytes")) return rc;
+    NBX_CHECK_ARG(bytes, "nbx_sh_residual_norm_backward_workspace_bytes: null result");
+    const ShPlan p = sh_plan(a->lmax, a->C);
+    *bytes = a->V ? (size_t)sh_units(p, a->V) * (p.RL + a->C) * sizeof(float) : 0;
+    return NBX_OK;
+}
+
+extern "C" int nbx_sh_residual_norm_backward(const nbx_sh_residual_norm_args* a, void* stream) {
+    if (int rc = sh_check(a, "nbx_sh_residual_norm_backward")) return rc;
+    NBX_CHECK_ARG(a->V >= 1, "nbx_sh_residual_norm_backward: need a node");
+    NBX_CHECK_ARG(a->stats && (!a->dz || a->h), "nbx_sh_residual_norm_backward: null operand");
+    const ShPlan p = sh_plan(a->lmax, a->C);
+    const int64_t units = sh_units(p, a->V);
+    const bool sums = a->dweight || a->dbias;
+    if (sums && !(a->workspace && a->workspace_bytes >= (size_t)units * (p.RL + a->C) * sizeof(float))) {
+        set_error("nbx_sh_residual_norm_backward: workspace too small");
+        return NBX_E_WORKSPACE;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    float* part = sums ? (float*)a->workspace : nullptr;
+    if (int rc = with_type(a->dtype, [&](auto t) { return sh_launch<true, decltype(t)>(*a, p, units, part, st); })) return rc;
+    NBX_LAUNCH_CHECK("sh_residual_norm_bwd");
+    if (sums) {
+        hipLaunchKernelGGL(sh_residual_sums_kernel, dim3((unsigned)ceil_div(a->C, 64), (unsigned)(a->lmax + 2)), dim3(1024),
+                           0, st, *a, p.RL, units, part);
+        NBX_LAUNCH_CHECK("sh_residual_sums");
+    }
+    return NBX_OK;
+}

@@ -1,0 +1,607 @@
+// Attention over the edges into a node (include/nbx.h "Block operators"): softmax of the edges' logits,
+// dropout of the weights (drawn from the counter, never stored), weighted sum of the edges' values, and the
+// backward pass.  Bound by HBM: every value is read once per direction; logits, weights and the CSR are a
+// few words per edge and stay in LDS.
+//   * list form: a block per (node, slice of the row) walks the node's list with a running maximum and sum;
+//   * chunk form, for long lists: a block per 64 positions of the CSR, whatever nodes they belong to; a list
+//     that crosses a chunk's border leaves partial sums with their own maximum, joined by a second launch.
+// Backward: a block per few positions (dvalues and the weights' gradient), then the softmax's own gradient
+// per list.
+#include <algorithm>
+#include <type_traits>
+
+#include "nbx_internal.h"
+#include "philox.h"
+#include "typed_io.h"
+
+namespace {
+
+using namespace nbx;
+
+constexpr int TILE = 64;      // positions whose weights are in LDS at once
+constexpr int SA_MAXH = 64;
+
+template <typename T, int VW>
+struct VecT {
+    typedef T type __attribute__((ext_vector_type(VW), aligned(sizeof(T))));
+};
+template <typename T, int VW>
+__device__ __forceinline__ void loadv(const T* p, float (&v)[VW]) {
+    if constexpr (VW == 1) {
+        v[0] = (float)p[0];
+    } else {
+        const typename VecT<T, VW>::type t = *reinterpret_cast<const typename VecT<T, VW>::type*>(p);
+#pragma unroll
+        for (int i = 0; i < VW; ++i) v[i] = (float)t[i];
+    }
+}
+template <typename T, int VW>
+__device__ __forceinline__ void storev(T* p, const float (&v)[VW]) {
+    if constexpr (VW == 1) {
+        p[0] = (T)v[0];
+    } else {
+        typename VecT<T, VW>::type t;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) t[i] = (T)v[i];
+        *reinterpret_cast<typename VecT<T, VW>::type*>(p) = t;
+    }
+}
+
+__device__ __forceinline__ float load_logit(const nbx_segment_attention_args& a, int64_t at) {
+    return a.l_dtype == NBX_F32 ? ((const float*)a.logits)[at]
+         : a.l_dtype == NBX_BF16 ? (float)((const bf16*)a.logits)[at] : (float)((const f16*)a.logits)[at];
+}
+
+__device__ __forceinline__ void store_dlogit(const nbx_segment_attention_args& a, int64_t at, float d) {
+    if (a.l_dtype == NBX_F32) ((float*)a.dlogits)[at] = d;
+    else if (a.l_dtype == NBX_BF16) ((bf16*)a.dlogits)[at] = (bf16)d;
+    else ((f16*)a.dlogits)[at] = (f16)d;
+}
+
+// exp(l - m) with m the finite maximum (0 for a list that is all -inf)
+__device__ __forceinline__ float weight_of(float l, float m) { return l == -INFINITY ? 0.f : __expf(l - m); }
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+struct SaPlan {
+    int T, RV, EL, slices;    // threads, vectors per row, edges side by side, blocks per row
+    int eb, TP, grp;          // backward: positions per block, threads that work, lanes of a head that shuffle
+    int chunked;
+    int64_t nc;               // chunks
+};
+
+__device__ __forceinline__ void note_used(const nbx_segment_attention_args& a) {
+    if (a.used && a.threshold && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+        a.used[0] = a.rng[0];
+        a.used[1] = a.rng[1];
+    }
+}
+
+// the node whose list holds position p: the last v with ptr[v] <= p
+__device__ __forceinline__ int node_of(const int32_t* ptr, int64_t V, int p) {
+    int64_t lo = 0, hi = V;
+    while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (ptr[mid] <= p) lo = mid;
+        else hi = mid;
+    }
+    return (int)lo;
+}
+
+// Sum over the EL groups of RV threads (thread = el RV + f), left in group 0.
+template <int VW>
+__device__ __forceinline__ void join_groups(float (&acc)[VW], float* red, int RV, int EL) {
+    const int t = threadIdx.x;
+    __syncthreads();
+    if (t < RV * EL)
+#pragma unroll
+        for (int i = 0; i < VW; ++i) red[t * VW + i] = acc[i];
+    __syncthreads();
+    if (t < RV)
+        for (int g = 1; g < EL; ++g)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) acc[i] += red[(g * RV + t) * VW + i];
+}
+
+// ======================================================================== forward, list form
+template <typename T, int VW>
+__global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment_attention_args a, SaPlan p, float keep) {
+    extern __shared__ float lds[];
+    const int H = a.H, t = threadIdx.x;
+    float* sW = lds;                       // [TILE][H] logits, then weights
+    float* sP = sW + TILE * H;             // [TILE][H] exp(l - m)
+    float* sM = sP + TILE * H;             // [H] running maximum
+    float* sR = sM + H;                    // [H] factor of what is summed so far
+    float* sS = sR + H;                    // [H] running sum
+    float* red = sS + H;                   // [T VW]
+    int* sE = reinterpret_cast<int*>(red + p.T * VW);   // [TILE]
+    note_used(a);
+    const DrawKey key = a.threshold ? draw_key(a.rng, a.call) : DrawKey{0, 0, 0, 0};
+    const int64_t v = blockIdx.x;
+    const int j0 = std::max(0, a.ptr[v]), j1 = (int)std::min<int64_t>(a.E, a.ptr[v + 1]);
+    const int el = p.slices > 1 ? 0 : t / p.RV;
+    const int f = p.slices > 1 ? (int)blockIdx.y * p.T + t : t - el * p.RV;
+    const bool on = el < p.EL && f < p.RV;
+    const int head = on ? (f * VW / a.D) % H : 0;
+    const int64_t RL = (int64_t)p.RV * VW;
+    float acc[VW] = {};
+    if (t < H) {
+        sM[t] = -INFINITY;
+        sS[t] = 0.f;
+    }
+    for (int b = j0; b < j1; b += TILE) {
+        const int cnt = std::min(TILE, j1 - b);
+        __syncthreads();
+        for (int i = t; i < cnt; i += p.T) {
+            const int e = a.eid[b + i];
+            sE[i] = e >= 0 && e < a.E ? e : -1;
+        }
+        __syncthreads();
+        for (int i = t; i < cnt * H; i += p.T) {
+            const int e = sE[i / H];
+            sW[i] = e < 0 ? -INFINITY : load_logit(a, (int64_t)e * H + i % H);
+        }
+        __syncthreads();
+        if (t < H) {
+            float m = sM[t];
+            for (int i = 0; i < cnt; ++i) m = fmaxf(m, sW[i * H + t]);
+            sR[t] = sM[t] == -INFINITY ? 0.f : __expf(sM[t] - m);
+            sM[t] = m;
+        }
+        __syncthreads();
+        for (int i = t; i < cnt * H; i += p.T) {
+            const float w = weight_of(sW[i], finite_max(sM[i % H]));
+            sP[i] = w;
+            sW[i] = !a.threshold || keep_one(key, (uint64_t)(int64_t)sE[i / H] * H + i % H, a.threshold) ? w : 0.f;
+        }
+        __syncthreads();
+        if (t < H) {
+            float s = sS[t] * sR[t];
+            for (int i = 0; i < cnt; ++i) s += sP[i * H + t];
+            sS[t] = s;
+        }
+        if (on) {
+            const float r = sR[head];
+#pragma unroll
+            for (int k = 0; k < VW; ++k) acc[k] *= r;
+#pragma unroll 4
+            for (int i = el; i < cnt; i += p.EL) {
+                const float w = sW[i * H + head];
+                if (w != 0.f) {
+                    float x[VW];
+                    loadv<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW, x);
+#pragma unroll
+                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, x[k], acc[k]);
+                }
+            }
+        }
+    }
+    if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
+    else __syncthreads();
+    if (on && el == 0) {
+        const float inv = keep / (sS[head] + 1e-16f);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) acc[k] = sS[head] == 0.f ? 0.f : acc[k] * inv;
+        storev<T, VW>((T*)a.out + v * RL + (int64_t)f * VW, acc);
+    }
+    if (a.stats && blockIdx.y == 0 && t < H) {
+        a.stats[v * H + t] = finite_max(sM[t]);
+        a.stats[(a.V + v) * H + t] = 1.0f / (sS[t] + 1e-16f);
+    }
+}
+
+// ======================================================================== forward, chunk form
+// partial sums of the lists that cross chunk c's borders: slot 2 c = the list that began before it, slot
+// 2 c + 1 = the list that begins in it and goes on: acc [2 nc][RL] unnormalised, ms [2 nc][2][H] (max, sum)
+template <typename T, int VW>
+__global__ __launch_bounds__(256) void segment_attention_chunk_kernel(nbx_segment_attention_args a, SaPlan p, float keep,
+                                                                      float* __restrict__ pacc, float* __restrict__ pms) {
+    extern __shared__ float lds[];
+    const int H = a.H, t = threadIdx.x;
+    float* sW = lds;
+    float* sM = sW + TILE * H;             // [TILE][H]: of the list that begins at the position
+    float* sS = sM + TILE * H;
+    float* red = sS + TILE * H;
+    int* sE = reinterpret_cast<int*>(red + p.T * VW);
+    int* sV = sE + TILE;
+    note_used(a);
+    const DrawKey key = a.threshold ? draw_key(a.rng, a.call) : DrawKey{0, 0, 0, 0};
+    const int64_t c = blockIdx.x;
+    const int p0 = (int)(c * TILE), cnt = (int)std::min<int64_t>(TILE, a.E - c * TILE);
+    if (t < cnt) {
+        const int e = a.eid[p0 + t];
+        sE[t] = e >= 0 && e < a.E ? e : -1;
+        const int v = node_of(a.ptr, a.V, p0 + t);
+        sV[t] = p0 + t >= a.ptr[v] && p0 + t < a.ptr[v + 1] ? v : -1;   // -1: in no list
+    }
+    __syncthreads();
+    for (int i = t; i < cnt * H; i += p.T) {
+        const int e = sE[i / H];
+        sW[i] = e < 0 ? -INFINITY : load_logit(a, (int64_t)e * H + i % H);
+    }
+    __syncthreads();
+    for (int k = t; k < cnt * H; k += p.T) {
+        const int i0 = k / H, h = k % H;
+        if (i0 && sV[i0] == sV[i0 - 1]) continue;
+        int i1 = i0;
+        float m = -INFINITY, s = 0.f;
+        for (; i1 < cnt && sV[i1] == sV[i0]; ++i1) m = fmaxf(m, sW[i1 * H + h]);
+        for (int i = i0; i < i1; ++i) {
+            const float w = weight_of(sW[i * H + h], finite_max(m));
+            s += w;
+            sW[i * H + h] = !a.threshold || keep_one(key, (uint64_t)(int64_t)sE[i] * H + h, a.threshold) ? w : 0.f;
+        }
+        sM[k] = m;
+        sS[k] = s;
+    }
+    __syncthreads();
+    const int el = p.slices > 1 ? 0 : t / p.RV;
+    const int f = p.slices > 1 ? (int)blockIdx.y * p.T + t : t - el * p.RV;
+    const bool on = el < p.EL && f < p.RV;
+    const int head = on ? (f * VW / a.D) % H : 0;
+    const int64_t RL = (int64_t)p.RV * VW;
+    for (int i0 = 0; i0 < cnt;) {
+        int i1 = i0 + 1;
+        while (i1 < cnt && sV[i1] == sV[i0]) ++i1;
+        const int v = sV[i0];
+        if (v < 0) {
+            i0 = i1;
+            continue;
+        }
+        float acc[VW] = {};
+        if (on)
+#pragma unroll 4
+            for (int i = i0 + el; i < i1; i += p.EL) {
+                const float w = sW[i * H + head];
+                if (w != 0.f) {
+                    float x[VW];
+                    loadv<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW, x);
+#pragma unroll
+                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, x[k], acc[k]);
+                }
+            }
+        if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
+        const bool before = a.ptr[v] < p0, after = a.ptr[v + 1] > p0 + cnt;
+        if (before || after) {
+            const int64_t slot = 2 * c + (before ? 0 : 1);
+            if (on && el == 0)
+#pragma unroll
+                for (int k = 0; k < VW; ++k) pacc[slot * RL + (int64_t)f * VW + k] = acc[k];
+            if (blockIdx.y == 0 && t < H) {
+                pms[(slot * 2) * H + t] = sM[i0 * H + t];
+                pms[(slot * 2 + 1) * H + t] = sS[i0 * H + t];
+            }
+        } else {
+            if (on && el == 0) {
+                const float s = sS[i0 * H + head], inv = keep / (s + 1e-16f);
+#pragma unroll
+                for (int k = 0; k < VW; ++k) acc[k] = s == 0.f ? 0.f : acc[k] * inv;
+                storev<T, VW>((T*)a.out + v * RL + (int64_t)f * VW, acc);
+            }
+            if (a.stats && blockIdx.y == 0 && t < H) {
+                a.stats[(int64_t)v * H + t] = finite_max(sM[i0 * H + t]);
+                a.stats[(a.V + v) * H + t] = 1.0f / (sS[i0 * H + t] + 1e-16f);
+            }
+        }
+        i0 = i1;
+    }
+}
+
+// joins the partial sums of a list over its chunks; an empty list gives 0
+template <typename T, int VW>
+__global__ __launch_bounds__(256) void segment_attention_join_kernel(nbx_segment_attention_args a, SaPlan p, float keep,
+                                                                     const float* __restrict__ pacc,
+                                                                     const float* __restrict__ pms) {
+    const int64_t v = blockIdx.x;
+    const int t = threadIdx.x, H = a.H;
+    const int j0 = std::max(0, a.ptr[v]), j1 = (int)std::min<int64_t>(a.E, a.ptr[v + 1]);
+    const int64_t c0 = j0 / TILE, c1 = j1 > j0 ? (j1 - 1) / TILE : c0;
+    if (j1 > j0 && c0 == c1) return;
+    const bool empty = j1 <= j0;
+    const int64_t RL = (int64_t)p.RV * VW;
+    auto slot = [&](int64_t c) { return 2 * c + (j0 < c * TILE ? 0 : 1); };
+    auto top = [&](int h) {
+        float m = -INFINITY;
+        if (!empty)
+            for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, pms[slot(c) * 2 * H + h]);
+        return m;
+    };
+    const int f = blockIdx.y * p.T + t;
+    if (f < p.RV) {
+        const int h = (f * VW / a.D) % H;
+        const float m = finite_max(top(h));
+        float acc[VW] = {}, s = 0.f;
+        if (!empty)
+            for (int64_t c = c0; c <= c1; ++c) {
+                const int64_t k = slot(c);
+                const float r = weight_of(pms[k * 2 * H + h], m);
+                s += r * pms[(k * 2 + 1) * H + h];
+                if (r != 0.f)
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) acc[i] += r * pacc[k * RL + (int64_t)f * VW + i];
+            }
+        const float inv = keep / (s + 1e-16f);
+#pragma unroll
+        for (int i = 0; i < VW; ++i) acc[i] = s == 0.f ? 0.f : acc[i] * inv;
+        storev<T, VW>((T*)a.out + v * RL + (int64_t)f * VW, acc);
+    }
+    if (a.stats && blockIdx.y == 0 && t < H) {
+        const float m = finite_max(top(t));
+        float s = 0.f;
+        if (!empty)
+            for (int64_t c = c0; c <= c1; ++c) s += weight_of(pms[slot(c) * 2 * H + t], m) * pms[(slot(c) * 2 + 1) * H + t];
+        a.stats[v * H + t] = m;
+        a.stats[(a.V + v) * H + t] = 1.0f / (s + 1e-16f);
+    }
+}
+
+// ======================================================================== backward
+// Positions [eb block, ..): dvalues = w dout[v], dp[position][h] = keep/(1-p) <dout[v], values>_h.
+// Threads: EL groups of RV, or (long rows) TP threads, a multiple of the H D / VW columns, over the row in
+// steps of TP: either way a thread stays with one head.
+template <typename T, int VW>
+__global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment_attention_args a, SaPlan p, float keep,
+                                                                     float* __restrict__ dp) {
+    extern __shared__ float lds[];
+    const int H = a.H, t = threadIdx.x;
+    float* sA = lds;                       // [eb][H] alpha
+    float* sK = sA + p.eb * H;             // [eb][H] keep / (1 - p) or 0
+    float* red = sK + p.eb * H;            // [T]
+    int* sE = reinterpret_cast<int*>(red + p.T);
+    int* sV = sE + p.eb;
+    const DrawKey key = a.threshold ? draw_key(a.rng, a.call) : DrawKey{0, 0, 0, 0};
+    const int64_t p0 = blockIdx.x * (int64_t)p.eb;
+    const int cnt = (int)std::min<int64_t>(p.eb, a.E - p0);
+    for (int i = t; i < cnt; i += p.T) {
+        const int e = a.eid[p0 + i], v = node_of(a.ptr, a.V, (int)p0 + i);
+        sE[i] = e >= 0 && e < a.E ? e : -1;
+        sV[i] = p0 + i >= a.ptr[v] && p0 + i < a.ptr[v + 1] ? v : -1;   // -1: in no list, its gradients are 0
+    }
+    __syncthreads();
+    for (int i = t; i < cnt * H; i += p.T) {
+        const int e = sE[i / H], h = i % H;
+        const int64_t v = sV[i / H];
+        float al = 0.f, k = 0.f;
+        if (e >= 0 && v < 0 && a.dlogits) store_dlogit(a, (int64_t)e * H + h, 0.f);
+        if (e >= 0 && v >= 0) {
+            al = weight_of(load_logit(a, (int64_t)e * H + h), a.stats[v * H + h]) * a.stats[(a.V + v) * H + h];
+            k = !a.threshold || keep_one(key, (uint64_t)(int64_t)e * H + h, a.threshold) ? keep : 0.f;
+        }
+        sA[i] = al;
+        sK[i] = k;
+    }
+    __syncthreads();
+    const bool wide = p.RV > p.T;          // one edge at a time, several vectors a thread
+    const int cols = H * a.D / VW, el = wide ? 0 : t / p.RV, f0 = wide ? t : t - el * p.RV;
+    const bool on = wide ? t < p.TP : el < p.EL;
+    const int head = on ? (f0 * VW / a.D) % H : 0;
+    const int64_t RL = (int64_t)p.RV * VW;
+    const int per = a.D / VW / p.grp;      // entries of a head and coefficient row in red
+    for (int i0 = 0; i0 < cnt; i0 += p.EL) {
+        const int i = i0 + el;
+        float s = 0.f;
+        if (on && i < cnt && sE[i] >= 0) {
+            const float w = sA[i * H + head] * sK[i * H + head];
+            for (int f = f0; f < p.RV; f += wide ? p.TP : p.RV) {
+                float d[VW], x[VW];
+                loadv<T, VW>((const T*)a.dout + (int64_t)std::max(0, sV[i]) * RL + (int64_t)f * VW, d);
+                if (w != 0.f && a.dlogits) {
+                    loadv<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW, x);
+#pragma unroll
+                    for (int k = 0; k < VW; ++k) s = fmaf(d[k], x[k], s);
+                }
+                if (a.dvalues) {
+#pragma unroll
+                    for (int k = 0; k < VW; ++k) d[k] = w == 0.f ? 0.f : d[k] * w;
+                    storev<T, VW>((T*)a.dvalues + (int64_t)sE[i] * RL + (int64_t)f * VW, d);
+                }
+            }
+        }
+        if (!a.dlogits) continue;
+        for (int m = p.grp >> 1; m; m >>= 1) s += __shfl_xor(s, m, 64);
+        if (on && t % p.grp == 0) red[t / p.grp] = s;
+        __syncthreads();
+        // red: rows of H per entries; a group (or the whole block) holds its threads' rows of them
+        const int rows = (wide ? p.TP : p.RV) / cols, row_entries = cols / p.grp;
+        for (int k = t; k < p.EL * H; k += p.T) {
+            const int g = k / H, h = k % H;
+            if (i0 + g >= cnt) continue;
+            float sum = 0.f;
+            for (int r = 0; r < rows; ++r)
+                for (int q = 0; q < per; ++q) sum += red[g * (p.RV / p.grp) + r * row_entries + h * per + q];
+            const int j = (i0 + g) * H + h;
+            dp[(p0 + i0 + g) * H + h] = sK[j] * sum;
+        }
+        __syncthreads();
+    }
+}
+
+// dl = a (dp - sum over the list of a dp): `threads` per node, thread = (position, head)
+__global__ __launch_bounds__(1024) void segment_attention_dlogits_kernel(nbx_segment_attention_args a,
+                                                                         const float* __restrict__ dp) {
+    __shared__ float red[1024];
+    const int t = threadIdx.x, T = blockDim.x, H = a.H;
+    const int64_t v = blockIdx.x;
+    const int j0 = std::max(0, a.ptr[v]), j1 = (int)std::min<int64_t>(a.E, a.ptr[v + 1]);
+    if (j1 <= j0) return;
+    const int step = T / H, h = t % H, r = t / H;
+    const bool on = r < step;
+    const float m = a.stats[v * H + h], inv = a.stats[(a.V + v) * H + h];
+    float s = 0.f;
+    if (on)
+        for (int j = j0 + r; j < j1; j += step) {
+            const int e = a.eid[j];
+            if (e < 0 || e >= a.E) continue;
+            s += weight_of(load_logit(a, (int64_t)e * H + h), m) * inv * dp[(int64_t)j * H + h];
+        }
+    red[t] = s;
+    __syncthreads();
+    if (t < H) {
+        float d = 0.f;
+        for (int i = 0; i < step; ++i) d += red[i * H + t];
+        red[t] = d;   // only this thread reads the entries h = t
+    }
+    __syncthreads();
+    const float delta = red[h];
+    if (on)
+        for (int j = j0 + r; j < j1; j += step) {
+            const int e = a.eid[j];
+            if (e < 0 || e >= a.E) continue;
+            const float al = weight_of(load_logit(a, (int64_t)e * H + h), m) * inv;
+            const float d = al == 0.f ? 0.f : al * (dp[(int64_t)j * H + h] - delta);
+            store_dlogit(a, (int64_t)e * H + h, d);
+        }
+}
+
+// ======================================================================== host
+bool dtype_ok(int32_t d) { return d == NBX_F32 || d == NBX_BF16 || d == NBX_F16; }
+
+int vector_width(const nbx_segment_attention_args& a) {
+    if (a.v_dtype != NBX_F32 && a.D % 8 == 0) return 8;
+    return a.D % 4 == 0 ? 4 : 1;
+}
+
+int sa_check(const nbx_segment_attention_args* a, const char* who) {
+    NBX_CHECK_ARG(a, "%s: null arguments", who);
+    const int64_t lim = (int64_t)1 << 31;
+    NBX_CHECK_ARG(a->V >= 0 && a->V < lim - 1 && a->E >= 0 && a->E < lim - TILE && a->K >= 1 && a->H >= 1 && a->D >= 1,
+                  "%s: bad sizes", who);
+    NBX_CHECK_ARG(dtype_ok(a->v_dtype) && (a->l_dtype == a->v_dtype || a->l_dtype == NBX_F32),
+                  "%s: l_dtype must be fp32 or v_dtype", who);
+    NBX_CHECK_ARG(a->H <= SA_MAXH && a->D <= 4096 && (int64_t)a->H * a->D <= (a->D % 4 == 0 ? 4096 : 1024),
+                  "%s: need H <= %d, H D <= 4096 (1024 if D %% 4)", who, SA_MAXH);
+    NBX_CHECK_ARG(a->K <= (1 << 22) && a->K * a->H * a->D <= (1 << 22), "%s: rows of more than 2^22 values", who);
+    // a launch's threads along x fit 32 bits (blocks of up to 1024 for a node or a position)
+    NBX_CHECK_ARG(a->V < (1 << 22) || (a->V < (1 << 24) && a->E * a->H < 256 * a->V), "%s: too many nodes", who);
+    NBX_CHECK_ARG(a->threshold < 65536 && (!a->threshold || a->rng), "%s: need threshold < 65536, and rng for a drop rate",
+                  who);
+    return NBX_OK;
+}
+
+SaPlan forward_plan(const nbx_segment_attention_args& a) {
+    SaPlan p = {};
+    const int VW = vector_width(a);
+    p.T = 256;
+    p.RV = (int)(a.K * a.H * a.D / VW);
+    p.EL = p.RV <= p.T ? p.T / p.RV : 1;
+    p.slices = p.RV <= p.T ? 1 : (int)ceil_div(p.RV, p.T);
+    p.chunked = a.E >= 32 * a.V;
+    p.nc = ceil_div(a.E, TILE);
+    return p;
+}
+
+SaPlan backward_plan(const nbx_segment_attention_args& a) {
+    SaPlan p = {};
+    const int VW = vector_width(a), cols = a.H * a.D / VW;
+    p.T = std::max(256, (int)ceil_div(cols, 64) * 64);
+    p.RV = (int)(a.K * a.H * a.D / VW);
+    p.EL = p.RV <= p.T ? std::min(p.T / p.RV, TILE) : 1;
+    p.TP = p.RV <= p.T ? p.RV * p.EL : p.T / cols * cols;
+    p.eb = p.RV <= p.T ? std::min(4 * p.EL, TILE) : 4;
+    const int g = a.D / VW;
+    p.grp = g <= 64 && (g & (g - 1)) == 0 ? g : 1;
+    return p;
+}
+
+// f(T{}, std::integral_constant<int, VW>{})
+template <typename F>
+int with_values(const nbx_segment_attention_args& a, F&& f) {
+    const int VW = vector_width(a);
+    auto pick = [&](auto t) -> int {
+        if constexpr (sizeof(t) == 2)
+            if (VW == 8) return f(t, std::integral_constant<int, 8>{});
+        if (VW == 4) return f(t, std::integral_constant<int, 4>{});
+        return f(t, std::integral_constant<int, 1>{});
+    };
+    if (a.v_dtype == NBX_F32) return pick(float{});
+    if (a.v_dtype == NBX_BF16) return pick(bf16{});
+    return pick(f16{});
+}
+
+size_t workspace_need(const nbx_segment_attention_args& a, bool backward) {
+    if (backward) return a.dlogits ? (size_t)a.E * a.H * sizeof(float) : 0;
+    const SaPlan p = forward_plan(a);
+    return p.chunked ? (size_t)2 * p.nc * (a.K * a.H * a.D + 2 * a.H) * sizeof(float) : 0;
+}
+
+}  // namespace
+
+// ======================================================================== C ABI (include/nbx.h)
+extern "C" int nbx_segment_attention_workspace_bytes(const nbx_segment_attention_args* a, int32_t backward,
+                                                     size_t* bytes) {
+    if (int rc = sa_check(a, "nbx_segment_attention_workspace_bytes")) return rc;
+    NBX_CHECK_ARG(bytes, "nbx_segment_attention_workspace_bytes: null result");
+    *bytes = workspace_need(*a, backward != 0);
+    return NBX_OK;
+}
+
+extern "C" int nbx_segment_attention(const nbx_segment_attention_args* a, void* stream) {
+    if (int rc = sa_check(a, "nbx_segment_attention")) return rc;
+    if (a->V == 0) return NBX_OK;
+    NBX_CHECK_ARG(a->ptr && a->out && (a->E == 0 || (a->eid && a->values && a->logits)),
+                  "nbx_segment_attention: null operand");
+    const size_t need = workspace_need(*a, false);
+    if (need && !(a->workspace && a->workspace_bytes >= need)) {
+        set_error("nbx_segment_attention: workspace too small");
+        return NBX_E_WORKSPACE;
+    }
+    const SaPlan p = forward_plan(*a);
+    hipStream_t st = (hipStream_t)stream;
+    const float keep = keep_scale(a->threshold);
+    return with_values(*a, [&](auto t, auto vw) -> int {
+        using T = decltype(t);
+        constexpr int VW = decltype(vw)::value;
+        if (!p.chunked) {
+            const size_t lds = (size_t)(2 * TILE * a->H + 3 * a->H + p.T * VW + TILE) * 4;
+            hipLaunchKernelGGL((segment_attention_list_kernel<T, VW>), dim3((unsigned)a->V, (unsigned)p.slices), dim3(p.T),
+                               lds, st, *a, p, keep);
+            NBX_LAUNCH_CHECK("segment_attention_list");
+            return NBX_OK;
+        }
+        float* pacc = (float*)a->workspace;
+        float* pms = pacc + 2 * p.nc * a->K * a->H * a->D;
+        const size_t lds = (size_t)(3 * TILE * a->H + p.T * VW + 2 * TILE) * 4;
+        NBX_CHECK_ARG(lds <= 64 * 1024, "nbx_segment_attention: too many heads");
+        if (p.nc) {
+            hipLaunchKernelGGL((segment_attention_chunk_kernel<T, VW>), dim3((unsigned)p.nc, (unsigned)p.slices), dim3(p.T),
+                               lds, st, *a, p, keep, pacc, pms);
+            NBX_LAUNCH_CHECK("segment_attention_chunk");
+        }
+        hipLaunchKernelGGL((segment_attention_join_kernel<T, VW>), dim3((unsigned)a->V, (unsigned)p.slices), dim3(p.T), 0,
+                           st, *a, p, keep, pacc, pms);
+        NBX_LAUNCH_CHECK("segment_attention_join");
+        return NBX_OK;
+    });
+}
+
+extern "C" int nbx_segment_attention_backward(const nbx_segment_attention_args* a, void* stream) {
+    if (int rc = sa_check(a, "nbx_segment_attention_backward")) return rc;
+    if (a->V == 0 || a->E == 0 || (!a->dvalues && !a->dlogits)) return NBX_OK;
+    NBX_CHECK_ARG(a->ptr && a->eid && a->values && a->logits && a->stats && a->dout,
+                  "nbx_segment_attention_backward: null operand");
+    const size_t need = workspace_need(*a, true);
+    if (need && !(a->workspace && a->workspace_bytes >= need)) {
+        set_error("nbx_segment_attention_backward: workspace too small");
+        return NBX_E_WORKSPACE;
+    }
+    const SaPlan p = backward_plan(*a);
+    NBX_CHECK_ARG(ceil_div(a->E, p.eb) * p.T < ((int64_t)1 << 32), "nbx_segment_attention_backward: too many edges");
+    hipStream_t st = (hipStream_t)stream;
+    const float keep = keep_scale(a->threshold);
+    float* dp = (float*)a->workspace;
+    if (int rc = with_values(*a, [&](auto t, auto vw) -> int {
+            using T = decltype(t);
+            constexpr int VW = decltype(vw)::value;
+            const size_t lds = (size_t)(2 * p.eb * a->H + p.T + 2 * p.eb) * 4;
+            hipLaunchKernelGGL((segment_attention_bwd_kernel<T, VW>), dim3((unsigned)ceil_div(a->E, p.eb)), dim3(p.T), lds,
+                               st, *a, p, keep, dp);
+            NBX_LAUNCH_CHECK("segment_attention_bwd");
+            return NBX_OK;
+        }))
+        return rc;
+    if (a->dlogits) {
+        const int threads = a->E * a->H >= 256 * a->V ? 1024 : 64;
+        hipLaunchKernelGGL(segment_attention_dlogits_kernel, dim3((unsigned)a->V), dim3(threads), 0, st, *a, dp);
+        NBX_LAUNCH_CHECK("segment_attention_dlogits");
+    }
+    return NBX_OK;
+}

@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define NBX_ABI_VERSION 19
+#define NBX_ABI_VERSION 20
 
 #define NBX_OK 0
 #define NBX_E_INVAL 1      /* bad argument (shape, size, pointer) */
@@ -928,6 +928,115 @@ int nbx_eqv2_rollout(const nbx_eqv2_weights* w, float* pos, float* vel, const fl
  * if an operand of an fp16x2 GEMM left the fp16 range (or an input was not finite).  Synchronises. */
 int nbx_eqv2_range_check(const nbx_eqv2_weights* w, const void* workspace, size_t workspace_bytes, int64_t batch_size,
                          int64_t num_nodes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Block operators (ABI 20): what surrounds the products of a training block.  Activations are fp32, bf16
+ * or fp16 (NBX_F32 / NBX_BF16 / NBX_F16); sums, statistics and draws' factors are fp32, each result is
+ * rounded once.  Every reduction runs in a fixed order (no atomics): calls are bit-reproducible.
+ *
+ * Draws: Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011) of key = seed and counter = (low, high word of
+ * q, call, low word of step); draw d is halfword d % 8 of block q = d / 8 (word (d % 8) / 2, its low half
+ * first).  A draw keeps iff its halfword >= threshold (= the rate p times 65536, rounded; 0: every draw
+ * keeps and rng is not read); what is kept is scaled by 65536 / (65536 - threshold).  `rng` is a device
+ * int64[2] (seed, step), read by the kernel, so a captured graph draws anew once the step is advanced on
+ * the device; `used` (NULL: not written) receives the pair the call drew with, and is the backward
+ * pass's rng.  No mask is stored.  A dropped element is 0 whatever it held.
+ */
+#define NBX_F32 0
+#define NBX_BF16 1
+#define NBX_F16 2
+
+#define NBX_DROP_ELEMENT 0 /* draw = the element's index in x [n][S][C] */
+#define NBX_DROP_GROUP 1   /* one draw for each `group` consecutive entries of the first axis */
+#define NBX_DROP_CHANNEL 2 /* draw = i Cp + c of x[i][s][c], Cp = C rounded up to 8: shared over s */
+
+/* Y = keep X / (1 - p) over contiguous [n][S][C]; its backward is the same call on the gradient. */
+int nbx_dropout(int32_t dtype, int32_t per, int64_t n, int64_t S, int64_t C, int64_t group, uint32_t threshold,
+                const int64_t* rng, uint32_t call, int64_t* used, const void* X, void* Y, void* stream);
+
+/* h = x + scale keep/(1-p) gate u,  u = y or N(y) post_w + post_b,  z = N(h) pre_w + pre_b, N = LayerNorm
+ * (norm 0, biased variance) or RMS norm (norm 1) over the C <= 8192 columns of a row.
+ * x / h / dx / dh in x_dtype, y / z / dy / dz in y_dtype (x_dtype = y_dtype, or x_dtype fp32), gate / post_* /
+ * pre_* and their gradients in param_dtype (fp32 or y_dtype).  post_w NULL: no norm of y; pre_w NULL: no z;
+ * *_b NULL: no bias; gate NULL: none, else [gate_groups][C], one row for each rows / gate_groups consecutive
+ * rows.  Draws: group 0: draw = row Cp + column (Cp = C rounded up to 8); group r > 0: one for each r rows.
+ * stats (fp32 [4][rows]: mean and 1/sqrt(.. + eps) of the y norm, then of the h norm; NULL: not kept) is what
+ * the backward call reads next to y and h.  x and y rows are ldx / ldy elements apart; everything else is
+ * contiguous. */
+typedef struct nbx_residual_norm_args {
+    int64_t rows, C, ldx, ldy, gate_groups, group;
+    int32_t x_dtype, y_dtype, param_dtype, norm;
+    float eps, scale;
+    uint32_t threshold, call;
+    const int64_t* rng;
+    int64_t* used;
+    const void *x, *y, *gate, *post_w, *post_b, *pre_w, *pre_b;
+    void *h, *z;
+    float* stats;
+    /* backward: dh / dz NULL = zero; dx .. dpre_b NULL = not wanted */
+    const void *dh, *dz;
+    void *dx, *dy, *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+    void* workspace;
+    size_t workspace_bytes;
+} nbx_residual_norm_args;
+
+int nbx_residual_norm(const nbx_residual_norm_args* a, void* stream);
+int nbx_residual_norm_backward_workspace_bytes(const nbx_residual_norm_args* a, size_t* bytes);
+int nbx_residual_norm_backward(const nbx_residual_norm_args* a, void* stream);
+
+/* The residual add with the EquiformerV2 norm of nbx_eqv2_rms_norm_general behind it, over [V][(lmax+1)^2][C]
+ * (lmax <= 6, C <= 512): h = x + k1 k2 y, z = norm(h; weight [lmax+1][C], bias [C]).  k1: one draw for each
+ * path_group consecutive nodes (path_threshold, call); k2: one for each (node, channel), draw = node Cp + c
+ * (channel_threshold, call + 1).  x, y, h, z and gradients in dtype, weight / bias in param_dtype (fp32 or
+ * dtype); stats fp32 [2][V] = (l = 0 mean, scale).  All contiguous. */
+typedef struct nbx_sh_residual_norm_args {
+    int64_t V, path_group;
+    int32_t lmax, C, dtype, param_dtype;
+    float eps;
+    uint32_t path_threshold, channel_threshold, call;
+    const int64_t* rng;
+    int64_t* used;
+    const void *x, *y, *weight, *bias;
+    void *h, *z;
+    float* stats;
+    const void *dh, *dz; /* NULL = zero */
+    void *dx, *dy, *dweight, *dbias; /* NULL = not wanted */
+    void* workspace;
+    size_t workspace_bytes;
+} nbx_sh_residual_norm_args;
+
+int nbx_sh_residual_norm(const nbx_sh_residual_norm_args* a, void* stream);
+int nbx_sh_residual_norm_backward_workspace_bytes(const nbx_sh_residual_norm_args* a, size_t* bytes);
+int nbx_sh_residual_norm_backward(const nbx_sh_residual_norm_args* a, void* stream);
+
+/* Attention over the edges into a node: a[e][h] = exp(l[e][h] - max) / (sum + 1e-16) over the edges of the
+ * node's list (ptr [V+1] / eid [E], the CSR of nbx_segment_softmax), w = keep a / (1-p) (draw = e H + h),
+ * out[v][k][h][:] = sum over the list of w[e][h] values[e][k][h][:].  An empty list, or one whose logits are
+ * all -inf, gives 0.  A weight that is exactly 0 (masked, dropped, underflown) reads nothing of its value.
+ * Backward: dvalues, dlogits (NULL: not wanted); eid is a permutation of the edges, and those in no list
+ * (positions from ptr[V] on) get gradients of 0.
+ * values / out in v_dtype, logits in l_dtype (fp32 or v_dtype); H <= 64, H D <= 4096 (1024 if D is no
+ * multiple of 4); stats fp32 [2][V][H] = (max, 1 / sum).  All contiguous.  workspace: forward and backward
+ * ask their own size. */
+typedef struct nbx_segment_attention_args {
+    int64_t V, E, K;
+    int32_t H, D, v_dtype, l_dtype;
+    uint32_t threshold, call;
+    const int64_t* rng;
+    int64_t* used;
+    const int32_t *ptr, *eid;
+    const void *values, *logits;
+    void* out;
+    float* stats;
+    const void* dout;
+    void *dvalues, *dlogits;
+    void* workspace;
+    size_t workspace_bytes;
+} nbx_segment_attention_args;
+
+int nbx_segment_attention_workspace_bytes(const nbx_segment_attention_args* a, int32_t backward, size_t* bytes);
+int nbx_segment_attention(const nbx_segment_attention_args* a, void* stream);
+int nbx_segment_attention_backward(const nbx_segment_attention_args* a, void* stream);
 
 #ifdef __cplusplus
 }
