@@ -22,11 +22,9 @@ Like the framework's other operators these run on the HIP device only.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -118,24 +116,48 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-_SAME = contextlib.nullcontext()
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else _lib.stream_ptr
+_current = torch.cuda.current_device
+_entries = {}
 
 
-def _on(dev):
-    """Launches go to the tensors' device, whichever is current."""
-    return _SAME if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _launch(name, dev, *args):
+    """Calls an entry point on the device's current stream, with that device current."""
+    f = _entries.get(name)
+    if f is None:
+        f = _entries[name] = getattr(_lib.lib(), name)
+    i = dev.index
+    if _current() == i:
+        rc = f(*args, _stream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = f(*args, _stream(i))
+    if rc:
+        _lib.check(rc, name)
 
 
-def _call(name, *args):
-    _lib.check(getattr(_lib.lib(), name)(*args), name)
+_sizes = {}
 
 
-def _workspace(name, args, dev, *more):
-    n = _lib.c_sz()
-    _call(name, ctypes.byref(args), *more, ctypes.byref(n))
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
-    args.workspace, args.workspace_bytes = _ptr(ws), n.value
+def _workspace(name, key, args, dev, *more):
+    """The workspace that a call with these arguments asks for (its size kept per ``key``)."""
+    n = _sizes.get((name, key))
+    if n is None:
+        size = _lib.c_sz()
+        _lib.check(getattr(_lib.lib(), name)(ctypes.byref(args), *more, ctypes.byref(size)), name)
+        if len(_sizes) >= 4096:
+            _sizes.clear()
+        n = _sizes[(name, key)] = size.value
+    if n == 0:
+        return None
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), n
     return ws
+
+
+def _first_derivatives_only():
+    if torch.is_grad_enabled():
+        raise _lib.NbxError("block operators have no second derivatives (a backward pass with create_graph)")
 
 
 def _wants_grad(*tensors):
@@ -147,30 +169,25 @@ def _dense(g):
 
 
 # ---------------------------------------------------------------------------------------------- dropout
-def _dropout(x, mode, dims, threshold, state, call, used):
+def _dropout(x, how, state, used):
     y = torch.empty_like(x)
-    dev = x.device
-    with _on(dev):
-        _call("nbx_dropout", _CODE[x.dtype], mode, *dims, threshold, state.data_ptr(), call, _ptr(used), x.data_ptr(),
-              y.data_ptr(), _lib.stream_ptr(dev))
+    _launch("nbx_dropout", x.device, *how[:-1], state.data_ptr(), how[-1], _ptr(used), x.data_ptr(), y.data_ptr())
     return y
 
 
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, mode, dims, threshold, state, call):
-        used = torch.empty(2, dtype=torch.int64, device=x.device)
-        y = _dropout(x, mode, dims, threshold, state, call, used)
+    def forward(ctx, x, how, state):
+        used = torch.empty_like(state)
+        y = _dropout(x, how, state, used)
         ctx.save_for_backward(used)
-        ctx.how = (mode, dims, threshold, call)
+        ctx.how = how
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        mode, dims, threshold, call = ctx.how
-        (used,) = ctx.saved_tensors
-        return _dropout(dy.contiguous(), mode, dims, threshold, used, call, None), None, None, None, None, None
+        _first_derivatives_only()
+        return _dropout(dy.contiguous(), ctx.how, ctx.saved_tensors[0], None), None, None
 
 
 def dropout(x, p, rng=None, *, call=None, per="element", group=1):
@@ -184,7 +201,7 @@ def dropout(x, p, rng=None, *, call=None, per="element", group=1):
         raise ValueError(f'per must be "element", "group" or "channel", got {per!r}')
     if int(group) < 1:
         raise ValueError(f"group must be at least 1, got {group}")
-    _dtype(x, "x")
+    code = _dtype(x, "x")
     if per != "element" and x.dim() < (1 if per == "group" else 2):
         raise ValueError(f"per={per!r} needs more axes than {list(x.shape)} has")
     dev = _device(x)
@@ -194,10 +211,10 @@ def dropout(x, p, rng=None, *, call=None, per="element", group=1):
     x = x.contiguous()
     n = x.shape[0] if x.dim() and per != "element" else 1
     C = x.shape[-1] if per == "channel" else 1
-    dims = (n, x.numel() // max(n * C, 1), C, int(group))
-    if _wants_grad(x):
-        return _DropoutFn.apply(x, _PER[per], dims, threshold, state, call)
-    return _dropout(x, _PER[per], dims, threshold, state, call, None)
+    how = (code, _PER[per], n, x.numel() // max(n * C, 1), C, int(group), threshold, call)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _DropoutFn.apply(x, how, state)
+    return _dropout(x, how, state, None)
 
 
 # ---------------------------------------------------------------------------------------------- residual + norms
@@ -223,8 +240,7 @@ def _residual_forward(how, x, y, gate, post_w, post_b, pre_w, pre_b, state, used
     z = torch.empty(y.shape, dtype=y.dtype, device=dev) if pre_w is not None else None
     a = _residual_args(how, x, y, gate, post_w, post_b, pre_w, pre_b)
     a.rng, a.used, a.h, a.z, a.stats = _ptr(state), _ptr(used), h.data_ptr(), _ptr(z), _ptr(stats)
-    with _on(dev):
-        _call("nbx_residual_norm", ctypes.byref(a), _lib.stream_ptr(dev))
+    _launch("nbx_residual_norm", dev, ctypes.byref(a))
     return h, z
 
 
@@ -245,8 +261,8 @@ class _ResidualNormFn(torch.autograd.Function):
         return (h, z) if z is not None else h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh, dz=None):
+        _first_derivatives_only()
         if dh is None and dz is None:
             return (None,) * 9
         y, h, gate, post_w, post_b, pre_w, pre_b, used, stats = ctx.saved_tensors
@@ -262,10 +278,8 @@ class _ResidualNormFn(torch.autograd.Function):
                   for i, t in enumerate((gate, post_w, post_b, pre_w, pre_b))]
         a.rng, a.h, a.stats, a.dh, a.dz = _ptr(used), _ptr(h), _ptr(stats), _ptr(dh), _ptr(dz)
         a.dx, a.dy, a.dgate, a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = (_ptr(g) for g in grads)
-        with _on(dev):
-            ws = _workspace("nbx_residual_norm_backward_workspace_bytes", a, dev)
-            _call("nbx_residual_norm_backward", ctypes.byref(a), _lib.stream_ptr(dev))
-        del ws
+        ws = _workspace("nbx_residual_norm_backward_workspace_bytes", (ctx.how[:2], a.gate_groups), a, dev)   # noqa: F841
+        _launch("nbx_residual_norm_backward", dev, ctypes.byref(a))
         return (None, None, *grads)
 
 
@@ -338,8 +352,7 @@ def _sh_forward(how, x, y, weight, bias, state, used, stats):
     a = _sh_args(how, weight, bias)
     a.rng, a.used, a.x, a.y, a.h, a.z, a.stats = (_ptr(state), _ptr(used), x.data_ptr(), y.data_ptr(), h.data_ptr(),
                                                   z.data_ptr(), _ptr(stats))
-    with _on(dev):
-        _call("nbx_sh_residual_norm", ctypes.byref(a), _lib.stream_ptr(dev))
+    _launch("nbx_sh_residual_norm", dev, ctypes.byref(a))
     return h, z
 
 
@@ -356,8 +369,8 @@ class _ShResidualNormFn(torch.autograd.Function):
         return h, z
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh, dz):
+        _first_derivatives_only()
         if dh is None and dz is None:
             return (None,) * 6
         h, weight, bias, used, stats = ctx.saved_tensors
@@ -367,10 +380,8 @@ class _ShResidualNormFn(torch.autograd.Function):
         grads = [torch.empty_like(t) if n else None for t, n in zip((h, h, weight, bias), need[2:])]
         a.rng, a.h, a.stats, a.dh, a.dz = _ptr(used), h.data_ptr(), stats.data_ptr(), _ptr(dh), _ptr(dz)
         a.dx, a.dy, a.dweight, a.dbias = (_ptr(g) for g in grads)
-        with _on(dev):
-            ws = _workspace("nbx_sh_residual_norm_backward_workspace_bytes", a, dev)
-            _call("nbx_sh_residual_norm_backward", ctypes.byref(a), _lib.stream_ptr(dev))
-        del ws
+        ws = _workspace("nbx_sh_residual_norm_backward_workspace_bytes", ctx.how[:4], a, dev)   # noqa: F841
+        _launch("nbx_sh_residual_norm_backward", dev, ctypes.byref(a))
         return (None, None, *grads)
 
 
@@ -424,10 +435,8 @@ def _attention_forward(how, values, logits, ptr, eid, state, used, stats):
     out = torch.empty(V, K, H, D, dtype=values.dtype, device=dev)
     a = _attention_args(how, ptr, eid, values, logits)
     a.rng, a.used, a.out, a.stats = _ptr(state), _ptr(used), out.data_ptr(), _ptr(stats)
-    with _on(dev):
-        ws = _workspace("nbx_segment_attention_workspace_bytes", a, dev, 0)
-        _call("nbx_segment_attention", ctypes.byref(a), _lib.stream_ptr(dev))
-    del ws
+    ws = _workspace("nbx_segment_attention_workspace_bytes", (how[:7], 0), a, dev, 0)   # noqa: F841
+    _launch("nbx_segment_attention", dev, ctypes.byref(a))
     return out
 
 
@@ -443,8 +452,8 @@ class _SegmentAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        _first_derivatives_only()
         values, logits, ptr, eid, used, stats = ctx.saved_tensors
         dev = values.device
         dout = dout.contiguous()
@@ -452,10 +461,8 @@ class _SegmentAttentionFn(torch.autograd.Function):
         dv = torch.empty_like(values) if ctx.needs_input_grad[2] else None
         dl = torch.empty_like(logits) if ctx.needs_input_grad[3] else None
         a.rng, a.stats, a.dout, a.dvalues, a.dlogits = _ptr(used), stats.data_ptr(), dout.data_ptr(), _ptr(dv), _ptr(dl)
-        with _on(dev):
-            ws = _workspace("nbx_segment_attention_workspace_bytes", a, dev, 1)
-            _call("nbx_segment_attention_backward", ctypes.byref(a), _lib.stream_ptr(dev))
-        del ws
+        ws = _workspace("nbx_segment_attention_workspace_bytes", (ctx.how[:7], 1, dl is None), a, dev, 1)   # noqa: F841
+        _launch("nbx_segment_attention_backward", dev, ctypes.byref(a))
         return None, None, dv, dl, None, None
 
 
