@@ -435,68 +435,63 @@ int with_types(const nbx_residual_norm_args& a, F&& f) {
 }
 
 // ======================================================================== residual add, spherical-harmonics norm
-// A node's (lmax+1)^2 C values sit in the registers of TPN threads: 64 (four nodes per block) or the block;
-// thread t keeps chunks t, t + TPN, .. of eight consecutive values (NJ of them).
+// A node's (lmax+1)^2 rows of C channels are cut into chunks of eight channels of one row (the last of a row may
+// be shorter), kept in the registers of TPN threads: 64 (four nodes per block) or the block; thread t holds
+// chunks t, t + TPN, .. (NJ of them).  The l = 0 row is chunks 0 .. C/8 - 1, all in the first wave, so its
+// centring needs no barrier: one block-wide sum per direction is left.
 constexpr int SH_MAXC = 512;
+constexpr int SH_LDS_HEAD = 64 + 2 * 4 * SH_MAXC / 8 / 4;   // floats before the rows in the backward pass's LDS
 
 struct ShPlan {
-    int S, RL, tpn, nj, npb, threads;   // npb: nodes in flight per block
+    int S, cpr, chunks, tpn, nj, npb, threads;   // cpr: chunks per row; npb: nodes in flight per block
 };
 
 ShPlan sh_plan(int lmax, int C) {
     ShPlan p = {};
     p.S = (lmax + 1) * (lmax + 1);
-    p.RL = p.S * C;
-    const int chunks = (p.RL + 7) / 8;
-    if (chunks <= 128) {
+    p.cpr = (C + 7) / 8;
+    p.chunks = p.S * p.cpr;
+    if (p.chunks <= 128) {
         p.tpn = 64;
-        p.nj = chunks <= 64 ? 1 : 2;
+        p.nj = p.chunks <= 64 ? 1 : 2;
         p.npb = 4;
         p.threads = 256;
     } else {
-        p.nj = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : 4;
-        p.tpn = p.threads = (int)ceil_div(ceil_div(chunks, p.nj), 64) * 64;
+        p.nj = p.chunks <= 1024 ? 1 : p.chunks <= 2048 ? 2 : 4;
+        p.tpn = p.threads = (int)ceil_div(ceil_div(p.chunks, p.nj), 64) * 64;
         p.npb = 1;
     }
     return p;
 }
 
-__device__ __forceinline__ int degree_of(int i) {
-    return (i >= 1) + (i >= 4) + (i >= 9) + (i >= 16) + (i >= 25) + (i >= 36);
-}
-
-// coefficient and channel of eight consecutive values starting at f0
-struct ShAt {
-    int i[8], c[8];
+// what chunk t + TPN j of a node is
+struct ShChunk {
+    int at, n, l, c8;   // offset in the node, channels (0: none), degree, channel / 8
+    bool first;         // of the l = 0 row
+    float bal;
 };
-__device__ __forceinline__ ShAt sh_at(int f0, int C) {
-    ShAt s;
-    int i = f0 / C, c = f0 - i * C;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        s.i[e] = i;
-        s.c[e] = c;
-        if (++c == C) {
-            c = 0;
-            ++i;
-        }
-    }
-    return s;
+__device__ __forceinline__ ShChunk sh_chunk(const ShPlan& p, int q, int C, int lmax) {
+    ShChunk k;
+    const int i = q / p.cpr;
+    k.c8 = q - i * p.cpr;
+    k.at = i * C + 8 * k.c8;
+    k.n = q < p.chunks ? std::min(8, C - 8 * k.c8) : 0;
+    k.l = (i >= 1) + (i >= 4) + (i >= 9) + (i >= 16) + (i >= 25) + (i >= 36);
+    k.first = i == 0;
+    k.bal = 1.0f / (float)((2 * k.l + 1) * (lmax + 1));
+    return k;
 }
 
+// sum over a node's threads, in all of them: SUB a wave, else the block (one barrier; `slot` alternates)
 template <bool SUB>
 __device__ __forceinline__ float node_sum(float x, float (*red)[16], int& slot) {
     return row_sum<SUB ? 64 : 0>(x, red, slot);
 }
 
-// the factors of a node's dropout: path (whole node) and the channel bits in LDS
-__device__ __forceinline__ void sh_channel_bits(const nbx_sh_residual_norm_args& a, int64_t node, bool live, int t,
-                                                int tpn, uint8_t* bits) {
-    if (!a.channel_threshold) return;
-    const int Cq = (a.C + 7) >> 3;
-    const DrawKey key = draw_key(a.rng, a.call + 1);
-    if (live)
-        for (int k = t; k < Cq; k += tpn) bits[k] = (uint8_t)keep_bits(key, (uint64_t)(node * Cq + k), a.channel_threshold);
+// the channel draws of a node as bits in LDS: one Philox block per eight channels, shared by its rows
+__device__ __forceinline__ void sh_channel_bits(const nbx_sh_residual_norm_args& a, const DrawKey& key, int64_t node,
+                                                int t, int cpr, uint8_t* bits) {
+    if (t < cpr) bits[t] = (uint8_t)keep_bits(key, (uint64_t)(node * cpr + t), a.channel_threshold);
 }
 
 template <typename T, int NJ, bool SUB>
@@ -508,64 +503,69 @@ __global__ __launch_bounds__(SUB ? 256 : 1024) void sh_residual_norm_kernel(nbx_
     if (a.path_threshold | a.channel_threshold) note_used(a.used, a.rng);
     const int t = SUB ? (int)threadIdx.x & 63 : (int)threadIdx.x, sub = SUB ? (int)threadIdx.x >> 6 : 0;
     const int64_t v = SUB ? blockIdx.x * (int64_t)4 + sub : blockIdx.x;
-    const bool live = v < a.V;
-    sh_channel_bits(a, v, live, t, p.tpn, bits[sub]);
-    __syncthreads();
-    if (!live) return;   // SUB: whole waves, no barrier below
-    const bool path = !a.path_threshold || keep_one(draw_key(a.rng, a.call), (uint64_t)(v / a.path_group), a.path_threshold);
-    const float k = (a.path_threshold ? k1 : 1.f) * (a.channel_threshold ? k2 : 1.f);
     const int C = a.C;
-    float h[NJ][8];
-    float s0 = 0.f;
+    const int64_t base = v * p.S * C;
+    const bool live = v < a.V;
+    ShChunk q[NJ];
+    float h[NJ][8], y[NJ][8];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        const int f0 = 8 * (t + p.tpn * j), n = std::max(0, std::min(8, p.RL - f0));
-        const int64_t at = v * p.RL + f0;
-        float y[8];
-        load8n((const T*)a.x + at, n, h[j]);
-        load8n((const T*)a.y + at, n, y);
-        const ShAt q = sh_at(f0, C);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const bool on = path && (!a.channel_threshold || (e < n && (bits[sub][q.c[e] >> 3] >> (q.c[e] & 7) & 1)));
-            h[j][e] += on ? k * y[e] : 0.f;
-            if (f0 + e < C) s0 += h[j][e];
-        }
-        store8n((T*)a.h + at, n, h[j]);
+        q[j] = sh_chunk(p, t + p.tpn * j, C, a.lmax);
+        if (!live) q[j].n = 0;
+        load8n((const T*)a.x + base + q[j].at, q[j].n, h[j]);
+        load8n((const T*)a.y + base + q[j].at, q[j].n, y[j]);
     }
-    const float m0 = node_sum<SUB>(s0, red, slot) / (float)C;
-    float qs = 0.f;
+    if (a.channel_threshold) {
+        if (live) sh_channel_bits(a, draw_key(a.rng, a.call + 1), v, t, p.cpr, bits[sub]);
+        __syncthreads();
+    }
+    if (!live) return;   // SUB: whole waves, no barrier below
+    float k = a.channel_threshold ? k2 : 1.f;
+    uint32_t path = 0xFFu;
+    if (a.path_threshold) {
+        k *= k1;
+        path = keep_one(draw_key(a.rng, a.call), (uint64_t)(v / a.path_group), a.path_threshold) ? 0xFFu : 0u;
+    }
+    float s0 = 0.f, qs = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        const int f0 = 8 * (t + p.tpn * j), n = std::max(0, std::min(8, p.RL - f0));
-        const ShAt q = sh_at(f0, C);
+        const uint32_t m = a.channel_threshold ? path & bits[sub][q[j].c8] : path;
+        float s = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (f0 + e < C) h[j][e] -= m0;
-            const int l = degree_of(q.i[e]);
-            if (e < n) qs += h[j][e] * h[j][e] / (float)((2 * l + 1) * (a.lmax + 1));
+            h[j][e] += (m >> e & 1) ? k * y[j][e] : 0.f;   // past the row: 0
+            s += h[j][e] * h[j][e];
+            if (j == 0 && q[0].first) s0 += h[0][e];
+        }
+        if (!q[j].first) qs += q[j].bal * s;
+        store8n((T*)a.h + base + q[j].at, q[j].n, h[j]);
+    }
+    float m0 = 0.f;
+    if (t < 64) {   // the first wave holds the l = 0 row
+        m0 = lanes_sum<64>(s0) / (float)C;
+        if (q[0].first) {
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                h[0][e] -= m0;
+                if (e < q[0].n) s += h[0][e] * h[0][e];
+            }
+            qs += q[0].bal * s;
         }
     }
     const float rs = 1.0f / sqrtf(node_sum<SUB>(qs, red, slot) / (float)C + a.eps);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        const int f0 = 8 * (t + p.tpn * j), n = std::max(0, std::min(8, p.RL - f0));
-        const ShAt q = sh_at(f0, C);
-        float z[8];
+        float w[8];
+        load8p(a.weight, a.param_dtype, q[j].l * C + 8 * q[j].c8, q[j].n, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            z[e] = 0.f;
-            if (e < n) {
-                float w[8], b[8];
-                load8p(a.weight, a.param_dtype, degree_of(q.i[e]) * C + q.c[e], 1, w);
-                z[e] = h[j][e] * rs * w[0];
-                if (f0 + e < C) {
-                    load8p(a.bias, a.param_dtype, q.c[e], 1, b);
-                    z[e] += b[0];
-                }
-            }
+        for (int e = 0; e < 8; ++e) h[j][e] = h[j][e] * rs * w[e];
+        if (j == 0 && q[0].first) {
+            load8p(a.bias, a.param_dtype, 8 * q[0].c8, q[0].n, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[0][e] += w[e];
         }
-        store8n((T*)a.z + v * p.RL + f0, n, z);
+        store8n((T*)a.z + base + q[j].at, q[j].n, h[j]);
     }
     if (a.stats && t == 0) {
         a.stats[v] = m0;
@@ -573,119 +573,136 @@ __global__ __launch_bounds__(SUB ? 256 : 1024) void sh_residual_norm_kernel(nbx_
     }
 }
 
-// Backward over nodes [unit, unit + nunits, ..) with the column sums per coefficient and channel in
-// registers: part[unit][S C + C] = (sum over nodes of dz hc rs | of dz's l = 0 row).
+// Backward over nodes unit, unit + nunits, ..: each thread keeps its chunks' weights, and the column sums of
+// dz hc rs per row and of dz's l = 0 row, in registers over the nodes.  At the end the rows of a degree are
+// summed in LDS: part[unit][(lmax + 2) C] = (dweight | dbias) of the unit's nodes.
 template <typename T, int NJ, bool SUB>
 __global__ __launch_bounds__(SUB ? 256 : 1024) void sh_residual_norm_bwd_kernel(nbx_sh_residual_norm_args a, ShPlan p,
                                                                                 float k1, float k2, int64_t nunits,
                                                                                 float* __restrict__ part) {
-    __shared__ float red[4][16];
-    __shared__ uint8_t bits[2][SUB ? 4 : 1][SH_MAXC / 8];
+    // all of it dynamic, so that the kernel's limit can be raised to the whole 160 KB
+    extern __shared__ float sh_lds[];
+    float (*red)[16] = reinterpret_cast<float (*)[16]>(sh_lds);                        // [4][16]
+    auto bits = reinterpret_cast<uint8_t (*)[SUB ? 4 : 1][SH_MAXC / 8]>(sh_lds + 64);   // [2]
+    float* rows = sh_lds + SH_LDS_HEAD;                                                // [npb][chunks 8]
     int slot = 0, flip = 0;
     const int t = SUB ? (int)threadIdx.x & 63 : (int)threadIdx.x, sub = SUB ? (int)threadIdx.x >> 6 : 0;
     const int64_t unit = SUB ? blockIdx.x * (int64_t)4 + sub : blockIdx.x;
-    const float k = (a.path_threshold ? k1 : 1.f) * (a.channel_threshold ? k2 : 1.f);
     const int C = a.C;
-    float aw[NJ][8] = {}, ab[8] = {};
+    const float k = (a.path_threshold ? k1 : 1.f) * (a.channel_threshold ? k2 : 1.f);
+    DrawKey key = {0, 0, 0, 0};
+    if (a.path_threshold | a.channel_threshold) key = draw_key(a.rng, a.call);
+    ShChunk q[NJ];
+    float w[NJ][8], aw[NJ][8] = {}, ab[8] = {};
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        q[j] = sh_chunk(p, t + p.tpn * j, C, a.lmax);
+        load8p(a.weight, a.param_dtype, q[j].l * C + 8 * q[j].c8, q[j].n, w[j]);
+    }
     const int64_t iters = (a.V + nunits - 1) / nunits;
     for (int64_t it = 0; it < iters; ++it) {
         const int64_t v = it * nunits + unit;
         const bool live = v < a.V;
-        sh_channel_bits(a, v, live, t, p.tpn, bits[flip][sub]);
-        __syncthreads();   // two copies of the bits: the next node's are written before this one's last read
+        if (a.channel_threshold) {   // two copies: the next node's bits are written before this one's last read
+            DrawKey ck = key;
+            ck.call = a.call + 1;
+            if (live) sh_channel_bits(a, ck, v, t, p.cpr, bits[flip][sub]);
+            __syncthreads();
+        }
         const uint8_t* bt = bits[flip][sub];
         flip ^= 1;
-        if (SUB && !live) continue;
-        if (!live) break;   // W = 0: the whole block
-        const bool path = !a.path_threshold || keep_one(draw_key(a.rng, a.call), (uint64_t)(v / a.path_group), a.path_threshold);
+        if (!live) {
+            if (SUB) continue;
+            break;   // the whole block
+        }
+        const int64_t base = v * p.S * C;
         const float m0 = a.stats[v], rs = a.stats[a.V + v];
-        float g[NJ][8], hc[NJ][8];
+        float g[NJ][8], hc[NJ][8], dh[NJ][8];
         float dot = 0.f, sg = 0.f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int f0 = 8 * (t + p.tpn * j), n = std::max(0, std::min(8, p.RL - f0));
-            const int64_t at = v * p.RL + f0;
-            const ShAt q = sh_at(f0, C);
-            if (a.dz) {
-                load8n((const T*)a.dz + at, n, g[j]);
-                load8n((const T*)a.h + at, n, hc[j]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) g[j][e] = hc[j][e] = 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (f0 + e < C) {
-                    hc[j][e] -= m0;
-                    if (j == 0) ab[e] += g[j][e];
-                }
-                aw[j][e] += g[j][e] * hc[j][e] * rs;
-                if (e < n) {
-                    float w[8];
-                    load8p(a.weight, a.param_dtype, degree_of(q.i[e]) * C + q.c[e], 1, w);
-                    g[j][e] *= w[0];
-                    dot += g[j][e] * hc[j][e];
-                    if (f0 + e < C) sg += g[j][e];
-                }
-            }
+            const int n = q[j].n;
+            load8n((const T*)a.dz + base + q[j].at, a.dz ? n : 0, g[j]);
+            load8n((const T*)a.h + base + q[j].at, a.dz ? n : 0, hc[j]);
+            load8n((const T*)a.dh + base + q[j].at, a.dh ? n : 0, dh[j]);
         }
-        dot = node_sum<SUB>(dot, red, slot);
-        sg = node_sum<SUB>(sg, red, slot);
-        const float coef = rs * rs * rs / (float)C * dot;
-        const float dm = rs * sg / (float)C;   // the centred row sums to 0, so only g is left of its mean
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int f0 = 8 * (t + p.tpn * j), n = std::max(0, std::min(8, p.RL - f0));
-            const int64_t at = v * p.RL + f0;
-            const ShAt q = sh_at(f0, C);
-            float dh[8];
-            if (a.dh) load8n((const T*)a.dh + at, n, dh);
+            if (j == 0 && q[0].first) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (e < q[0].n) hc[0][e] -= m0;
+                    ab[e] += g[0][e];
+                    sg += g[0][e] * w[0][e];
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float bal = 1.0f / (float)((2 * degree_of(q.i[e]) + 1) * (a.lmax + 1));
-                float d = rs * g[j][e] - coef * bal * hc[j][e] - (f0 + e < C ? dm : 0.f);
-                if (a.dh) d += dh[e];
-                g[j][e] = d;
-                const bool on = path && (!a.channel_threshold || (e < n && (bt[q.c[e] >> 3] >> (q.c[e] & 7) & 1)));
-                hc[j][e] = on ? k * d : 0.f;
+                hc[j][e] *= rs;
+                aw[j][e] += g[j][e] * hc[j][e];
+                g[j][e] *= w[j][e];
+                dot += g[j][e] * hc[j][e];
             }
-            if (a.dx) store8n((T*)a.dx + at, n, g[j]);
-            if (a.dy) store8n((T*)a.dy + at, n, hc[j]);
+        }
+        dot = node_sum<SUB>(dot, red, slot) / (float)C;
+        // the centred row sums to 0, so only g is left of the l = 0 row's mean
+        const float dm = t < 64 ? lanes_sum<64>(sg) / (float)C : 0.f;
+        uint32_t path = 0xFFu;
+        if (a.path_threshold)
+            path = keep_one(key, (uint64_t)(v / a.path_group), a.path_threshold) ? 0xFFu : 0u;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const uint32_t m = a.channel_threshold ? path & bt[q[j].c8] : path;
+            const float cb = dot * q[j].bal, d0 = q[j].first ? dm : 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float d = dh[j][e] + rs * (g[j][e] - cb * hc[j][e] - d0);
+                g[j][e] = d;
+                hc[j][e] = (m >> e & 1) ? k * d : 0.f;
+            }
+            if (a.dx) store8n((T*)a.dx + base + q[j].at, q[j].n, g[j]);
+            if (a.dy) store8n((T*)a.dy + base + q[j].at, q[j].n, hc[j]);
         }
     }
     if (!part) return;
-    float* to = part + unit * (p.RL + C);
+    const int row = 8 * p.cpr;
+    float* mine = rows + sub * 8 * p.chunks;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        const int f0 = 8 * (t + p.tpn * j);
-        store8n(to + f0, std::max(0, std::min(8, p.RL - f0)), aw[j]);
-        if (j == 0) store8n(to + p.RL + f0, std::max(0, std::min(8, C - f0)), ab);
+    for (int j = 0; j < NJ; ++j)
+        if (q[j].n) store8(mine + 8 * (t + p.tpn * j), aw[j]);
+    float* to = part + unit * (int64_t)(a.lmax + 2) * C;
+    if (q[0].first && q[0].n) store8n(to + (a.lmax + 1) * C + 8 * q[0].c8, q[0].n, ab);
+    __syncthreads();
+    for (int o = t; o < (a.lmax + 1) * C; o += p.tpn) {
+        const int l = o / C, c = o - l * C;
+        float s = 0.f;
+        for (int i = l * l; i < (l + 1) * (l + 1); ++i) s += mine[i * row + c];
+        to[o] = s;
     }
 }
 
-// dweight [lmax+1][C] | dbias [C] from the units' partial sums: 64 columns x 16 waves in a fixed order
-__global__ __launch_bounds__(1024) void sh_residual_sums_kernel(nbx_sh_residual_norm_args a, int RL, int64_t nunits,
+// dweight [lmax+1][C] | dbias [C] from the units' partial rows: 64 columns x 16 waves in a fixed order
+__global__ __launch_bounds__(1024) void sh_residual_sums_kernel(nbx_sh_residual_norm_args a, int64_t nunits,
                                                                 const float* __restrict__ part) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + lane, l = blockIdx.y, C = a.C;   // l = lmax + 1: the bias
-    const int i0 = l <= a.lmax ? l * l : 0, ni = l <= a.lmax ? 2 * l + 1 : 1;
-    const int64_t ld = RL + C;
-    const float* p = part + (l <= a.lmax ? i0 * C : RL) + c;
+    const int64_t ld = (int64_t)(a.lmax + 2) * a.C;
+    const int64_t c = blockIdx.x * (int64_t)64 + lane;
     float s = 0.f;
-    if (c < C)
-        for (int64_t u = w; u < nunits; u += 16)
-            for (int i = 0; i < ni; ++i) s += p[u * ld + i * C];
+    if (c < ld)
+#pragma unroll 8
+        for (int64_t u = w; u < nunits; u += 16) s += part[u * ld + c];
     red[w][lane] = s;
     __syncthreads();
-    if (w == 0 && c < C) {
+    if (w == 0 && c < ld) {
         float t = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) t += red[i][lane];
-        if (l <= a.lmax) {
-            if (a.dweight) store1p(a.dweight, a.param_dtype, (int64_t)l * C + c, t);
+        const int64_t nw = ld - a.C;
+        if (c < nw) {
+            if (a.dweight) store1p(a.dweight, a.param_dtype, c, t);
         } else if (a.dbias) {
-            store1p(a.dbias, a.param_dtype, c, t);
+            store1p(a.dbias, a.param_dtype, c - nw, t);
         }
     }
 }
@@ -694,6 +711,10 @@ __global__ __launch_bounds__(1024) void sh_residual_sums_kernel(nbx_sh_residual_
 int64_t sh_units(const ShPlan& p, int64_t V) {
     const int64_t most = 512 * (int64_t)p.npb;
     return std::max<int64_t>(1, ceil_div(std::min(most, ceil_div(V, 4)), p.npb)) * p.npb;
+}
+
+size_t sh_workspace(const ShPlan& p, int64_t V, int lmax, int C) {
+    return (size_t)sh_units(p, V) * (lmax + 2) * C * sizeof(float);
 }
 
 int sh_check(const nbx_sh_residual_norm_args* a, const char* who) {
@@ -714,20 +735,23 @@ int sh_launch(const nbx_sh_residual_norm_args& a, const ShPlan& p, int64_t units
     const float k1 = keep_scale(a.path_threshold), k2 = keep_scale(a.channel_threshold);
     const unsigned blocks = (unsigned)ceil_div(BWD ? units : a.V, p.npb);
     auto go = [&](auto fwd, auto bwd) {
-        if constexpr (BWD)
-            hipLaunchKernelGGL(bwd, dim3(blocks), dim3(p.threads), 0, st, a, p, k1, k2, units, part);
-        else
+        if constexpr (BWD) {
+            // up to 98 KB of LDS (lmax 6, 512 channels)
+            const size_t lds = (SH_LDS_HEAD + (part ? (size_t)p.npb * p.chunks * 8 : 0)) * sizeof(float);
+            if (lds > 60 * 1024) NBX_LDS_160K(bwd);
+            hipLaunchKernelGGL(bwd, dim3(blocks), dim3(p.threads), lds, st, a, p, k1, k2, units, part);
+        } else {
             hipLaunchKernelGGL(fwd, dim3(blocks), dim3(p.threads), 0, st, a, p, k1, k2);
+        }
+        return NBX_OK;
     };
     if (p.npb == 4) {
-        if (p.nj == 1) go(sh_residual_norm_kernel<T, 1, true>, sh_residual_norm_bwd_kernel<T, 1, true>);
-        else go(sh_residual_norm_kernel<T, 2, true>, sh_residual_norm_bwd_kernel<T, 2, true>);
-    } else {
-        if (p.nj == 1) go(sh_residual_norm_kernel<T, 1, false>, sh_residual_norm_bwd_kernel<T, 1, false>);
-        else if (p.nj == 2) go(sh_residual_norm_kernel<T, 2, false>, sh_residual_norm_bwd_kernel<T, 2, false>);
-        else go(sh_residual_norm_kernel<T, 4, false>, sh_residual_norm_bwd_kernel<T, 4, false>);
+        if (p.nj == 1) return go(sh_residual_norm_kernel<T, 1, true>, sh_residual_norm_bwd_kernel<T, 1, true>);
+        return go(sh_residual_norm_kernel<T, 2, true>, sh_residual_norm_bwd_kernel<T, 2, true>);
     }
-    return NBX_OK;
+    if (p.nj == 1) return go(sh_residual_norm_kernel<T, 1, false>, sh_residual_norm_bwd_kernel<T, 1, false>);
+    if (p.nj == 2) return go(sh_residual_norm_kernel<T, 2, false>, sh_residual_norm_bwd_kernel<T, 2, false>);
+    return go(sh_residual_norm_kernel<T, 4, false>, sh_residual_norm_bwd_kernel<T, 4, false>);
 }
 
 }  // namespace
@@ -860,7 +884,7 @@ extern "C" int nbx_sh_residual_norm_backward_workspace_bytes(const nbx_sh_residu
     if (int rc = sh_check(a, "nbx_sh_residual_norm_backward_workspace_bytes")) return rc;
     NBX_CHECK_ARG(bytes, "nbx_sh_residual_norm_backward_workspace_bytes: null result");
     const ShPlan p = sh_plan(a->lmax, a->C);
-    *bytes = a->V ? (size_t)sh_units(p, a->V) * (p.RL + a->C) * sizeof(float) : 0;
+    *bytes = a->V ? sh_workspace(p, a->V, a->lmax, a->C) : 0;
     return NBX_OK;
 }
 
@@ -871,7 +895,7 @@ extern "C" int nbx_sh_residual_norm_backward(const nbx_sh_residual_norm_args* a,
     const ShPlan p = sh_plan(a->lmax, a->C);
     const int64_t units = sh_units(p, a->V);
     const bool sums = a->dweight || a->dbias;
-    if (sums && !(a->workspace && a->workspace_bytes >= (size_t)units * (p.RL + a->C) * sizeof(float))) {
+    if (sums && !(a->workspace && a->workspace_bytes >= sh_workspace(p, a->V, a->lmax, a->C))) {
         set_error("nbx_sh_residual_norm_backward: workspace too small");
         return NBX_E_WORKSPACE;
     }
@@ -880,8 +904,8 @@ extern "C" int nbx_sh_residual_norm_backward(const nbx_sh_residual_norm_args* a,
     if (int rc = with_type(a->dtype, [&](auto t) { return sh_launch<true, decltype(t)>(*a, p, units, part, st); })) return rc;
     NBX_LAUNCH_CHECK("sh_residual_norm_bwd");
     if (sums) {
-        hipLaunchKernelGGL(sh_residual_sums_kernel, dim3((unsigned)ceil_div(a->C, 64), (unsigned)(a->lmax + 2)), dim3(1024),
-                           0, st, *a, p.RL, units, part);
+        hipLaunchKernelGGL(sh_residual_sums_kernel, dim3((unsigned)ceil_div((a->lmax + 2) * a->C, 64)), dim3(1024), 0, st,
+                           *a, units, part);
         NBX_LAUNCH_CHECK("sh_residual_sums");
     }
     return NBX_OK;

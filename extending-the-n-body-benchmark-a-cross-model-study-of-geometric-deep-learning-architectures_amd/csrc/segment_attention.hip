@@ -5,8 +5,8 @@
 //   * list form: a block per (node, slice of the row) walks the node's list with a running maximum and sum;
 //   * chunk form, for long lists: a block per 64 positions of the CSR, whatever nodes they belong to; a list
 //     that crosses a chunk's border leaves partial sums with their own maximum, joined by a second launch.
-// Backward: a block per few positions (dvalues and the weights' gradient), then the softmax's own gradient
-// per list.
+// Backward: a block per few positions forms dvalues, the weights' gradient and, for lists that lie within
+// the block, the softmax's own gradient; a second launch finishes the lists that cross blocks.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,6 +20,7 @@ using namespace nbx;
 
 constexpr int TILE = 64;      // positions whose weights are in LDS at once
 constexpr int SA_MAXH = 64;
+constexpr int PREFETCH = 4;   // values of a thread that are loaded before the weights are known
 
 template <typename T, int VW>
 struct VecT {
@@ -66,7 +67,7 @@ struct SaPlan {
     int T, RV, EL, slices;    // threads, vectors per row, edges side by side, blocks per row
     int eb, TP, grp;          // backward: positions per block, threads that work, lanes of a head that shuffle
     int chunked;
-    int64_t nc;               // chunks
+    int64_t nc;               // chunks (forward) or blocks (backward)
 };
 
 __device__ __forceinline__ void note_used(const nbx_segment_attention_args& a) {
@@ -76,15 +77,36 @@ __device__ __forceinline__ void note_used(const nbx_segment_attention_args& a) {
     }
 }
 
-// the node whose list holds position p: the last v with ptr[v] <= p
-__device__ __forceinline__ int node_of(const int32_t* ptr, int64_t V, int p) {
+// sV[i], i < cnt <= 64: the node whose list holds position p0 + i (the last v with ptr[v] <= p0 + i), or -1 in
+// none.  One wave: a 64-way search for the first position, then the starts of the nodes after it are dropped
+// on their positions and spread to the right.
+__device__ __forceinline__ void nodes_of_positions(const int32_t* __restrict__ ptr, int64_t V, int64_t p0, int cnt,
+                                                   int* sV) {
+    const int lane = threadIdx.x & 63;
     int64_t lo = 0, hi = V;
     while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (ptr[mid] <= p) lo = mid;
-        else hi = mid;
+        const int64_t step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step;
+        const uint64_t below = __ballot(at < hi && ptr[std::min(at, V)] <= p0);
+        lo += __popcll(below) * step;
+        hi = std::min(hi, lo + step);
     }
-    return (int)lo;
+    sV[lane] = lane == 0 ? (int)lo : -1;
+    __threadfence_block();
+    for (int64_t v = lo + 1; v < V; v += 64) {
+        const int64_t mine = v + lane;
+        const int64_t at = mine < V ? ptr[mine] - p0 : cnt;
+        if (at > 0 && at < cnt) atomicMax(&sV[at], (int)mine);
+        if (__ballot(at >= cnt)) break;   // starts ascend: the later ones lie behind the block
+    }
+    __threadfence_block();
+    int v = sV[lane];
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const int left = __shfl_up(v, m, 64);
+        if (lane >= m) v = std::max(v, left);
+    }
+    const int64_t p = p0 + lane;
+    sV[lane] = lane < cnt && p >= ptr[v] && p < ptr[v + 1] ? v : -1;
 }
 
 // Sum over the EL groups of RV threads (thread = el RV + f), left in group 0.
@@ -136,6 +158,14 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
             sE[i] = e >= 0 && e < a.E ? e : -1;
         }
         __syncthreads();
+        // the first values are on their way while the weights are formed
+        float first[PREFETCH][VW];
+#pragma unroll
+        for (int k = 0; k < PREFETCH; ++k) {
+            const int i = el + k * p.EL;
+            if (on && i < cnt && sE[i] >= 0)
+                loadv<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW, first[k]);
+        }
         for (int i = t; i < cnt * H; i += p.T) {
             const int e = sE[i / H];
             sW[i] = e < 0 ? -INFINITY : load_logit(a, (int64_t)e * H + i % H);
@@ -163,8 +193,16 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
             const float r = sR[head];
 #pragma unroll
             for (int k = 0; k < VW; ++k) acc[k] *= r;
+#pragma unroll
+            for (int j = 0; j < PREFETCH; ++j) {
+                const int i = el + j * p.EL;
+                const float w = i < cnt ? sW[i * H + head] : 0.f;
+                if (w != 0.f)
+#pragma unroll
+                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, first[j][k], acc[k]);
+            }
 #pragma unroll 4
-            for (int i = el; i < cnt; i += p.EL) {
+            for (int i = el + PREFETCH * p.EL; i < cnt; i += p.EL) {
                 const float w = sW[i * H + head];
                 if (w != 0.f) {
                     float x[VW];
@@ -203,20 +241,21 @@ __global__ __launch_bounds__(256) void segment_attention_chunk_kernel(nbx_segmen
     float* red = sS + TILE * H;
     int* sE = reinterpret_cast<int*>(red + p.T * VW);
     int* sV = sE + TILE;
+    uint8_t* sK = reinterpret_cast<uint8_t*>(sV + TILE);   // [TILE][H]
     note_used(a);
     const DrawKey key = a.threshold ? draw_key(a.rng, a.call) : DrawKey{0, 0, 0, 0};
     const int64_t c = blockIdx.x;
     const int p0 = (int)(c * TILE), cnt = (int)std::min<int64_t>(TILE, a.E - c * TILE);
-    if (t < cnt) {
-        const int e = a.eid[p0 + t];
-        sE[t] = e >= 0 && e < a.E ? e : -1;
-        const int v = node_of(a.ptr, a.V, p0 + t);
-        sV[t] = p0 + t >= a.ptr[v] && p0 + t < a.ptr[v + 1] ? v : -1;   // -1: in no list
+    if (t < 64) nodes_of_positions(a.ptr, a.V, p0, cnt, sV);
+    else if (t < 64 + cnt) {
+        const int e = a.eid[p0 + t - 64];
+        sE[t - 64] = e >= 0 && e < a.E ? e : -1;
     }
     __syncthreads();
     for (int i = t; i < cnt * H; i += p.T) {
         const int e = sE[i / H];
         sW[i] = e < 0 ? -INFINITY : load_logit(a, (int64_t)e * H + i % H);
+        sK[i] = !a.threshold || keep_one(key, (uint64_t)(int64_t)e * H + i % H, a.threshold);
     }
     __syncthreads();
     for (int k = t; k < cnt * H; k += p.T) {
@@ -228,7 +267,7 @@ __global__ __launch_bounds__(256) void segment_attention_chunk_kernel(nbx_segmen
         for (int i = i0; i < i1; ++i) {
             const float w = weight_of(sW[i * H + h], finite_max(m));
             s += w;
-            sW[i * H + h] = !a.threshold || keep_one(key, (uint64_t)(int64_t)sE[i] * H + h, a.threshold) ? w : 0.f;
+            sW[i * H + h] = sK[i * H + h] ? w : 0.f;
         }
         sM[k] = m;
         sS[k] = s;
@@ -286,80 +325,111 @@ __global__ __launch_bounds__(256) void segment_attention_chunk_kernel(nbx_segmen
     }
 }
 
-// joins the partial sums of a list over its chunks; an empty list gives 0
+// joins the partial sums of a list over its chunks, EL of them side by side; an empty list gives 0
 template <typename T, int VW>
 __global__ __launch_bounds__(256) void segment_attention_join_kernel(nbx_segment_attention_args a, SaPlan p, float keep,
                                                                      const float* __restrict__ pacc,
                                                                      const float* __restrict__ pms) {
+    extern __shared__ float lds[];
     const int64_t v = blockIdx.x;
     const int t = threadIdx.x, H = a.H;
     const int j0 = std::max(0, a.ptr[v]), j1 = (int)std::min<int64_t>(a.E, a.ptr[v + 1]);
-    const int64_t c0 = j0 / TILE, c1 = j1 > j0 ? (j1 - 1) / TILE : c0;
-    if (j1 > j0 && c0 == c1) return;
-    const bool empty = j1 <= j0;
+    const int64_t c0 = j0 / TILE, c1 = j1 > j0 ? (j1 - 1) / TILE : c0 - 1;
+    if (c1 == c0) return;   // within one chunk: done there
+    float* sR = lds;              // [TILE][H] factors of a tile of parts
+    float* sQ = sR + TILE * H;    // [TILE][H] and their sums
+    float* sM = sQ + TILE * H;    // [T] maxima, then [H] the list's
+    float* sS = sM + p.T;         // [H]
+    float* red = sS + H;          // [T VW]
     const int64_t RL = (int64_t)p.RV * VW;
     auto slot = [&](int64_t c) { return 2 * c + (j0 < c * TILE ? 0 : 1); };
-    auto top = [&](int h) {
-        float m = -INFINITY;
-        if (!empty)
-            for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, pms[slot(c) * 2 * H + h]);
-        return m;
-    };
-    const int f = blockIdx.y * p.T + t;
-    if (f < p.RV) {
-        const int h = (f * VW / a.D) % H;
-        const float m = finite_max(top(h));
-        float acc[VW] = {}, s = 0.f;
-        if (!empty)
-            for (int64_t c = c0; c <= c1; ++c) {
-                const int64_t k = slot(c);
-                const float r = weight_of(pms[k * 2 * H + h], m);
-                s += r * pms[(k * 2 + 1) * H + h];
-                if (r != 0.f)
+    const int hs = p.T / H, h = t % H, r = t / H;   // threads per head
+    float m = -INFINITY;
+    if (r < hs)
+        for (int64_t c = c0 + r; c <= c1; c += hs) m = fmaxf(m, pms[slot(c) * 2 * H + h]);
+    sM[t] = m;
+    __syncthreads();
+    if (t < H) {
+        for (int i = 1; i < hs; ++i) m = fmaxf(m, sM[i * H + t]);
+        sM[t] = finite_max(m);
+        sS[t] = 0.f;
+    }
+    const int el = p.slices > 1 ? 0 : t / p.RV;
+    const int f = p.slices > 1 ? (int)blockIdx.y * p.T + t : t - el * p.RV;
+    const bool on = el < p.EL && f < p.RV;
+    const int head = on ? (f * VW / a.D) % H : 0;
+    float acc[VW] = {};
+    for (int64_t b = c0; b <= c1; b += TILE) {
+        const int cnt = (int)std::min<int64_t>(TILE, c1 + 1 - b);
+        __syncthreads();
+        for (int i = t; i < cnt * H; i += p.T) {
+            const float* ms = pms + slot(b + i / H) * 2 * H + i % H;
+            const float w = weight_of(ms[0], sM[i % H]);
+            sR[i] = w;
+            sQ[i] = w * ms[H];
+        }
+        __syncthreads();
+        if (t < H) {
+            float s = sS[t];
+            for (int i = 0; i < cnt; ++i) s += sQ[i * H + t];
+            sS[t] = s;
+        }
+        if (on)
+#pragma unroll 4
+            for (int i = el; i < cnt; i += p.EL) {
+                const float w = sR[i * H + head];
+                if (w != 0.f) {
+                    float x[VW];
+                    loadv<float, VW>(pacc + slot(b + i) * RL + (int64_t)f * VW, x);
 #pragma unroll
-                    for (int i = 0; i < VW; ++i) acc[i] += r * pacc[k * RL + (int64_t)f * VW + i];
+                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, x[k], acc[k]);
+                }
             }
-        const float inv = keep / (s + 1e-16f);
+    }
+    if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
+    else __syncthreads();
+    if (on && el == 0) {
+        const float inv = keep / (sS[head] + 1e-16f);
 #pragma unroll
-        for (int i = 0; i < VW; ++i) acc[i] = s == 0.f ? 0.f : acc[i] * inv;
+        for (int k = 0; k < VW; ++k) acc[k] = sS[head] == 0.f ? 0.f : acc[k] * inv;
         storev<T, VW>((T*)a.out + v * RL + (int64_t)f * VW, acc);
     }
     if (a.stats && blockIdx.y == 0 && t < H) {
-        const float m = finite_max(top(t));
-        float s = 0.f;
-        if (!empty)
-            for (int64_t c = c0; c <= c1; ++c) s += weight_of(pms[slot(c) * 2 * H + t], m) * pms[(slot(c) * 2 + 1) * H + t];
-        a.stats[v * H + t] = m;
-        a.stats[(a.V + v) * H + t] = 1.0f / (s + 1e-16f);
+        a.stats[v * H + t] = sM[t];
+        a.stats[(a.V + v) * H + t] = 1.0f / (sS[t] + 1e-16f);
     }
 }
 
 // ======================================================================== backward
-// Positions [eb block, ..): dvalues = w dout[v], dp[position][h] = keep/(1-p) <dout[v], values>_h.
-// Threads: EL groups of RV, or (long rows) TP threads, a multiple of the H D / VW columns, over the row in
-// steps of TP: either way a thread stays with one head.
+// Positions [eb block, ..): dvalues = w dout[v], and with dp = keep/(1-p) <dout[v], values>_h the softmax's
+// dl = a (dp - sum over the list of a dp).  A list that crosses the block's borders leaves its a, dp (per
+// position) and its share of the sum: slot 2 block = the list that began before, 2 block + 1 = the one that
+// goes on.  Threads: EL groups of RV, or (long rows) TP threads, a multiple of the H D / VW columns, over the
+// row in steps of TP: either way a thread stays with one head.
 template <typename T, int VW>
 __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment_attention_args a, SaPlan p, float keep,
-                                                                     float* __restrict__ dp) {
+                                                                     float* __restrict__ wa, float* __restrict__ wd,
+                                                                     float* __restrict__ share) {
     extern __shared__ float lds[];
     const int H = a.H, t = threadIdx.x;
     float* sA = lds;                       // [eb][H] alpha
     float* sK = sA + p.eb * H;             // [eb][H] keep / (1 - p) or 0
-    float* red = sK + p.eb * H;            // [T]
-    int* sE = reinterpret_cast<int*>(red + p.T);
-    int* sV = sE + p.eb;
+    float* sD = sK + p.eb * H;             // [eb][H] dp
+    float* red = sD + p.eb * H;            // [T]
+    int* sE = reinterpret_cast<int*>(red + p.T);   // [64]
+    int* sV = sE + 64;
     const DrawKey key = a.threshold ? draw_key(a.rng, a.call) : DrawKey{0, 0, 0, 0};
     const int64_t p0 = blockIdx.x * (int64_t)p.eb;
     const int cnt = (int)std::min<int64_t>(p.eb, a.E - p0);
-    for (int i = t; i < cnt; i += p.T) {
-        const int e = a.eid[p0 + i], v = node_of(a.ptr, a.V, (int)p0 + i);
-        sE[i] = e >= 0 && e < a.E ? e : -1;
-        sV[i] = p0 + i >= a.ptr[v] && p0 + i < a.ptr[v + 1] ? v : -1;   // -1: in no list, its gradients are 0
+    if (t < 64) nodes_of_positions(a.ptr, a.V, p0, cnt, sV);
+    else if (t < 64 + cnt) {
+        const int e = a.eid[p0 + t - 64];
+        sE[t - 64] = e >= 0 && e < a.E ? e : -1;
     }
     __syncthreads();
     for (int i = t; i < cnt * H; i += p.T) {
         const int e = sE[i / H], h = i % H;
-        const int64_t v = sV[i / H];
+        const int64_t v = sV[i / H];   // -1: in no list, its gradients are 0
         float al = 0.f, k = 0.f;
         if (e >= 0 && v < 0 && a.dlogits) store_dlogit(a, (int64_t)e * H + h, 0.f);
         if (e >= 0 && v >= 0) {
@@ -409,47 +479,68 @@ __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment
             for (int r = 0; r < rows; ++r)
                 for (int q = 0; q < per; ++q) sum += red[g * (p.RV / p.grp) + r * row_entries + h * per + q];
             const int j = (i0 + g) * H + h;
-            dp[(p0 + i0 + g) * H + h] = sK[j] * sum;
+            sD[j] = sK[j] * sum;
         }
         __syncthreads();
     }
+    if (!a.dlogits) return;
+    for (int k = t; k < cnt * H; k += p.T) {
+        const int i0 = k / H, h = k % H, v = sV[i0];
+        if (v < 0 || (i0 && sV[i0 - 1] == v)) continue;   // a thread per (list, head)
+        int i1 = i0;
+        float s = 0.f;
+        for (; i1 < cnt && sV[i1] == v; ++i1) s += sA[i1 * H + h] * sD[i1 * H + h];
+        const bool before = a.ptr[v] < p0, after = a.ptr[v + 1] > p0 + cnt;
+        if (before || after) share[(2 * (int64_t)blockIdx.x + (before ? 0 : 1)) * H + h] = s;
+        for (int i = i0; i < i1; ++i) {
+            const float al = sA[i * H + h], d = sD[i * H + h];
+            if (before || after) {
+                wa[(p0 + i) * H + h] = al;
+                wd[(p0 + i) * H + h] = d;
+            } else if (sE[i] >= 0) {
+                store_dlogit(a, (int64_t)sE[i] * H + h, al == 0.f ? 0.f : al * (d - s));
+            }
+        }
+    }
 }
 
-// dl = a (dp - sum over the list of a dp): `threads` per node, thread = (position, head)
-__global__ __launch_bounds__(1024) void segment_attention_dlogits_kernel(nbx_segment_attention_args a,
-                                                                         const float* __restrict__ dp) {
-    __shared__ float red[1024];
-    const int t = threadIdx.x, T = blockDim.x, H = a.H;
-    const int64_t v = blockIdx.x;
-    const int j0 = std::max(0, a.ptr[v]), j1 = (int)std::min<int64_t>(a.E, a.ptr[v + 1]);
-    if (j1 <= j0) return;
-    const int step = T / H, h = t % H, r = t / H;
-    const bool on = r < step;
-    const float m = a.stats[v * H + h], inv = a.stats[(a.V + v) * H + h];
-    float s = 0.f;
-    if (on)
-        for (int j = j0 + r; j < j1; j += step) {
-            const int e = a.eid[j];
-            if (e < 0 || e >= a.E) continue;
-            s += weight_of(load_logit(a, (int64_t)e * H + h), m) * inv * dp[(int64_t)j * H + h];
-        }
-    red[t] = s;
+// finishes the lists that cross the block's borders: at most one that began before it and one that goes on
+__global__ __launch_bounds__(256) void segment_attention_dlogits_kernel(nbx_segment_attention_args a, SaPlan p,
+                                                                        const float* __restrict__ wa,
+                                                                        const float* __restrict__ wd,
+                                                                        const float* __restrict__ share) {
+    __shared__ float red[256];
+    __shared__ int sV[64];
+    const int t = threadIdx.x, H = a.H;
+    const int64_t p0 = blockIdx.x * (int64_t)p.eb;
+    const int cnt = (int)std::min<int64_t>(p.eb, a.E - p0);
+    if (t < 64) nodes_of_positions(a.ptr, a.V, p0, cnt, sV);
     __syncthreads();
-    if (t < H) {
-        float d = 0.f;
-        for (int i = 0; i < step; ++i) d += red[i * H + t];
-        red[t] = d;   // only this thread reads the entries h = t
+    const int hs = 256 / H, h = t % H, r = t / H;
+    for (int side = 0; side < 2; ++side) {
+        const int v = side ? sV[cnt - 1] : sV[0];
+        if (v < 0 || (side && v == sV[0])) continue;
+        const int64_t q0 = std::max(0, a.ptr[v]), q1 = std::min<int64_t>(a.E, a.ptr[v + 1]);
+        if (q0 >= p0 && q1 <= p0 + cnt) continue;
+        const int64_t b0 = q0 / p.eb, b1 = (q1 - 1) / p.eb;
+        float s = 0.f;
+        if (r < hs)
+#pragma unroll 4
+            for (int64_t b = b0 + r; b <= b1; b += hs) s += share[(2 * b + (q0 < b * p.eb ? 0 : 1)) * H + h];
+        __syncthreads();
+        red[t] = s;
+        __syncthreads();
+        float delta = 0.f;
+        for (int i = 0; i < hs; ++i) delta += red[i * H + h];
+        const int64_t from = std::max(q0, p0), to = std::min(q1, p0 + cnt);
+        if (r < hs)
+            for (int64_t j = from + r; j < to; j += hs) {
+                const int e = a.eid[j];
+                if (e < 0 || e >= a.E) continue;
+                const float al = wa[j * H + h];
+                store_dlogit(a, (int64_t)e * H + h, al == 0.f ? 0.f : al * (wd[j * H + h] - delta));
+            }
     }
-    __syncthreads();
-    const float delta = red[h];
-    if (on)
-        for (int j = j0 + r; j < j1; j += step) {
-            const int e = a.eid[j];
-            if (e < 0 || e >= a.E) continue;
-            const float al = weight_of(load_logit(a, (int64_t)e * H + h), m) * inv;
-            const float d = al == 0.f ? 0.f : al * (dp[(int64_t)j * H + h] - delta);
-            store_dlogit(a, (int64_t)e * H + h, d);
-        }
 }
 
 // ======================================================================== host
@@ -470,8 +561,7 @@ int sa_check(const nbx_segment_attention_args* a, const char* who) {
     NBX_CHECK_ARG(a->H <= SA_MAXH && a->D <= 4096 && (int64_t)a->H * a->D <= (a->D % 4 == 0 ? 4096 : 1024),
                   "%s: need H <= %d, H D <= 4096 (1024 if D %% 4)", who, SA_MAXH);
     NBX_CHECK_ARG(a->K <= (1 << 22) && a->K * a->H * a->D <= (1 << 22), "%s: rows of more than 2^22 values", who);
-    // a launch's threads along x fit 32 bits (blocks of up to 1024 for a node or a position)
-    NBX_CHECK_ARG(a->V < (1 << 22) || (a->V < (1 << 24) && a->E * a->H < 256 * a->V), "%s: too many nodes", who);
+    NBX_CHECK_ARG(a->V < (1 << 24), "%s: too many nodes", who);   // a launch's threads along x fit 32 bits
     NBX_CHECK_ARG(a->threshold < 65536 && (!a->threshold || a->rng), "%s: need threshold < 65536, and rng for a drop rate",
                   who);
     return NBX_OK;
@@ -499,6 +589,7 @@ SaPlan backward_plan(const nbx_segment_attention_args& a) {
     p.eb = p.RV <= p.T ? std::min(4 * p.EL, TILE) : 4;
     const int g = a.D / VW;
     p.grp = g <= 64 && (g & (g - 1)) == 0 ? g : 1;
+    p.nc = ceil_div(a.E, p.eb);
     return p;
 }
 
@@ -518,7 +609,7 @@ int with_values(const nbx_segment_attention_args& a, F&& f) {
 }
 
 size_t workspace_need(const nbx_segment_attention_args& a, bool backward) {
-    if (backward) return a.dlogits ? (size_t)a.E * a.H * sizeof(float) : 0;
+    if (backward) return a.dlogits ? (size_t)2 * (a.E + backward_plan(a).nc) * a.H * sizeof(float) : 0;
     const SaPlan p = forward_plan(a);
     return p.chunked ? (size_t)2 * p.nc * (a.K * a.H * a.D + 2 * a.H) * sizeof(float) : 0;
 }
@@ -559,15 +650,15 @@ extern "C" int nbx_segment_attention(const nbx_segment_attention_args* a, void* 
         }
         float* pacc = (float*)a->workspace;
         float* pms = pacc + 2 * p.nc * a->K * a->H * a->D;
-        const size_t lds = (size_t)(3 * TILE * a->H + p.T * VW + 2 * TILE) * 4;
-        NBX_CHECK_ARG(lds <= 64 * 1024, "nbx_segment_attention: too many heads");
+        const size_t lds = (size_t)(3 * TILE * a->H + p.T * VW + 2 * TILE) * 4 + TILE * a->H;   // <= 61.5 KB
         if (p.nc) {
             hipLaunchKernelGGL((segment_attention_chunk_kernel<T, VW>), dim3((unsigned)p.nc, (unsigned)p.slices), dim3(p.T),
                                lds, st, *a, p, keep, pacc, pms);
             NBX_LAUNCH_CHECK("segment_attention_chunk");
         }
-        hipLaunchKernelGGL((segment_attention_join_kernel<T, VW>), dim3((unsigned)a->V, (unsigned)p.slices), dim3(p.T), 0,
-                           st, *a, p, keep, pacc, pms);
+        const size_t jlds = (size_t)(2 * TILE * a->H + p.T + a->H + p.T * VW) * 4;
+        hipLaunchKernelGGL((segment_attention_join_kernel<T, VW>), dim3((unsigned)a->V, (unsigned)p.slices), dim3(p.T),
+                           jlds, st, *a, p, keep, pacc, pms);
         NBX_LAUNCH_CHECK("segment_attention_join");
         return NBX_OK;
     });
@@ -584,23 +675,24 @@ extern "C" int nbx_segment_attention_backward(const nbx_segment_attention_args* 
         return NBX_E_WORKSPACE;
     }
     const SaPlan p = backward_plan(*a);
-    NBX_CHECK_ARG(ceil_div(a->E, p.eb) * p.T < ((int64_t)1 << 32), "nbx_segment_attention_backward: too many edges");
+    NBX_CHECK_ARG(p.nc * p.T < ((int64_t)1 << 32), "nbx_segment_attention_backward: too many edges");
     hipStream_t st = (hipStream_t)stream;
     const float keep = keep_scale(a->threshold);
-    float* dp = (float*)a->workspace;
+    float* wa = (float*)a->workspace;
+    float* wd = wa + a->E * a->H;
+    float* share = wd + a->E * a->H;
     if (int rc = with_values(*a, [&](auto t, auto vw) -> int {
             using T = decltype(t);
             constexpr int VW = decltype(vw)::value;
-            const size_t lds = (size_t)(2 * p.eb * a->H + p.T + 2 * p.eb) * 4;
-            hipLaunchKernelGGL((segment_attention_bwd_kernel<T, VW>), dim3((unsigned)ceil_div(a->E, p.eb)), dim3(p.T), lds,
-                               st, *a, p, keep, dp);
+            const size_t lds = (size_t)(3 * p.eb * a->H + p.T + 128) * 4;
+            hipLaunchKernelGGL((segment_attention_bwd_kernel<T, VW>), dim3((unsigned)p.nc), dim3(p.T), lds, st, *a, p, keep,
+                               wa, wd, share);
             NBX_LAUNCH_CHECK("segment_attention_bwd");
             return NBX_OK;
         }))
         return rc;
     if (a->dlogits) {
-        const int threads = a->E * a->H >= 256 * a->V ? 1024 : 64;
-        hipLaunchKernelGGL(segment_attention_dlogits_kernel, dim3((unsigned)a->V), dim3(threads), 0, st, *a, dp);
+        hipLaunchKernelGGL(segment_attention_dlogits_kernel, dim3((unsigned)p.nc), dim3(256), 0, st, *a, p, wa, wd, share);
         NBX_LAUNCH_CHECK("segment_attention_dlogits");
     }
     return NBX_OK;

@@ -88,11 +88,24 @@ __device__ __forceinline__ void store8p(void* p, int dtype, int64_t at, int n, c
     else store8n((f16*)p + at, n, v);
 }
 
-// Sum over the 16 or 64 lanes that share a row.
+// Sum over the 16 or 64 lanes that share a row, in every one of them.  Rotations within 16 lanes are operand
+// modifiers of the add (no LDS permute); the four sixteens are then read as scalars.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
+}
 template <int W>
 __device__ __forceinline__ float lanes_sum(float x) {
-#pragma unroll
-    for (int m = W / 2; m >= 1; m >>= 1) x += __shfl_xor(x, m, 64);
+    static_assert(W == 16 || W == 64, "16 or 64 lanes");
+    x = dpp_add<0x128>(x);   // row_ror:8, 4, 2, 1
+    x = dpp_add<0x124>(x);
+    x = dpp_add<0x122>(x);
+    x = dpp_add<0x121>(x);
+    if constexpr (W == 64) {
+        const int i = __float_as_int(x);
+        x = (__int_as_float(__builtin_amdgcn_readlane(i, 0)) + __int_as_float(__builtin_amdgcn_readlane(i, 16))) +
+            (__int_as_float(__builtin_amdgcn_readlane(i, 32)) + __int_as_float(__builtin_amdgcn_readlane(i, 48)));
+    }
     return x;
 }
 
