@@ -20,31 +20,37 @@ using namespace nbx;
 
 constexpr int TILE = 64;      // positions whose weights are in LDS at once
 constexpr int SA_MAXH = 64;
-constexpr int PREFETCH = 4;   // values of a thread that are loaded before the weights are known
+constexpr int AHEAD = 4;        // values of a thread that are on their way at once
 
+// VW consecutive elements as loaded (RawV: waits only where it is used) and as fp32
 template <typename T, int VW>
 struct VecT {
     typedef T type __attribute__((ext_vector_type(VW), aligned(sizeof(T))));
 };
+template <typename T>
+struct VecT<T, 1> {
+    typedef T type;
+};
 template <typename T, int VW>
-__device__ __forceinline__ void loadv(const T* p, float (&v)[VW]) {
-    if constexpr (VW == 1) {
-        v[0] = (float)p[0];
-    } else {
-        const typename VecT<T, VW>::type t = *reinterpret_cast<const typename VecT<T, VW>::type*>(p);
-#pragma unroll
-        for (int i = 0; i < VW; ++i) v[i] = (float)t[i];
-    }
+using RawV = typename VecT<T, VW>::type;
+template <typename T, int VW>
+__device__ __forceinline__ RawV<T, VW> loadr(const T* p) {
+    return *reinterpret_cast<const RawV<T, VW>*>(p);
+}
+template <typename T, int VW>
+__device__ __forceinline__ float lane_of(const RawV<T, VW>& r, int i) {
+    if constexpr (VW == 1) return (float)r;
+    else return (float)r[i];
 }
 template <typename T, int VW>
 __device__ __forceinline__ void storev(T* p, const float (&v)[VW]) {
     if constexpr (VW == 1) {
         p[0] = (T)v[0];
     } else {
-        typename VecT<T, VW>::type t;
+        RawV<T, VW> t;
 #pragma unroll
         for (int i = 0; i < VW; ++i) t[i] = (T)v[i];
-        *reinterpret_cast<typename VecT<T, VW>::type*>(p) = t;
+        *reinterpret_cast<RawV<T, VW>*>(p) = t;
     }
 }
 
@@ -65,7 +71,8 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 
 struct SaPlan {
     int T, RV, EL, slices;    // threads, vectors per row, edges side by side, blocks per row
-    int eb, TP, grp;          // backward: positions per block, threads that work, lanes of a head that shuffle
+    int eb, TP, grp, entries; // backward: positions per block, threads that work, lanes of a head that shuffle,
+                              // what they leave per position
     int chunked;
     int64_t nc;               // chunks (forward) or blocks (backward)
 };
@@ -107,6 +114,50 @@ __device__ __forceinline__ void nodes_of_positions(const int32_t* __restrict__ p
     }
     const int64_t p = p0 + lane;
     sV[lane] = lane < cnt && p >= ptr[v] && p < ptr[v + 1] ? v : -1;
+}
+
+// The lists that have positions in a block: sP[j] = first position of the j-th, sP[lists] = cnt; returns how
+// many.  One wave, after nodes_of_positions.
+__device__ __forceinline__ int lists_of_positions(const int* sV, int cnt, int* sP) {
+    const int lane = threadIdx.x & 63;
+    const bool first = lane < cnt && (lane == 0 || sV[lane] != sV[lane - 1]);
+    const uint64_t m = __ballot(first);
+    if (first) sP[__popcll(m & (((uint64_t)1 << lane) - 1))] = lane;
+    const int n = __popcll(m);
+    if (lane == 0) sP[n] = cnt;
+    return n;
+}
+
+// max / sum over the 8 lanes of a (list, head)
+__device__ __forceinline__ float max8(float x) {
+#pragma unroll
+    for (int m = 4; m; m >>= 1) x = fmaxf(x, __shfl_xor(x, m, 64));
+    return x;
+}
+__device__ __forceinline__ float sum8(float x) {
+#pragma unroll
+    for (int m = 4; m; m >>= 1) x += __shfl_xor(x, m, 64);
+    return x;
+}
+
+// acc += w[i] row(i) over i = i0, i0 + step, .. < i1, AHEAD rows at a time; a weight of 0 reads nothing
+template <typename T, int VW, typename W, typename R>
+__device__ __forceinline__ void weighted_rows(float (&acc)[VW], int i0, int i1, int step, W&& weight, R&& row) {
+    for (int i = i0; i < i1; i += AHEAD * step) {
+        float w[AHEAD];
+        RawV<T, VW> x[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int k = i + u * step;
+            w[u] = k < i1 ? weight(k) : 0.f;
+            if (w[u] != 0.f) x[u] = loadr<T, VW>(row(k));
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (w[u] != 0.f)
+#pragma unroll
+                for (int k = 0; k < VW; ++k) acc[k] = fmaf(w[u], lane_of<T, VW>(x[u], k), acc[k]);
+    }
 }
 
 // Sum over the EL groups of RV threads (thread = el RV + f), left in group 0.
@@ -159,12 +210,12 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
         }
         __syncthreads();
         // the first values are on their way while the weights are formed
-        float first[PREFETCH][VW];
+        RawV<T, VW> first[AHEAD];
 #pragma unroll
-        for (int k = 0; k < PREFETCH; ++k) {
+        for (int k = 0; k < AHEAD; ++k) {
             const int i = el + k * p.EL;
             if (on && i < cnt && sE[i] >= 0)
-                loadv<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW, first[k]);
+                first[k] = loadr<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW);
         }
         for (int i = t; i < cnt * H; i += p.T) {
             const int e = sE[i / H];
@@ -194,23 +245,15 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
 #pragma unroll
             for (int k = 0; k < VW; ++k) acc[k] *= r;
 #pragma unroll
-            for (int j = 0; j < PREFETCH; ++j) {
+            for (int j = 0; j < AHEAD; ++j) {
                 const int i = el + j * p.EL;
                 const float w = i < cnt ? sW[i * H + head] : 0.f;
                 if (w != 0.f)
 #pragma unroll
-                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, first[j][k], acc[k]);
+                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, lane_of<T, VW>(first[j], k), acc[k]);
             }
-#pragma unroll 4
-            for (int i = el + PREFETCH * p.EL; i < cnt; i += p.EL) {
-                const float w = sW[i * H + head];
-                if (w != 0.f) {
-                    float x[VW];
-                    loadv<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW, x);
-#pragma unroll
-                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, x[k], acc[k]);
-                }
-            }
+            weighted_rows<T, VW>(acc, el + AHEAD * p.EL, cnt, p.EL, [&](int i) { return sW[i * H + head]; },
+                                 [&](int i) { return (const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW; });
         }
     }
     if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
@@ -241,13 +284,18 @@ __global__ __launch_bounds__(256) void segment_attention_chunk_kernel(nbx_segmen
     float* red = sS + TILE * H;
     int* sE = reinterpret_cast<int*>(red + p.T * VW);
     int* sV = sE + TILE;
-    uint8_t* sK = reinterpret_cast<uint8_t*>(sV + TILE);   // [TILE][H]
+    int* sP = sV + TILE;                                   // [TILE + 1], then how many
+    uint8_t* sK = reinterpret_cast<uint8_t*>(sP + TILE + 2);   // [TILE][H]
     note_used(a);
     const DrawKey key = a.threshold ? draw_key(a.rng, a.call) : DrawKey{0, 0, 0, 0};
     const int64_t c = blockIdx.x;
     const int p0 = (int)(c * TILE), cnt = (int)std::min<int64_t>(TILE, a.E - c * TILE);
-    if (t < 64) nodes_of_positions(a.ptr, a.V, p0, cnt, sV);
-    else if (t < 64 + cnt) {
+    if (t < 64) {
+        nodes_of_positions(a.ptr, a.V, p0, cnt, sV);
+        __threadfence_block();
+        const int n = lists_of_positions(sV, cnt, sP);
+        if (t == 0) sP[TILE + 1] = n;
+    } else if (t < 64 + cnt) {
         const int e = a.eid[p0 + t - 64];
         sE[t - 64] = e >= 0 && e < a.E ? e : -1;
     }
@@ -258,19 +306,22 @@ __global__ __launch_bounds__(256) void segment_attention_chunk_kernel(nbx_segmen
         sK[i] = !a.threshold || keep_one(key, (uint64_t)(int64_t)e * H + i % H, a.threshold);
     }
     __syncthreads();
-    for (int k = t; k < cnt * H; k += p.T) {
-        const int i0 = k / H, h = k % H;
-        if (i0 && sV[i0] == sV[i0 - 1]) continue;
-        int i1 = i0;
+    const int lists = sP[TILE + 1];
+    for (int k = t >> 3; k < lists * H; k += p.T >> 3) {   // 8 lanes per (list, head)
+        const int i0 = sP[k / H], i1 = sP[k / H + 1], h = k % H;
         float m = -INFINITY, s = 0.f;
-        for (; i1 < cnt && sV[i1] == sV[i0]; ++i1) m = fmaxf(m, sW[i1 * H + h]);
-        for (int i = i0; i < i1; ++i) {
+        for (int i = i0 + (t & 7); i < i1; i += 8) m = fmaxf(m, sW[i * H + h]);
+        m = max8(m);
+        for (int i = i0 + (t & 7); i < i1; i += 8) {
             const float w = weight_of(sW[i * H + h], finite_max(m));
             s += w;
             sW[i * H + h] = sK[i * H + h] ? w : 0.f;
         }
-        sM[k] = m;
-        sS[k] = s;
+        s = sum8(s);
+        if ((t & 7) == 0) {
+            sM[i0 * H + h] = m;
+            sS[i0 * H + h] = s;
+        }
     }
     __syncthreads();
     const int el = p.slices > 1 ? 0 : t / p.RV;
@@ -278,26 +329,13 @@ __global__ __launch_bounds__(256) void segment_attention_chunk_kernel(nbx_segmen
     const bool on = el < p.EL && f < p.RV;
     const int head = on ? (f * VW / a.D) % H : 0;
     const int64_t RL = (int64_t)p.RV * VW;
-    for (int i0 = 0; i0 < cnt;) {
-        int i1 = i0 + 1;
-        while (i1 < cnt && sV[i1] == sV[i0]) ++i1;
-        const int v = sV[i0];
-        if (v < 0) {
-            i0 = i1;
-            continue;
-        }
+    for (int j = 0; j < lists; ++j) {
+        const int i0 = sP[j], i1 = sP[j + 1], v = sV[i0];
+        if (v < 0) continue;
         float acc[VW] = {};
         if (on)
-#pragma unroll 4
-            for (int i = i0 + el; i < i1; i += p.EL) {
-                const float w = sW[i * H + head];
-                if (w != 0.f) {
-                    float x[VW];
-                    loadv<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW, x);
-#pragma unroll
-                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, x[k], acc[k]);
-                }
-            }
+            weighted_rows<T, VW>(acc, i0 + el, i1, p.EL, [&](int i) { return sW[i * H + head]; },
+                                 [&](int i) { return (const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW; });
         if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
         const bool before = a.ptr[v] < p0, after = a.ptr[v + 1] > p0 + cnt;
         if (before || after) {
@@ -321,7 +359,6 @@ __global__ __launch_bounds__(256) void segment_attention_chunk_kernel(nbx_segmen
                 a.stats[(a.V + v) * H + t] = 1.0f / (sS[i0 * H + t] + 1e-16f);
             }
         }
-        i0 = i1;
     }
 }
 
@@ -375,16 +412,8 @@ __global__ __launch_bounds__(256) void segment_attention_join_kernel(nbx_segment
             sS[t] = s;
         }
         if (on)
-#pragma unroll 4
-            for (int i = el; i < cnt; i += p.EL) {
-                const float w = sR[i * H + head];
-                if (w != 0.f) {
-                    float x[VW];
-                    loadv<float, VW>(pacc + slot(b + i) * RL + (int64_t)f * VW, x);
-#pragma unroll
-                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, x[k], acc[k]);
-                }
-            }
+            weighted_rows<float, VW>(acc, el, cnt, p.EL, [&](int i) { return sR[i * H + head]; },
+                                     [&](int i) { return pacc + slot(b + i) * RL + (int64_t)f * VW; });
     }
     if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
     else __syncthreads();
@@ -415,14 +444,19 @@ __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment
     float* sA = lds;                       // [eb][H] alpha
     float* sK = sA + p.eb * H;             // [eb][H] keep / (1 - p) or 0
     float* sD = sK + p.eb * H;             // [eb][H] dp
-    float* red = sD + p.eb * H;            // [T]
-    int* sE = reinterpret_cast<int*>(red + p.T);   // [64]
+    float* red = sD + p.eb * H;            // [eb][entries]: sums over grp lanes
+    int* sE = reinterpret_cast<int*>(red + p.eb * p.entries);   // [64]
     int* sV = sE + 64;
+    int* sP = sV + 64;                     // [64 + 1], then how many
     const DrawKey key = a.threshold ? draw_key(a.rng, a.call) : DrawKey{0, 0, 0, 0};
     const int64_t p0 = blockIdx.x * (int64_t)p.eb;
     const int cnt = (int)std::min<int64_t>(p.eb, a.E - p0);
-    if (t < 64) nodes_of_positions(a.ptr, a.V, p0, cnt, sV);
-    else if (t < 64 + cnt) {
+    if (t < 64) {
+        nodes_of_positions(a.ptr, a.V, p0, cnt, sV);
+        __threadfence_block();
+        const int n = lists_of_positions(sV, cnt, sP);
+        if (t == 0) sP[65] = n;
+    } else if (t < 64 + cnt) {
         const int e = a.eid[p0 + t - 64];
         sE[t - 64] = e >= 0 && e < a.E ? e : -1;
     }
@@ -445,60 +479,73 @@ __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment
     const bool on = wide ? t < p.TP : el < p.EL;
     const int head = on ? (f0 * VW / a.D) % H : 0;
     const int64_t RL = (int64_t)p.RV * VW;
-    const int per = a.D / VW / p.grp;      // entries of a head and coefficient row in red
-    for (int i0 = 0; i0 < cnt; i0 += p.EL) {
-        const int i = i0 + el;
-        float s = 0.f;
-        if (on && i < cnt && sE[i] >= 0) {
-            const float w = sA[i * H + head] * sK[i * H + head];
-            for (int f = f0; f < p.RV; f += wide ? p.TP : p.RV) {
-                float d[VW], x[VW];
-                loadv<T, VW>((const T*)a.dout + (int64_t)std::max(0, sV[i]) * RL + (int64_t)f * VW, d);
-                if (w != 0.f && a.dlogits) {
-                    loadv<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW, x);
+    // items of a thread: AHEAD of its positions (one vector each), or AHEAD vectors of one position
+    const int nf = wide ? (p.RV + p.TP - 1) / p.TP : 1, items = (wide ? cnt : (cnt + p.EL - 1) / p.EL) * nf;
+    float s = 0.f;
+    for (int q = 0; q < items; q += AHEAD) {
+        RawV<T, VW> d[AHEAD], x[AHEAD];
+        float w[AHEAD];
+        int at[AHEAD], pos[AHEAD];
 #pragma unroll
-                    for (int k = 0; k < VW; ++k) s = fmaf(d[k], x[k], s);
-                }
-                if (a.dvalues) {
-#pragma unroll
-                    for (int k = 0; k < VW; ++k) d[k] = w == 0.f ? 0.f : d[k] * w;
-                    storev<T, VW>((T*)a.dvalues + (int64_t)sE[i] * RL + (int64_t)f * VW, d);
-                }
+        for (int u = 0; u < AHEAD; ++u) {
+            const int k = q + u, i = wide ? k / nf : k * p.EL + el, f = wide ? f0 + k % nf * p.TP : f0;
+            const bool live = on && k < items && i < cnt && f < p.RV && sE[i] >= 0;
+            pos[u] = i;
+            at[u] = live ? f : -1;
+            w[u] = live ? sA[i * H + head] * sK[i * H + head] : 0.f;
+            if (w[u] != 0.f) {
+                d[u] = loadr<T, VW>((const T*)a.dout + (int64_t)sV[i] * RL + (int64_t)f * VW);
+                if (a.dlogits) x[u] = loadr<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW);
             }
         }
-        if (!a.dlogits) continue;
-        for (int m = p.grp >> 1; m; m >>= 1) s += __shfl_xor(s, m, 64);
-        if (on && t % p.grp == 0) red[t / p.grp] = s;
-        __syncthreads();
-        // red: rows of H per entries; a group (or the whole block) holds its threads' rows of them
-        const int rows = (wide ? p.TP : p.RV) / cols, row_entries = cols / p.grp;
-        for (int k = t; k < p.EL * H; k += p.T) {
-            const int g = k / H, h = k % H;
-            if (i0 + g >= cnt) continue;
-            float sum = 0.f;
-            for (int r = 0; r < rows; ++r)
-                for (int q = 0; q < per; ++q) sum += red[g * (p.RV / p.grp) + r * row_entries + h * per + q];
-            const int j = (i0 + g) * H + h;
-            sD[j] = sK[j] * sum;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            float g[VW];
+#pragma unroll
+            for (int k = 0; k < VW; ++k) {
+                const float dk = lane_of<T, VW>(d[u], k);
+                g[k] = w[u] == 0.f ? 0.f : dk * w[u];
+                if (w[u] != 0.f && a.dlogits) s = fmaf(dk, lane_of<T, VW>(x[u], k), s);
+            }
+            if (a.dvalues && at[u] >= 0)
+                storev<T, VW>((T*)a.dvalues + (int64_t)sE[pos[u]] * RL + (int64_t)at[u] * VW, g);
+            if (q + u < items && (!wide || (q + u) % nf == nf - 1)) {   // a position of this thread is complete
+                if (a.dlogits) {
+                    for (int m = p.grp >> 1; m; m >>= 1) s += __shfl_xor(s, m, 64);
+                    if (on && t % p.grp == 0 && pos[u] < cnt) red[pos[u] * p.entries + (wide ? t : f0) / p.grp] = s;
+                }
+                s = 0.f;
+            }
         }
-        __syncthreads();
     }
     if (!a.dlogits) return;
+    __syncthreads();
+    // red: a position's entries are rows of `per` per head
+    const int per = a.D / VW / p.grp, rows = p.entries / (cols / p.grp);
     for (int k = t; k < cnt * H; k += p.T) {
-        const int i0 = k / H, h = k % H, v = sV[i0];
-        if (v < 0 || (i0 && sV[i0 - 1] == v)) continue;   // a thread per (list, head)
-        int i1 = i0;
-        float s = 0.f;
-        for (; i1 < cnt && sV[i1] == v; ++i1) s += sA[i1 * H + h] * sD[i1 * H + h];
+        const float* r = red + k / H * p.entries + k % H * per;
+        float sum = 0.f;
+        for (int j = 0; j < rows; ++j)
+            for (int i = 0; i < per; ++i) sum += r[j * (cols / p.grp) + i];
+        sD[k] = sK[k] == 0.f ? 0.f : sK[k] * sum;
+    }
+    __syncthreads();
+    const int lists = sP[65];
+    for (int k = t >> 3; k < lists * H; k += p.T >> 3) {   // 8 lanes per (list, head)
+        const int i0 = sP[k / H], i1 = sP[k / H + 1], h = k % H, v = sV[i0];
+        float d = 0.f;
+        for (int i = i0 + (t & 7); i < i1; i += 8) d += sA[i * H + h] * sD[i * H + h];
+        d = sum8(d);
+        if (v < 0) continue;
         const bool before = a.ptr[v] < p0, after = a.ptr[v + 1] > p0 + cnt;
-        if (before || after) share[(2 * (int64_t)blockIdx.x + (before ? 0 : 1)) * H + h] = s;
-        for (int i = i0; i < i1; ++i) {
-            const float al = sA[i * H + h], d = sD[i * H + h];
+        if ((before || after) && (t & 7) == 0) share[(2 * (int64_t)blockIdx.x + (before ? 0 : 1)) * H + h] = d;
+        for (int i = i0 + (t & 7); i < i1; i += 8) {
+            const float al = sA[i * H + h], dp = sD[i * H + h];
             if (before || after) {
                 wa[(p0 + i) * H + h] = al;
-                wd[(p0 + i) * H + h] = d;
+                wd[(p0 + i) * H + h] = dp;
             } else if (sE[i] >= 0) {
-                store_dlogit(a, (int64_t)sE[i] * H + h, al == 0.f ? 0.f : al * (d - s));
+                store_dlogit(a, (int64_t)sE[i] * H + h, al == 0.f ? 0.f : al * (dp - d));
             }
         }
     }
@@ -586,9 +633,14 @@ SaPlan backward_plan(const nbx_segment_attention_args& a) {
     p.RV = (int)(a.K * a.H * a.D / VW);
     p.EL = p.RV <= p.T ? std::min(p.T / p.RV, TILE) : 1;
     p.TP = p.RV <= p.T ? p.RV * p.EL : p.T / cols * cols;
-    p.eb = p.RV <= p.T ? std::min(4 * p.EL, TILE) : 4;
     const int g = a.D / VW;
     p.grp = g <= 64 && (g & (g - 1)) == 0 ? g : 1;
+    p.entries = std::min(p.RV, p.TP) / p.grp;
+    // positions per block: enough blocks for the chip first, then few (each has its searches and sums), within
+    // 48 KB of LDS
+    p.eb = p.RV <= p.T ? TILE : 4;
+    while (p.eb > 4 && (a.E < 1024 * (int64_t)p.eb || p.eb * (p.entries + 3 * a.H) > 12288)) p.eb /= 2;
+    p.eb = std::max(p.eb, std::min(p.EL, TILE));
     p.nc = ceil_div(a.E, p.eb);
     return p;
 }
@@ -650,7 +702,7 @@ extern "C" int nbx_segment_attention(const nbx_segment_attention_args* a, void* 
         }
         float* pacc = (float*)a->workspace;
         float* pms = pacc + 2 * p.nc * a->K * a->H * a->D;
-        const size_t lds = (size_t)(3 * TILE * a->H + p.T * VW + 2 * TILE) * 4 + TILE * a->H;   // <= 61.5 KB
+        const size_t lds = (size_t)(3 * TILE * a->H + p.T * VW + 3 * TILE + 2) * 4 + TILE * a->H;   // <= 62 KB
         if (p.nc) {
             hipLaunchKernelGGL((segment_attention_chunk_kernel<T, VW>), dim3((unsigned)p.nc, (unsigned)p.slices), dim3(p.T),
                                lds, st, *a, p, keep, pacc, pms);
@@ -684,7 +736,7 @@ extern "C" int nbx_segment_attention_backward(const nbx_segment_attention_args* 
     if (int rc = with_values(*a, [&](auto t, auto vw) -> int {
             using T = decltype(t);
             constexpr int VW = decltype(vw)::value;
-            const size_t lds = (size_t)(3 * p.eb * a->H + p.T + 128) * 4;
+            const size_t lds = (size_t)(3 * p.eb * a->H + p.eb * p.entries + 196) * 4;
             hipLaunchKernelGGL((segment_attention_bwd_kernel<T, VW>), dim3((unsigned)p.nc), dim3(p.T), lds, st, *a, p, keep,
                                wa, wd, share);
             NBX_LAUNCH_CHECK("segment_attention_bwd");
