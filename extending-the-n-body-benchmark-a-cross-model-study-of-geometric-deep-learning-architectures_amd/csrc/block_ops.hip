@@ -8,6 +8,7 @@
 // (mean, then squares around it) cost no second read.  Column sums (parameter gradients) stay in registers
 // over a block's rows, then one partial row per block is summed by a second launch in a fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include "nbx_internal.h"
 #include "philox.h"
@@ -164,10 +165,14 @@ __global__ __launch_bounds__(W ? 256 : 1024) void residual_norm_kernel(nbx_resid
     const int C = (int)a.C, c0 = 8 * lane, n = std::max(0, std::min(8, C - c0));
     Draws d = {{0, 0, 0, 0}, a.threshold, a.group, (a.C + 7) >> 3, keep};
     if (a.threshold) d.key = draw_key(a.rng, a.call);
+    Raw8<TX> rx;
+    Raw8<TY> ry;
+    fetch8n((const TX*)a.x + r * a.ldx + c0, n, rx);
+    fetch8n((const TY*)a.y + r * a.ldy + c0, n, ry);
+    const uint32_t m = row_keep(d, r, lane);   // while the rows are on their way
     float x[8], u[8], w[8], b[8];
-    load8n((const TX*)a.x + r * a.ldx + c0, n, x);
-    load8n((const TY*)a.y + r * a.ldy + c0, n, u);
-    const uint32_t m = row_keep(d, r, lane);
+    unpack8(rx, x);
+    unpack8(ry, u);
     if (a.post_w) {
         float mu, rs;
         row_stats<W>(u, n, C, a.norm, a.eps, mu, rs, red, slot);
@@ -205,22 +210,27 @@ __global__ __launch_bounds__(W ? 256 : 1024) void residual_norm_kernel(nbx_resid
     }
 }
 
-// Which rows a block of the backward pass owns.  ALIGNED: rows [g rpg + k cs, ..) of gate group g, k = block
-// % cpg: a group's gate gradient is the sum of its cpg partial rows.  WHOLE (groups shorter than a block's
-// share): every row slot owns gps whole groups and writes their gate gradients itself.
+// Which rows a block of the backward pass owns.  A block has `rpb` row slots: 16 or 64 lanes, or (W = 0) nw
+// waves each.  ALIGNED: rows [g rpg + k cs, ..) of gate group g, k = block % cpg, dealt to the slots in turn.
+// WHOLE (groups shorter than a block's share): every slot owns gps whole groups.  The slots of a block run the
+// same number of rows, so that they can share barriers.
 struct RowPlan {
     int64_t rpg, cs, cpg, gps, nblocks;
-    int whole, W, rpb, threads;
+    int whole, W, nw, rpb, threads;
 };
 
 RowPlan row_plan(int64_t rows, int64_t C, int64_t gate_groups) {
     RowPlan p = {};
-    p.W = C <= 128 ? 16 : C <= 512 ? 64 : 0;
-    p.threads = p.W ? 256 : (int)(ceil_div(C, 512) * 64);
-    p.rpb = p.W ? 256 / p.W : 1;
+    p.W = C <= 128 ? 16 : C <= 512 ? 64 : C <= 2048 ? 0 : -1;
+    p.nw = (int)ceil_div(C, 512);
+    p.rpb = p.W > 0 ? 256 / p.W : std::max(1, 4 / p.nw);
+    p.threads = p.W > 0 ? 256 : p.rpb * p.nw * 64;
     const int64_t groups = gate_groups > 0 && gate_groups < rows ? gate_groups : 1;
     p.rpg = rows / groups;
-    const int64_t chunk = std::max<int64_t>(4 * p.rpb, ceil_div(rows, 1024));
+    // up to 768 blocks, three on each CU at its 168 registers; each leaves one partial row per sum, read once
+    // more.  16384 rows of 2048 bf16 columns, kernel + sums: 109 + 10 us at 512 blocks, 94 + 14 at 768, 110 + 18
+    // at 1024 (149 + 19 at four blocks to a CU: the registers spill)
+    const int64_t chunk = std::max<int64_t>(p.rpb, ceil_div(rows, 768));
     p.whole = p.rpg < chunk && groups > 1;
     if (p.whole) {
         p.gps = std::max<int64_t>(1, chunk / p.rpb / p.rpg);
@@ -234,175 +244,290 @@ RowPlan row_plan(int64_t rows, int64_t C, int64_t gate_groups) {
     return p;
 }
 
-enum { SUM_POST_W, SUM_POST_B, SUM_PRE_W, SUM_PRE_B, SUM_GATE, SUMS };
+// Partial sums per block and column.  A gate shared by a block's rows is taken out of them: SUM_A = sum of du
+// yhat (du y without a norm of y), SUM_B = sum of du, du = the gradient behind the gate.  OWN (a gate per row,
+// or WHOLE) has the gate inside: SUM_A = sum of dn yhat, SUM_B = sum of dn, dn = du gate.
+enum { SUM_A, SUM_B, SUM_PRE_W, SUM_PRE_B, SUMS };
 
-template <typename TX, typename TY, int W>
-__global__ __launch_bounds__(W ? 256 : 1024) void residual_norm_bwd_kernel(nbx_residual_norm_args a, RowPlan p,
-                                                                           float keep, float* __restrict__ part) {
-    __shared__ float red[4][16];
-    __shared__ float comb[W ? 2048 : 1];
-    int slot = 0;
-    constexpr int RPB = W ? 256 / (W ? W : 1) : 1;
-    const int lane = W ? (int)threadIdx.x % (W ? W : 1) : (int)threadIdx.x;
-    const int mine = W ? (int)threadIdx.x / (W ? W : 1) : 0;
-    const int C = (int)a.C, c0 = 8 * lane, n = std::max(0, std::min(8, C - c0));
+template <typename TX, typename TY>
+struct RowIn {   // a row's eight columns as loaded, one row ahead of their use
+    Raw8<TX> dh, h;
+    Raw8<TY> dz, y;
+    float mu1, rs1, mu2, rs2;
+    int64_t r;
+    int n;
+};
+
+template <typename TX, typename TY, int W, bool NORM, bool OWN>
+__global__ __launch_bounds__(W >= 0 ? 256 : 1024, W >= 0 ? 3 : 1) void residual_norm_bwd_kernel(nbx_residual_norm_args a, RowPlan p,
+                                                                                    float keep,
+                                                                                    float* __restrict__ part) {
+    __shared__ float red[4][16][2];
+    __shared__ float comb[W >= 0 ? 2048 : 1];
+    int turn = 0;
+    const int slot_threads = W > 0 ? W : p.nw * 64;
+    // a wave has one row (but for the 16-lane form): the row's addresses and statistics are scalars
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int mine = W == 16 ? (int)threadIdx.x / 16 : W > 0 ? wave : wave / p.nw;
+    const int lane = (int)threadIdx.x - mine * slot_threads;
+    const int C = (int)a.C, c0 = 8 * lane, cn = std::max(0, std::min(8, C - c0));
+    // two sums over a slot's threads at once
+    auto slot_sums = [&](float& x, float& y) {
+        if constexpr (W > 0) {
+            x = lanes_sum<W>(x);
+            y = lanes_sum<W>(y);
+        } else {
+            x = lanes_sum<64>(x);
+            y = lanes_sum<64>(y);
+            float(*r)[2] = red[turn];
+            turn = (turn + 1) & 3;
+            if ((threadIdx.x & 63) == 0) {
+                r[threadIdx.x >> 6][0] = x;
+                r[threadIdx.x >> 6][1] = y;
+            }
+            __syncthreads();
+            x = y = 0.f;
+            for (int i = 0; i < p.nw; ++i) {
+                x += r[mine * p.nw + i][0];
+                y += r[mine * p.nw + i][1];
+            }
+        }
+    };
     Draws d = {{0, 0, 0, 0}, a.threshold, a.group, (a.C + 7) >> 3, keep};
     if (a.threshold) d.key = draw_key(a.rng, a.call);
     const float s = a.scale * keep, invC = 1.0f / (float)C;
-    const bool rowgate = a.gate && a.gate_groups == a.rows && a.rows > 1;
-    const bool gsum = a.dgate && !rowgate;
-    float acc[SUMS][8] = {};
-    float pw[8], pb[8] = {}, qw[8], gt[8];
-    if (a.post_w) load8p(a.post_w, a.param_dtype, c0, n, pw);
-    if (a.post_b) load8p(a.post_b, a.param_dtype, c0, n, pb);
-    if (a.pre_w) load8p(a.pre_w, a.param_dtype, c0, n, qw);
-    int64_t g0, g1, r0, r1, step;
-    const int64_t groups = a.gate && !rowgate ? a.gate_groups : 1;
+    const bool rowgate = OWN && !p.whole, post = NORM && a.post_w, pre = NORM && a.pre_w && a.dz;
+    const bool need_y = post || a.dgate;
+    float acc[SUMS][8] = {}, ag[OWN ? 8 : 1] = {};
+    float pw[8], pb[OWN ? 8 : 1] = {}, qw[8], gt[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) gt[i] = 1.f;
+    if (post) load8p(a.post_w, a.param_dtype, c0, cn, pw);
+    if constexpr (OWN)
+        if (post && a.post_b) load8p(a.post_b, a.param_dtype, c0, cn, pb);
+    if (pre) load8p(a.pre_w, a.param_dtype, c0, cn, qw);
+    // the slot's rows: first, past the last, step; all slots of a block run `iters` rows
+    int64_t r0, r1, step, iters, left = 0;
     if (p.whole) {
-        const int64_t unit = blockIdx.x * (int64_t)RPB + mine;
-        g0 = std::min(unit * p.gps, groups);
-        g1 = std::min(g0 + p.gps, groups);
-        r0 = 0;
-        r1 = p.rpg;
+        const int64_t unit = blockIdx.x * (int64_t)p.rpb + mine;
+        r0 = std::min(unit * p.gps * p.rpg, a.rows);
+        r1 = std::min(r0 + p.gps * p.rpg, a.rows);
         step = 1;
+        iters = p.gps * p.rpg;
     } else {
-        g0 = blockIdx.x / p.cpg;
-        g1 = g0 + 1;
-        r0 = blockIdx.x % p.cpg * p.cs;
-        r1 = std::min(r0 + p.cs, p.rpg);
-        r0 += mine;
-        step = RPB;
+        const int64_t g = blockIdx.x / p.cpg, k0 = blockIdx.x % p.cpg * p.cs;
+        r0 = g * p.rpg + k0 + mine;
+        r1 = g * p.rpg + std::min(k0 + p.cs, p.rpg);
+        step = p.rpb;
+        iters = (p.cs + p.rpb - 1) / p.rpb;
+        if constexpr (!OWN) {
+            if (a.gate) load8p(a.gate, a.param_dtype, g * a.C + c0, cn, gt);
+            if (post)   // the norm's weight and the gate act on the same values
+#pragma unroll
+                for (int i = 0; i < 8; ++i) gt[i] *= i < cn ? pw[i] : 0.f;
+        }
     }
-    for (int64_t g = g0; g < g1; ++g) {
-        if (a.gate && !rowgate) load8p(a.gate, a.param_dtype, g * a.C + c0, n, gt);
-        for (int64_t rr = r0; rr < r1; rr += step) {
-            const int64_t r = g * p.rpg + rr;
-            float t[8], v[8], e[8];
-            if (a.dh) load8n((const TX*)a.dh + r * a.C + c0, n, t);
-            else
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = 0.f;
-            if (a.pre_w && a.dz) {
-                load8n((const TY*)a.dz + r * a.C + c0, n, e);
-                load8n((const TX*)a.h + r * a.C + c0, n, v);
-                const float mu = a.stats[2 * a.rows + r], rs = a.stats[3 * a.rows + r];
-                float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    v[i] = (v[i] - mu) * rs;   // from h as it is stored
-                    acc[SUM_PRE_W][i] += e[i] * v[i];
-                    acc[SUM_PRE_B][i] += e[i];
-                    e[i] = i < n ? e[i] * qw[i] : 0.f;
-                    s1 += e[i];
-                    s2 += e[i] * v[i];
-                }
-                s1 = a.norm ? 0.f : row_sum<W>(s1, red, slot) * invC;
-                s2 = row_sum<W>(s2, red, slot) * invC;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] += rs * (e[i] - s1 - v[i] * s2);
-            }
-            if (a.dx) store8n((TX*)a.dx + r * a.C + c0, n, t);
-            const uint32_t m = row_keep(d, r, lane);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = (m >> i & 1) ? s * t[i] : 0.f;
-            float mu = 0.f, rs = 1.f;
-            if (a.post_w || a.dgate) {
-                load8n((const TY*)a.y + r * a.ldy + c0, n, v);
-                if (a.post_w) {
-                    mu = a.stats[r];
-                    rs = a.stats[a.rows + r];
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = (v[i] - mu) * rs;
-            }
-            if (a.gate) {
-                if (rowgate) load8p(a.gate, a.param_dtype, r * a.C + c0, n, gt);
-                if (a.dgate) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float u = a.post_w ? v[i] * pw[i] + pb[i] : v[i];
-                        e[i] = (m >> i & 1) ? t[i] * u : 0.f;   // a dropped place counts 0 whatever it held
-                        acc[SUM_GATE][i] += e[i];
-                    }
-                    if (rowgate) store8p(a.dgate, a.param_dtype, r * a.C + c0, n, e);
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] *= gt[i];
-            }
-            if (a.post_w) {
-                float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    acc[SUM_POST_W][i] += t[i] * v[i];
-                    acc[SUM_POST_B][i] += t[i];
-                    t[i] = i < n ? t[i] * pw[i] : 0.f;
-                    s1 += t[i];
-                    s2 += t[i] * v[i];
-                }
-                s1 = a.norm ? 0.f : row_sum<W>(s1, red, slot) * invC;
-                s2 = row_sum<W>(s2, red, slot) * invC;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = rs * (t[i] - s1 - v[i] * s2);
-            }
-            if (a.dy) store8n((TY*)a.dy + r * a.C + c0, n, t);
+    using In = RowIn<TX, TY>;
+    auto fetch = [&](int64_t r, In& in) {
+        in.n = r < r1 ? cn : 0;
+        in.r = r < r1 ? r : 0;
+        const int64_t row = in.r * a.C;
+        fetch8n((const TX*)a.dh + row + (uint32_t)c0, a.dh ? in.n : 0, in.dh);
+        if (pre) {
+            fetch8n((const TY*)a.dz + row + (uint32_t)c0, in.n, in.dz);
+            fetch8n((const TX*)a.h + row + (uint32_t)c0, in.n, in.h);
+            in.mu2 = a.stats[2 * a.rows + in.r];
+            in.rs2 = a.stats[3 * a.rows + in.r];
         }
-        if (gsum && p.whole) {
-            store8p(a.dgate, a.param_dtype, g * a.C + c0, n, acc[SUM_GATE]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[SUM_GATE][i] = 0.f;
+        if (need_y) fetch8n((const TY*)a.y + in.r * a.ldy + (uint32_t)c0, in.n, in.y);
+        if (post) {
+            in.mu1 = a.stats[in.r];
+            in.rs1 = a.stats[a.rows + in.r];
         }
+    };
+    In in;
+    fetch(r0, in);
+    for (int64_t i = 0; i < iters; ++i) {
+        In next;
+        if (i + 1 < iters) fetch(r0 + (i + 1) * step, next);
+        const int n = in.n;
+        const int64_t row = in.r * a.C;
+        if constexpr (OWN) {
+            if (rowgate) load8p(a.gate, a.param_dtype, row + (uint32_t)c0, n, gt);
+            else if (left == 0) load8p(a.gate, a.param_dtype, in.r / p.rpg * a.C + c0, n, gt);
+        }
+        float t[8], v[8], e[8];
+        unpack8(in.dh, t);
+        if (pre) {
+            unpack8(in.dz, e);
+            unpack8(in.h, v);
+            float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] = (v[k] - in.mu2) * in.rs2;   // from h as it is stored
+                acc[SUM_PRE_W][k] += e[k] * v[k];  // past the row e is 0
+                acc[SUM_PRE_B][k] += e[k];
+                e[k] *= k < n ? qw[k] : 0.f;
+                s1 += e[k];
+                s2 += e[k] * v[k];
+            }
+            slot_sums(s1, s2);
+            s1 = a.norm ? 0.f : s1 * invC;
+            s2 *= invC;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] += in.rs2 * (e[k] - s1 - v[k] * s2);
+        }
+        if (a.dx) store8n((TX*)a.dx + row + (uint32_t)c0, n, t);
+        const uint32_t m = row_keep(d, in.r, lane);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = (m >> k & 1) && k < n ? s * t[k] : 0.f;
+        if (need_y) {
+            unpack8(in.y, v);
+            if (post)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = (v[k] - in.mu1) * in.rs1;
+        }
+        if constexpr (OWN) {
+            if (a.dgate) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float u = post ? v[k] * pw[k] + pb[k] : v[k];
+                    e[k] = (m >> k & 1) ? t[k] * u : 0.f;   // a dropped place counts 0 whatever it held
+                    ag[k] += e[k];
+                }
+                if (rowgate) store8p(a.dgate, a.param_dtype, row + (uint32_t)c0, n, e);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] *= gt[k];
+        }
+        if (post || (!OWN && a.dgate))
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                acc[SUM_A][k] += (m >> k & 1) ? t[k] * v[k] : 0.f;
+                acc[SUM_B][k] += t[k];
+            }
+        if constexpr (!OWN)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] *= gt[k];
+        if (post) {
+            float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if constexpr (OWN) t[k] *= k < n ? pw[k] : 0.f;
+                s1 += t[k];
+                s2 += t[k] * v[k];
+            }
+            slot_sums(s1, s2);
+            s1 = a.norm ? 0.f : s1 * invC;
+            s2 *= invC;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = in.rs1 * (t[k] - s1 - v[k] * s2);
+        }
+        if (a.dy) store8n((TY*)a.dy + row + (uint32_t)c0, n, t);
+        if constexpr (OWN) {
+            left = left + 1 == p.rpg ? 0 : left + 1;
+            if (p.whole && left == 0 && a.dgate) {   // a whole gate group ends: this slot had all of it
+                float g[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    g[k] = ag[k];
+                    ag[k] = 0.f;
+                }
+                store8p(a.dgate, a.param_dtype, in.r / p.rpg * a.C + c0, n, g);
+            }
+        }
+        in = next;
     }
     // one partial row per block and sum: part[sum][block][C]
 #pragma unroll
     for (int k = 0; k < SUMS; ++k) {
-        const bool want = k == SUM_POST_W ? a.dpost_w != nullptr : k == SUM_POST_B ? a.dpost_b != nullptr
-                        : k == SUM_PRE_W ? a.dpre_w != nullptr : k == SUM_PRE_B ? a.dpre_b != nullptr
-                        : gsum && !p.whole;
+        const bool want = k == SUM_A ? a.dpost_w || (!OWN && a.dgate) : k == SUM_B ? a.dpost_b || (!OWN && a.dgate && post)
+                        : k == SUM_PRE_W ? a.dpre_w != nullptr : a.dpre_b != nullptr;
         if (!want) continue;
         float* to = part + ((int64_t)k * p.nblocks + blockIdx.x) * a.C;
-        if constexpr (W == 0) {
-            store8n(to + c0, n, acc[k]);
+        if (p.rpb == 1) {
+            store8n(to + c0, cn, acc[k]);
         } else {
+            const int ld = 8 * slot_threads;
             __syncthreads();
-            store8(comb + mine * 8 * W + c0, acc[k]);
+            store8(comb + mine * ld + c0, acc[k]);
             __syncthreads();
-            for (int c = threadIdx.x; c < C; c += 256) {
+            for (int c = threadIdx.x; c < C; c += blockDim.x) {
                 float t = 0.f;
-#pragma unroll 4
-                for (int q = 0; q < RPB; ++q) t += comb[q * 8 * W + c];
+                for (int q = 0; q < p.rpb; ++q) t += comb[q * ld + c];
                 to[c] = t;
             }
         }
     }
 }
 
-// Column sums of the partial rows: job j < 4: a parameter gradient over all blocks; job 4 + g: gate group g
-// over its cpg blocks.  64 columns x 16 waves, each wave every 16th row, combined in order.
+// Column sums of the partial rows.  The first jobs * ceil(C / 64) blocks: a parameter over all blocks (dpost_*
+// with each block's gate row put back), 64 columns x 16 waves, each wave every 16th row, combined in order.
+// Then gate group after group over its cpg blocks: the same, or (cpg <= 16) a thread per column.
+enum { OUT_POST_W, OUT_POST_B, OUT_PRE_W, OUT_PRE_B, OUTS };
 struct FinalSums {
-    void* out[SUMS];
+    void* out[OUTS];
+    void* dgate;
+    const void *gate, *post_w, *post_b;   // gate NULL: it is in the sums already
     int dtype, jobs;
-    int job[SUMS];
+    int job[OUTS];
 };
+
+__device__ __forceinline__ float load1p(const void* p, int dtype, int64_t at) {
+    return dtype == NBX_F32 ? ((const float*)p)[at]
+         : dtype == NBX_BF16 ? (float)((const bf16*)p)[at] : (float)((const f16*)p)[at];
+}
 
 __global__ __launch_bounds__(1024) void residual_norm_sums_kernel(FinalSums f, int64_t nblocks, int64_t cpg, int64_t C,
                                                                   const float* __restrict__ part) {
-    __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t c = blockIdx.x * (int64_t)64 + lane;
-    const int k = (int)blockIdx.y < f.jobs ? f.job[blockIdx.y] : SUM_GATE;
-    const int64_t g = (int)blockIdx.y < f.jobs ? 0 : blockIdx.y - f.jobs;
-    const int64_t b0 = k == SUM_GATE ? g * cpg : 0, nb = k == SUM_GATE ? cpg : nblocks;
-    const float* p = part + ((int64_t)k * nblocks + b0) * C + c;
-    float s = 0.f;
-    if (c < C)
-        for (int64_t b = w; b < nb; b += 16) s += p[b * C];
-    red[w][lane] = s;
-    __syncthreads();
-    if (w == 0 && c < C) {
-        float t = 0.f;
+    __shared__ float red[2][16][64];
+    const int tiles = (int)((C + 63) / 64), job = (int)blockIdx.x / tiles;
+    const bool gates = job >= f.jobs, thread_per_column = gates && cpg <= 16;
+    const int gtiles = cpg <= 16 ? (int)((C + 1023) / 1024) : tiles, gb = (int)blockIdx.x - f.jobs * tiles;
+    const int lane = threadIdx.x & 63, w = thread_per_column ? 0 : threadIdx.x >> 6;
+    const int64_t c = thread_per_column ? gb % gtiles * (int64_t)1024 + threadIdx.x
+                                        : (gates ? gb % gtiles : (int)blockIdx.x % tiles) * (int64_t)64 + lane;
+    const int k = gates ? SUM_A : f.job[job], step = thread_per_column ? 1 : 16;
+    const int64_t g = gates ? gb / gtiles : 0;
+    const int nb = (int)(gates ? cpg : nblocks);
+    const float* p = part + ((int64_t)k * nblocks + g * cpg) * C + c;
+    const bool scaled = !gates && f.gate && k <= OUT_POST_B, both = gates && f.post_w;
+    float s = 0.f, s2 = 0.f;
+    if (c < C) {
+        if (scaled) {
+            auto with_gate = [&](auto* gate) {
+#pragma unroll 8
+                for (int b = w; b < nb; b += step) s += p[b * C] * (float)gate[b / (int)cpg * C + c];
+            };
+            if (f.dtype == NBX_F32) with_gate((const float*)f.gate);
+            else if (f.dtype == NBX_BF16) with_gate((const bf16*)f.gate);
+            else with_gate((const f16*)f.gate);
+        } else {
+#pragma unroll 8
+            for (int b = w; b < nb; b += step) s += p[b * C];
+            if (both)
+#pragma unroll 8
+                for (int b = w; b < nb; b += step) s2 += p[(nblocks + b) * C];
+        }
+    }
+    if (!thread_per_column) {
+        red[0][w][lane] = s;
+        red[1][w][lane] = s2;
+        __syncthreads();
+        if (w) return;
+        s = s2 = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t += red[i][lane];
-        store1p(f.out[k], f.dtype, g * C + c, t);
+        for (int i = 0; i < 16; ++i) {
+            s += red[0][i][lane];
+            s2 += red[1][i][lane];
+        }
+    }
+    if (c >= C) return;
+    if (!gates) {
+        store1p(f.out[k], f.dtype, c, s);
+    } else {
+        if (both) s = s * load1p(f.post_w, f.dtype, c) + (f.post_b ? s2 * load1p(f.post_b, f.dtype, c) : 0.f);
+        store1p(f.dgate, f.dtype, g * C + c, s);
     }
 }
 
@@ -710,7 +835,7 @@ __global__ __launch_bounds__(1024) void sh_residual_sums_kernel(nbx_sh_residual_
 // the units (nodes in flight) of the backward pass: its partial rows are read and written once more
 int64_t sh_units(const ShPlan& p, int64_t V) {
     const int64_t most = 512 * (int64_t)p.npb;
-    return std::max<int64_t>(1, ceil_div(std::min(most, ceil_div(V, 4)), p.npb)) * p.npb;
+    return ceil_div(std::min(most, V), p.npb) * p.npb;
 }
 
 size_t sh_workspace(const ShPlan& p, int64_t V, int lmax, int C) {
@@ -803,16 +928,16 @@ extern "C" int nbx_residual_norm(const nbx_residual_norm_args* a, void* stream) 
     if (int rc = residual_check(a, "nbx_residual_norm")) return rc;
     if (a->rows == 0) return NBX_OK;
     NBX_CHECK_ARG(a->x && a->y && a->h && (!a->pre_w || a->z), "nbx_residual_norm: null operand");
-    const RowPlan p = row_plan(a->rows, a->C, 0);
-    NBX_CHECK_ARG(grid_ok(ceil_div(a->rows, p.rpb), p.threads), "nbx_residual_norm: too many rows");
-    const unsigned blocks = (unsigned)ceil_div(a->rows, p.rpb);
+    const int W = a->C <= 128 ? 16 : a->C <= 512 ? 64 : 0, threads = W ? 256 : (int)ceil_div(a->C, 512) * 64;
+    const int64_t blocks = ceil_div(a->rows, W ? 256 / W : 1);
+    NBX_CHECK_ARG(grid_ok(blocks, threads), "nbx_residual_norm: too many rows");
     const float keep = keep_scale(a->threshold);
     return with_types(*a, [&](auto x, auto y) -> int {
         using TX = decltype(x);
         using TY = decltype(y);
-        auto k = p.W == 16 ? residual_norm_kernel<TX, TY, 16> : p.W == 64 ? residual_norm_kernel<TX, TY, 64>
-                                                                          : residual_norm_kernel<TX, TY, 0>;
-        hipLaunchKernelGGL(k, dim3(blocks), dim3(p.threads), 0, (hipStream_t)stream, *a, keep);
+        auto k = W == 16 ? residual_norm_kernel<TX, TY, 16> : W == 64 ? residual_norm_kernel<TX, TY, 64>
+                                                                      : residual_norm_kernel<TX, TY, 0>;
+        hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(threads), 0, (hipStream_t)stream, *a, keep);
         NBX_LAUNCH_CHECK("residual_norm");
         return NBX_OK;
     });
@@ -845,24 +970,32 @@ extern "C" int nbx_residual_norm_backward(const nbx_residual_norm_args* a, void*
     hipStream_t st = (hipStream_t)stream;
     const float keep = keep_scale(a->threshold);
     float* part = (float*)a->workspace;
+    const bool own = a->gate && (p.whole || (a->gate_groups == rows && rows > 1));
     if (int rc = with_types(*a, [&](auto x, auto y) -> int {
             using TX = decltype(x);
             using TY = decltype(y);
-            auto k = p.W == 16 ? residual_norm_bwd_kernel<TX, TY, 16>
-                   : p.W == 64 ? residual_norm_bwd_kernel<TX, TY, 64> : residual_norm_bwd_kernel<TX, TY, 0>;
+            const bool norm = a->post_w || a->pre_w;
+            auto pick = [&](auto w) {
+                constexpr int W = decltype(w)::value;
+                return norm ? (own ? residual_norm_bwd_kernel<TX, TY, W, true, true> : residual_norm_bwd_kernel<TX, TY, W, true, false>)
+                            : (own ? residual_norm_bwd_kernel<TX, TY, W, false, true> : residual_norm_bwd_kernel<TX, TY, W, false, false>);
+            };
+            auto k = p.W == 16 ? pick(std::integral_constant<int, 16>{}) : p.W == 64 ? pick(std::integral_constant<int, 64>{})
+                   : p.W == 0 ? pick(std::integral_constant<int, 0>{}) : pick(std::integral_constant<int, -1>{});
             hipLaunchKernelGGL(k, dim3((unsigned)p.nblocks), dim3(p.threads), 0, st, *a, p, keep, part);
             NBX_LAUNCH_CHECK("residual_norm_bwd");
             return NBX_OK;
         }))
         return rc;
-    FinalSums f = {{a->dpost_w, a->dpost_b, a->dpre_w, a->dpre_b, a->dgate}, a->param_dtype, 0, {}};
-    for (int k = 0; k < SUM_GATE; ++k)
+    FinalSums f = {{a->dpost_w, a->dpost_b, a->dpre_w, a->dpre_b}, a->dgate, own ? nullptr : a->gate, a->post_w, a->post_b,
+                   a->param_dtype, 0, {}};
+    for (int k = 0; k < OUTS; ++k)
         if (f.out[k]) f.job[f.jobs++] = k;
-    const bool rowgate = a->gate && a->gate_groups == rows && rows > 1;
-    const int64_t jobs = f.jobs + (a->dgate && !rowgate && !p.whole ? a->gate_groups : 0);
-    if (jobs) {
-        hipLaunchKernelGGL(residual_norm_sums_kernel, dim3((unsigned)ceil_div(C, 64), (unsigned)jobs), dim3(1024), 0, st,
-                           f, p.nblocks, p.cpg, C, part);
+    const int64_t blocks = f.jobs * ceil_div(C, 64) +
+                           (a->dgate && !own ? a->gate_groups * ceil_div(C, p.cpg <= 16 ? 1024 : 64) : 0);
+    if (blocks) {
+        hipLaunchKernelGGL(residual_norm_sums_kernel, dim3((unsigned)blocks), dim3(1024), 0, st, f, p.nblocks, p.cpg, C,
+                           part);
         NBX_LAUNCH_CHECK("residual_norm_sums");
     }
     return NBX_OK;

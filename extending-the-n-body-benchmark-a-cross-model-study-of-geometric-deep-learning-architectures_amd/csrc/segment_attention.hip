@@ -71,6 +71,7 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 
 struct SaPlan {
     int T, RV, EL, slices;    // threads, vectors per row, edges side by side, blocks per row
+    int RB, spb;              // join: vectors of a row per block; list form: slices per block
     int eb, TP, grp, entries; // backward: positions per block, threads that work, lanes of a head that shuffle,
                               // what they leave per position
     int chunked;
@@ -176,6 +177,9 @@ __device__ __forceinline__ void join_groups(float (&acc)[VW], float* red, int RV
 }
 
 // ======================================================================== forward, list form
+// A block per node and `spb` slices of T vectors of its row.  A list of up to 64 edges has its weights formed
+// once for all slices, while the first slice's values are on their way; the next slice's are loaded before
+// this one's result is stored.
 template <typename T, int VW>
 __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment_attention_args a, SaPlan p, float keep) {
     extern __shared__ float lds[];
@@ -191,32 +195,22 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
     const DrawKey key = a.threshold ? draw_key(a.rng, a.call) : DrawKey{0, 0, 0, 0};
     const int64_t v = blockIdx.x;
     const int j0 = std::max(0, a.ptr[v]), j1 = (int)std::min<int64_t>(a.E, a.ptr[v + 1]);
-    const int el = p.slices > 1 ? 0 : t / p.RV;
-    const int f = p.slices > 1 ? (int)blockIdx.y * p.T + t : t - el * p.RV;
-    const bool on = el < p.EL && f < p.RV;
-    const int head = on ? (f * VW / a.D) % H : 0;
     const int64_t RL = (int64_t)p.RV * VW;
-    float acc[VW] = {};
-    if (t < H) {
-        sM[t] = -INFINITY;
-        sS[t] = 0.f;
-    }
-    for (int b = j0; b < j1; b += TILE) {
-        const int cnt = std::min(TILE, j1 - b);
+    const int el = p.slices > 1 ? 0 : t / p.RV;
+    const int s0 = blockIdx.y * p.spb, s1 = std::min(s0 + p.spb, p.slices);
+    auto column = [&](int s) { return p.slices > 1 ? s * p.T + t : t - el * p.RV; };
+    auto is_on = [&](int f) { return el < p.EL && f < p.RV; };
+    auto value = [&](int i, int f) { return (const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW; };
+    // the weights of positions [b, b + cnt) with the running maximum and sum; `meanwhile` runs once the edges
+    // are known
+    auto weigh = [&](int b, int cnt, auto&& meanwhile) {
         __syncthreads();
         for (int i = t; i < cnt; i += p.T) {
             const int e = a.eid[b + i];
             sE[i] = e >= 0 && e < a.E ? e : -1;
         }
         __syncthreads();
-        // the first values are on their way while the weights are formed
-        RawV<T, VW> first[AHEAD];
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            const int i = el + k * p.EL;
-            if (on && i < cnt && sE[i] >= 0)
-                first[k] = loadr<T, VW>((const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW);
-        }
+        meanwhile();
         for (int i = t; i < cnt * H; i += p.T) {
             const int e = sE[i / H];
             sW[i] = e < 0 ? -INFINITY : load_logit(a, (int64_t)e * H + i % H);
@@ -240,29 +234,73 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
             for (int i = 0; i < cnt; ++i) s += sP[i * H + t];
             sS[t] = s;
         }
-        if (on) {
-            const float r = sR[head];
+    };
+    auto finish = [&](float (&acc)[VW], int f, int head) {   // after a barrier that follows the sums
+        if (is_on(f) && el == 0) {
+            const float inv = keep / (sS[head] + 1e-16f);
 #pragma unroll
-            for (int k = 0; k < VW; ++k) acc[k] *= r;
+            for (int k = 0; k < VW; ++k) acc[k] = sS[head] == 0.f ? 0.f : acc[k] * inv;
+            storev<T, VW>((T*)a.out + v * RL + (int64_t)f * VW, acc);
+        }
+    };
+    auto head_of = [&](int f) { return is_on(f) ? (f * VW / a.D) % H : 0; };
+    if (j1 - j0 <= TILE) {
+        const int cnt = std::max(0, j1 - j0);
+        RawV<T, VW> x[AHEAD];
+        auto fetch = [&](int f) {
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const int i = el + k * p.EL;
+                if (is_on(f) && i < cnt && sE[i] >= 0) x[k] = loadr<T, VW>(value(i, f));
+            }
+        };
+        if (t < H) {
+            sM[t] = -INFINITY;
+            sS[t] = 0.f;
+        }
+        weigh(j0, cnt, [&] { fetch(column(s0)); });
+        __syncthreads();
+        for (int s = s0; s < s1; ++s) {
+            const int f = column(s), head = head_of(f);
+            float acc[VW] = {};
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const int i = el + j * p.EL;
-                const float w = i < cnt ? sW[i * H + head] : 0.f;
+                const float w = is_on(f) && i < cnt ? sW[i * H + head] : 0.f;
                 if (w != 0.f)
 #pragma unroll
-                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, lane_of<T, VW>(first[j], k), acc[k]);
+                    for (int k = 0; k < VW; ++k) acc[k] = fmaf(w, lane_of<T, VW>(x[j], k), acc[k]);
             }
-            weighted_rows<T, VW>(acc, el + AHEAD * p.EL, cnt, p.EL, [&](int i) { return sW[i * H + head]; },
-                                 [&](int i) { return (const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW; });
+            if (is_on(f) && cnt > AHEAD * p.EL)
+                weighted_rows<T, VW>(acc, el + AHEAD * p.EL, cnt, p.EL, [&](int i) { return sW[i * H + head]; },
+                                     [&](int i) { return value(i, f); });
+            if (s + 1 < s1) fetch(column(s + 1));
+            if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
+            finish(acc, f, head);
         }
-    }
-    if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
-    else __syncthreads();
-    if (on && el == 0) {
-        const float inv = keep / (sS[head] + 1e-16f);
+    } else {
+        for (int s = s0; s < s1; ++s) {
+            const int f = column(s), head = head_of(f);
+            float acc[VW] = {};
+            __syncthreads();
+            if (t < H) {
+                sM[t] = -INFINITY;
+                sS[t] = 0.f;
+            }
+            for (int b = j0; b < j1; b += TILE) {
+                const int cnt = std::min(TILE, j1 - b);
+                weigh(b, cnt, [] {});
+                const float r = sR[head];
 #pragma unroll
-        for (int k = 0; k < VW; ++k) acc[k] = sS[head] == 0.f ? 0.f : acc[k] * inv;
-        storev<T, VW>((T*)a.out + v * RL + (int64_t)f * VW, acc);
+                for (int k = 0; k < VW; ++k) acc[k] *= r;
+                if (is_on(f))
+                    weighted_rows<T, VW>(acc, el, cnt, p.EL, [&](int i) { return sW[i * H + head]; },
+                                         [&](int i) { return value(i, f); });
+            }
+            if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
+            else __syncthreads();
+            finish(acc, f, head);
+        }
     }
     if (a.stats && blockIdx.y == 0 && t < H) {
         a.stats[v * H + t] = finite_max(sM[t]);
@@ -391,8 +429,7 @@ __global__ __launch_bounds__(256) void segment_attention_join_kernel(nbx_segment
         sM[t] = finite_max(m);
         sS[t] = 0.f;
     }
-    const int el = p.slices > 1 ? 0 : t / p.RV;
-    const int f = p.slices > 1 ? (int)blockIdx.y * p.T + t : t - el * p.RV;
+    const int el = t / p.RB, f = (int)blockIdx.y * p.RB + t - el * p.RB;
     const bool on = el < p.EL && f < p.RV;
     const int head = on ? (f * VW / a.D) % H : 0;
     float acc[VW] = {};
@@ -415,8 +452,7 @@ __global__ __launch_bounds__(256) void segment_attention_join_kernel(nbx_segment
             weighted_rows<float, VW>(acc, el, cnt, p.EL, [&](int i) { return sR[i * H + head]; },
                                      [&](int i) { return pacc + slot(b + i) * RL + (int64_t)f * VW; });
     }
-    if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
-    else __syncthreads();
+    join_groups<VW>(acc, red, p.RB, p.EL);
     if (on && el == 0) {
         const float inv = keep / (sS[head] + 1e-16f);
 #pragma unroll
@@ -607,7 +643,7 @@ int sa_check(const nbx_segment_attention_args* a, const char* who) {
                   "%s: l_dtype must be fp32 or v_dtype", who);
     NBX_CHECK_ARG(a->H <= SA_MAXH && a->D <= 4096 && (int64_t)a->H * a->D <= (a->D % 4 == 0 ? 4096 : 1024),
                   "%s: need H <= %d, H D <= 4096 (1024 if D %% 4)", who, SA_MAXH);
-    NBX_CHECK_ARG(a->K <= (1 << 22) && a->K * a->H * a->D <= (1 << 22), "%s: rows of more than 2^22 values", who);
+    NBX_CHECK_ARG(a->K < (1 << 20) && a->K * a->H * a->D < (1 << 20), "%s: need K H D < 2^20", who);
     NBX_CHECK_ARG(a->V < (1 << 24), "%s: too many nodes", who);   // a launch's threads along x fit 32 bits
     NBX_CHECK_ARG(a->threshold < 65536 && (!a->threshold || a->rng), "%s: need threshold < 65536, and rng for a drop rate",
                   who);
@@ -622,6 +658,9 @@ SaPlan forward_plan(const nbx_segment_attention_args& a) {
     p.EL = p.RV <= p.T ? p.T / p.RV : 1;
     p.slices = p.RV <= p.T ? 1 : (int)ceil_div(p.RV, p.T);
     p.chunked = a.E >= 32 * a.V;
+    // about 1024 blocks or more: 640 nodes of 7 slices take 24.4 us at one slice per block, 20.3 at two, 18.1 at
+    // four, 19.2 at seven
+    p.spb = (int)ceil_div(p.slices, std::min<int64_t>(p.slices, std::max<int64_t>(1, ceil_div(1024, std::max<int64_t>(1, a.V)))));
     p.nc = ceil_div(a.E, TILE);
     return p;
 }
@@ -639,7 +678,7 @@ SaPlan backward_plan(const nbx_segment_attention_args& a) {
     // positions per block: enough blocks for the chip first, then few (each has its searches and sums), within
     // 48 KB of LDS
     p.eb = p.RV <= p.T ? TILE : 4;
-    while (p.eb > 4 && (a.E < 1024 * (int64_t)p.eb || p.eb * (p.entries + 3 * a.H) > 12288)) p.eb /= 2;
+    while (p.eb > 4 && (a.E < 768 * (int64_t)p.eb || p.eb * (p.entries + 3 * a.H) > 12288)) p.eb /= 2;
     p.eb = std::max(p.eb, std::min(p.EL, TILE));
     p.nc = ceil_div(a.E, p.eb);
     return p;
@@ -695,8 +734,8 @@ extern "C" int nbx_segment_attention(const nbx_segment_attention_args* a, void* 
         constexpr int VW = decltype(vw)::value;
         if (!p.chunked) {
             const size_t lds = (size_t)(2 * TILE * a->H + 3 * a->H + p.T * VW + TILE) * 4;
-            hipLaunchKernelGGL((segment_attention_list_kernel<T, VW>), dim3((unsigned)a->V, (unsigned)p.slices), dim3(p.T),
-                               lds, st, *a, p, keep);
+            hipLaunchKernelGGL((segment_attention_list_kernel<T, VW>), dim3((unsigned)a->V, (unsigned)ceil_div(p.slices, p.spb)),
+                               dim3(p.T), lds, st, *a, p, keep);
             NBX_LAUNCH_CHECK("segment_attention_list");
             return NBX_OK;
         }
@@ -708,9 +747,13 @@ extern "C" int nbx_segment_attention(const nbx_segment_attention_args* a, void* 
                                lds, st, *a, p, keep, pacc, pms);
             NBX_LAUNCH_CHECK("segment_attention_chunk");
         }
+        SaPlan j = p;   // sixteen vectors of a row per block, so that many parts are read side by side
+        j.RB = std::min(p.RV, 16);
+        j.EL = 256 / j.RB;
+        j.slices = (int)ceil_div(p.RV, j.RB);
         const size_t jlds = (size_t)(2 * TILE * a->H + p.T + a->H + p.T * VW) * 4;
-        hipLaunchKernelGGL((segment_attention_join_kernel<T, VW>), dim3((unsigned)a->V, (unsigned)p.slices), dim3(p.T),
-                           jlds, st, *a, p, keep, pacc, pms);
+        hipLaunchKernelGGL((segment_attention_join_kernel<T, VW>), dim3((unsigned)a->V, (unsigned)j.slices), dim3(p.T),
+                           jlds, st, *a, j, keep, pacc, pms);
         NBX_LAUNCH_CHECK("segment_attention_join");
         return NBX_OK;
     });

@@ -71,6 +71,49 @@ __device__ __forceinline__ void store8n(T* p, int n, const float (&v)[8]) {
         if (i < n) p[i] = (T)v[i];
 }
 
+// Eight elements as loaded: nothing waits for them before unpack8.
+template <typename T>
+struct Raw8 {
+    typename Vec8<T>::type v;
+};
+template <>
+struct Raw8<float> {
+    f32x4u a, b;
+};
+template <typename T>
+__device__ __forceinline__ void fetch8n(const T* p, int n, Raw8<T>& r) {
+    if (n == 8) {
+        r.v = *reinterpret_cast<const typename Vec8<T>::type*>(p);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = i < n ? p[i] : (T)0.f;
+}
+__device__ __forceinline__ void fetch8n(const float* p, int n, Raw8<float>& r) {
+    if (n == 8) {
+        r.a = *reinterpret_cast<const f32x4u*>(p);
+        r.b = *reinterpret_cast<const f32x4u*>(p + 4);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r.a[i] = i < n ? p[i] : 0.f;
+        r.b[i] = 4 + i < n ? p[4 + i] : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)r.v[i];
+}
+__device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = r.a[i];
+        v[4 + i] = r.b[i];
+    }
+}
+
 // Parameters: fp32, or the 16-bit type of the activations (code NBX_F32 / NBX_BF16 / NBX_F16, uniform).
 __device__ __forceinline__ void load8p(const void* p, int dtype, int64_t at, int n, float (&v)[8]) {
     if (dtype == 0) load8n((const float*)p + at, n, v);
