@@ -6,12 +6,14 @@ raises if it is missing or if a tensor is not on a HIP device.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("NBX_LIB") or os.path.join(_HERE, "lib", "libnbx.so")  # NBX_LIB: A/B builds only
+TORCH_LIB_PATH = os.path.join(_HERE, "lib", "nbx_torch.so")
 ABI_VERSION = 20
 COMM_ID_BYTES = 128
 ROLLOUT_ABSOLUTE = 1   # NBX_ROLLOUT_ABSOLUTE
@@ -295,6 +297,30 @@ def lib():
             raise NbxError("libnbx ABI version mismatch")
         _lib = handle
     return _lib
+
+
+_torch_ops = None
+
+
+def torch_ops():
+    """The autograd operators of csrc/block_ops_torch.cpp (lib/nbx_torch.so), bound to the loaded library."""
+    global _torch_ops
+    if _torch_ops is None:
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise NbxError(f"extension not built: {TORCH_LIB_PATH} is missing (run __graft_entry__.build())")
+        spec = importlib.util.spec_from_file_location("nbx_torch", TORCH_LIB_PATH)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        if m.abi_version != ABI_VERSION:
+            raise NbxError("nbx_torch ABI version mismatch")
+        handle = lib()
+        m.bind({n: ctypes.cast(getattr(handle, n), c_p).value for n in (
+            "nbx_last_error", "nbx_dropout", "nbx_residual_norm", "nbx_residual_norm_backward_workspace_bytes",
+            "nbx_residual_norm_backward", "nbx_sh_residual_norm", "nbx_sh_residual_norm_backward_workspace_bytes",
+            "nbx_sh_residual_norm_backward", "nbx_segment_attention_workspace_bytes", "nbx_segment_attention",
+            "nbx_segment_attention_backward")}, NbxError)
+        _torch_ops = m
+    return _torch_ops
 
 
 def check(rc: int, what: str):

@@ -1,5 +1,5 @@
 """Operators around a training block's products (include/nbx.h "Block operators", csrc/block_ops.hip and
-csrc/segment_attention.hip), each an autograd operator on the caller's stream:
+csrc/segment_attention.hip), each an autograd operator (csrc/block_ops_torch.cpp) on the caller's stream:
 
 * :func:`dropout` — dropout of elements, of whole groups of rows (stochastic depth) or of channels, whose
   mask is never stored: forward and backward draw it from a counter;
@@ -22,13 +22,10 @@ Like the framework's other operators these run on the HIP device only.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 
-_f32 = torch.float32
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _PER = {"element": _lib.DROP_ELEMENT, "group": _lib.DROP_GROUP, "channel": _lib.DROP_CHANNEL}
 _NORM = {"layer": 0, "rms": 1}
@@ -112,84 +109,7 @@ def _dtype(t, what):
     return code
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else _lib.stream_ptr
-_current = torch.cuda.current_device
-_entries = {}
-
-
-def _launch(name, dev, *args):
-    """Calls an entry point on the device's current stream, with that device current."""
-    f = _entries.get(name)
-    if f is None:
-        f = _entries[name] = getattr(_lib.lib(), name)
-    i = dev.index
-    if _current() == i:
-        rc = f(*args, _stream(i))
-    else:
-        with torch.cuda.device(i):
-            rc = f(*args, _stream(i))
-    if rc:
-        _lib.check(rc, name)
-
-
-_sizes = {}
-
-
-def _workspace(name, key, args, dev, *more):
-    """The workspace that a call with these arguments asks for (its size kept per ``key``)."""
-    n = _sizes.get((name, key))
-    if n is None:
-        size = _lib.c_sz()
-        _lib.check(getattr(_lib.lib(), name)(ctypes.byref(args), *more, ctypes.byref(size)), name)
-        if len(_sizes) >= 4096:
-            _sizes.clear()
-        n = _sizes[(name, key)] = size.value
-    if n == 0:
-        return None
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), n
-    return ws
-
-
-def _first_derivatives_only():
-    if torch.is_grad_enabled():
-        raise _lib.NbxError("block operators have no second derivatives (a backward pass with create_graph)")
-
-
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _dense(g):
-    return None if g is None else g.contiguous()
-
-
 # ---------------------------------------------------------------------------------------------- dropout
-def _dropout(x, how, state, used):
-    y = torch.empty_like(x)
-    _launch("nbx_dropout", x.device, *how[:-1], state.data_ptr(), how[-1], _ptr(used), x.data_ptr(), y.data_ptr())
-    return y
-
-
-class _DropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, how, state):
-        used = torch.empty_like(state)
-        y = _dropout(x, how, state, used)
-        ctx.save_for_backward(used)
-        ctx.how = how
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        _first_derivatives_only()
-        return _dropout(dy.contiguous(), ctx.how, ctx.saved_tensors[0], None), None, None
-
-
 def dropout(x, p, rng=None, *, call=None, per="element", group=1):
     """``x`` with a share ``p`` of it set to 0 and the rest scaled by 1 / (1 - p).
 
@@ -208,81 +128,12 @@ def dropout(x, p, rng=None, *, call=None, per="element", group=1):
     if threshold == 0:
         return x
     state, call = _draws(rng, call, 1, dev)
-    x = x.contiguous()
     n = x.shape[0] if x.dim() and per != "element" else 1
     C = x.shape[-1] if per == "channel" else 1
-    how = (code, _PER[per], n, x.numel() // max(n * C, 1), C, int(group), threshold, call)
-    if x.requires_grad and torch.is_grad_enabled():
-        return _DropoutFn.apply(x, how, state)
-    return _dropout(x, how, state, None)
+    return _lib.torch_ops().dropout(x, state, code, _PER[per], n, x.numel() // max(n * C, 1), C, int(group), threshold, call)
 
 
 # ---------------------------------------------------------------------------------------------- residual + norms
-def _rows(t, C):
-    """(tensor, elements between its rows): strided rows are read in place, anything else is copied."""
-    if t.dim() == 2 and t.shape[0] > 1 and t.stride(1) == 1 and t.stride(0) >= C:
-        return t, t.stride(0)
-    return t.contiguous(), C
-
-
-def _residual_args(how, x, y, gate, post_w, post_b, pre_w, pre_b):
-    rows, C, ldx, ldy, codes, norm, eps, scale, threshold, group, call = how
-    a = _lib.ResidualNormArgs(rows, C, ldx, ldy, gate.numel() // C if gate is not None else 0, group, *codes, norm, eps,
-                              scale, threshold, call)
-    a.x, a.y, a.gate = _ptr(x), _ptr(y), _ptr(gate)
-    a.post_w, a.post_b, a.pre_w, a.pre_b = _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(pre_b)
-    return a
-
-
-def _residual_forward(how, x, y, gate, post_w, post_b, pre_w, pre_b, state, used, stats):
-    dev = x.device
-    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    z = torch.empty(y.shape, dtype=y.dtype, device=dev) if pre_w is not None else None
-    a = _residual_args(how, x, y, gate, post_w, post_b, pre_w, pre_b)
-    a.rng, a.used, a.h, a.z, a.stats = _ptr(state), _ptr(used), h.data_ptr(), _ptr(z), _ptr(stats)
-    _launch("nbx_residual_norm", dev, ctypes.byref(a))
-    return h, z
-
-
-class _ResidualNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, how, state, x, y, gate, post_w, post_b, pre_w, pre_b):
-        dev, rows = x.device, how[0]
-        used = torch.empty(2, dtype=torch.int64, device=dev) if state is not None else None
-        norms = post_w is not None or pre_w is not None
-        stats = torch.empty(4, rows, dtype=_f32, device=dev) if norms else None
-        h, z = _residual_forward(how, x, y, gate, post_w, post_b, pre_w, pre_b, state, used, stats)
-        # y is read again for its norm and the gate's gradient only, h for the norm behind it
-        keep_y = y if post_w is not None or (gate is not None and ctx.needs_input_grad[4]) else None
-        ctx.save_for_backward(keep_y, h if pre_w is not None else None, gate, post_w, post_b, pre_w, pre_b, used, stats)
-        ctx.how = how
-        ctx.shapes = (x.shape, x.dtype, y.shape, y.dtype)
-        ctx.set_materialize_grads(False)
-        return (h, z) if z is not None else h
-
-    @staticmethod
-    def backward(ctx, dh, dz=None):
-        _first_derivatives_only()
-        if dh is None and dz is None:
-            return (None,) * 9
-        y, h, gate, post_w, post_b, pre_w, pre_b, used, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        xs, xt, ys, yt = ctx.shapes
-        dh, dz = _dense(dh), _dense(dz)
-        dev = (dh if dh is not None else dz).device
-        a = _residual_args(ctx.how, None, y, gate, post_w, post_b, pre_w, pre_b)
-        grads = [torch.empty(xs, dtype=xt, device=dev) if need[2] else None,
-                 torch.empty(ys, dtype=yt, device=dev) if need[3] else None]
-        # without dz nothing reaches the norm behind the sum: its parameters' gradients are 0
-        grads += [torch.empty_like(t) if need[4 + i] and t is not None else None
-                  for i, t in enumerate((gate, post_w, post_b, pre_w, pre_b))]
-        a.rng, a.h, a.stats, a.dh, a.dz = _ptr(used), _ptr(h), _ptr(stats), _ptr(dh), _ptr(dz)
-        a.dx, a.dy, a.dgate, a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = (_ptr(g) for g in grads)
-        ws = _workspace("nbx_residual_norm_backward_workspace_bytes", (ctx.how[:2], a.gate_groups), a, dev)   # noqa: F841
-        _launch("nbx_residual_norm_backward", dev, ctypes.byref(a))
-        return (None, None, *grads)
-
-
 def residual_norm(x, y, *, gate=None, scale=1.0, post=None, pre=None, norm="rms", eps=1e-5, p=0.0, group=0, rng=None,
                   call=None):
     """The residual stream after a block: ``h = x + scale * dropout(gate * u)`` with ``u = y`` or, with ``post``
@@ -327,64 +178,12 @@ def residual_norm(x, y, *, gate=None, scale=1.0, post=None, pre=None, norm="rms"
     if threshold:
         state, call = _draws(rng, call, 1, dev)
     if rows == 0:
-        return x.clone(), (y.clone() if pre_w is not None else None)
-    x, ldx = _rows(x, C)
-    y, ldy = _rows(y, C)
-    params = [None if t is None else t.contiguous() for t in (gate, post_w, post_b, pre_w, pre_b)]
-    how = (rows, C, ldx, ldy, (cx, cy, cp), _NORM[norm], float(eps), float(scale), threshold, int(group), call or 0)
-    if _wants_grad(x, y, *params):
-        out = _ResidualNormFn.apply(how, state, x, y, *params)
-        return out if pre_w is not None else (out, None)
-    return _residual_forward(how, x, y, *params, state, None, None)
+        return x + y, (y * pre_w.to(y.dtype) if pre_w is not None else None)
+    return _lib.torch_ops().residual_norm(x, y, gate, post_w, post_b, pre_w, pre_b, state, cx, cy, cp, _NORM[norm], eps,
+                                          scale, threshold, int(group), call or 0)
 
 
 # ---------------------------------------------------------------------------------------------- spherical harmonics
-def _sh_args(how, weight, bias):
-    V, path_group, lmax, C, code, cp, eps, t1, t2, call = how
-    a = _lib.ShResidualNormArgs(V, path_group, lmax, C, code, cp, eps, t1, t2, call)
-    a.weight, a.bias = _ptr(weight), _ptr(bias)
-    return a
-
-
-def _sh_forward(how, x, y, weight, bias, state, used, stats):
-    dev = x.device
-    h, z = torch.empty_like(x), torch.empty_like(x)
-    a = _sh_args(how, weight, bias)
-    a.rng, a.used, a.x, a.y, a.h, a.z, a.stats = (_ptr(state), _ptr(used), x.data_ptr(), y.data_ptr(), h.data_ptr(),
-                                                  z.data_ptr(), _ptr(stats))
-    _launch("nbx_sh_residual_norm", dev, ctypes.byref(a))
-    return h, z
-
-
-class _ShResidualNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, how, state, x, y, weight, bias):
-        dev = x.device
-        used = torch.empty(2, dtype=torch.int64, device=dev) if state is not None else None
-        stats = torch.empty(2, x.shape[0], dtype=_f32, device=dev)
-        h, z = _sh_forward(how, x, y, weight, bias, state, used, stats)
-        ctx.save_for_backward(h, weight, bias, used, stats)
-        ctx.how = how
-        ctx.set_materialize_grads(False)
-        return h, z
-
-    @staticmethod
-    def backward(ctx, dh, dz):
-        _first_derivatives_only()
-        if dh is None and dz is None:
-            return (None,) * 6
-        h, weight, bias, used, stats = ctx.saved_tensors
-        dev, need = h.device, ctx.needs_input_grad
-        dh, dz = _dense(dh), _dense(dz)
-        a = _sh_args(ctx.how, weight, bias)
-        grads = [torch.empty_like(t) if n else None for t, n in zip((h, h, weight, bias), need[2:])]
-        a.rng, a.h, a.stats, a.dh, a.dz = _ptr(used), h.data_ptr(), stats.data_ptr(), _ptr(dh), _ptr(dz)
-        a.dx, a.dy, a.dweight, a.dbias = (_ptr(g) for g in grads)
-        ws = _workspace("nbx_sh_residual_norm_backward_workspace_bytes", ctx.how[:4], a, dev)   # noqa: F841
-        _launch("nbx_sh_residual_norm_backward", dev, ctypes.byref(a))
-        return (None, None, *grads)
-
-
 def sh_residual_norm(x, y, weight, bias, *, eps=1e-5, path_p=0.0, path_group=1, channel_p=0.0, rng=None, call=None):
     """The residual add of an EquiformerV2 block with the norm behind it: ``h = x + dropout(y)`` and z, the
     equivariant RMS norm of h (degree-balanced mean square over coefficients and channels, the l = 0 row
@@ -413,59 +212,12 @@ def sh_residual_norm(x, y, weight, bias, *, eps=1e-5, path_p=0.0, path_group=1, 
     if t1 or t2:
         state, call = _draws(rng, call, 2, dev)
     if V == 0:
-        return x.clone(), y.clone()
-    x, y, weight, bias = x.contiguous(), y.contiguous(), weight.contiguous(), bias.contiguous()
-    how = (V, int(path_group), lmax, C, code, cp, float(eps), t1, t2, call or 0)
-    if _wants_grad(x, y, weight, bias):
-        return _ShResidualNormFn.apply(how, state, x, y, weight, bias)
-    return _sh_forward(how, x, y, weight, bias, state, None, None)
+        return x + y, y * bias.to(y.dtype)
+    return _lib.torch_ops().sh_residual_norm(x, y, weight, bias, state, lmax, code, cp, eps, t1, int(path_group), t2,
+                                             call or 0)
 
 
 # ---------------------------------------------------------------------------------------------- segment attention
-def _attention_args(how, ptr, eid, values, logits):
-    V, E, K, H, D, cv, cl, threshold, call = how
-    a = _lib.SegmentAttentionArgs(V, E, K, H, D, cv, cl, threshold, call)
-    a.ptr, a.eid, a.values, a.logits = _ptr(ptr), _ptr(eid), _ptr(values), _ptr(logits)
-    return a
-
-
-def _attention_forward(how, values, logits, ptr, eid, state, used, stats):
-    dev = values.device
-    V, _, K, H, D = how[:5]
-    out = torch.empty(V, K, H, D, dtype=values.dtype, device=dev)
-    a = _attention_args(how, ptr, eid, values, logits)
-    a.rng, a.used, a.out, a.stats = _ptr(state), _ptr(used), out.data_ptr(), _ptr(stats)
-    ws = _workspace("nbx_segment_attention_workspace_bytes", (how[:7], 0), a, dev, 0)   # noqa: F841
-    _launch("nbx_segment_attention", dev, ctypes.byref(a))
-    return out
-
-
-class _SegmentAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, how, state, values, logits, ptr, eid):
-        dev = values.device
-        used = torch.empty(2, dtype=torch.int64, device=dev) if state is not None else None
-        stats = torch.empty(2, how[0], how[3], dtype=_f32, device=dev)
-        out = _attention_forward(how, values, logits, ptr, eid, state, used, stats)
-        ctx.save_for_backward(values, logits, ptr, eid, used, stats)
-        ctx.how = how
-        return out
-
-    @staticmethod
-    def backward(ctx, dout):
-        _first_derivatives_only()
-        values, logits, ptr, eid, used, stats = ctx.saved_tensors
-        dev = values.device
-        dout = dout.contiguous()
-        a = _attention_args(ctx.how, ptr, eid, values, logits)
-        dv = torch.empty_like(values) if ctx.needs_input_grad[2] else None
-        dl = torch.empty_like(logits) if ctx.needs_input_grad[3] else None
-        a.rng, a.stats, a.dout, a.dvalues, a.dlogits = _ptr(used), stats.data_ptr(), dout.data_ptr(), _ptr(dv), _ptr(dl)
-        ws = _workspace("nbx_segment_attention_workspace_bytes", (ctx.how[:7], 1, dl is None), a, dev, 1)   # noqa: F841
-        _launch("nbx_segment_attention_backward", dev, ctypes.byref(a))
-        return None, None, dv, dl, None, None
-
-
 def segment_attention(values, logits, ptr, eid, *, p=0.0, rng=None, call=None):
     """Attention over the edges into each node: ``out[v] = sum over v's edges of dropout(a[e, h]) values[e, :, h]``
     with a the softmax of the edges' ``logits`` over v's list.  Returns [V, K, H, D].
@@ -489,8 +241,4 @@ def segment_attention(values, logits, ptr, eid, *, p=0.0, rng=None, call=None):
     state = None
     if threshold:
         state, call = _draws(rng, call, 1, dev)
-    how = (ptr.numel() - 1, E, K, H, D, cv, cl, threshold, call or 0)
-    values, logits, ptr, eid = values.contiguous(), logits.contiguous(), ptr.contiguous(), eid.contiguous()
-    if _wants_grad(values, logits):
-        return _SegmentAttentionFn.apply(how, state, values, logits, ptr, eid)
-    return _attention_forward(how, values, logits, ptr, eid, state, None, None)
+    return _lib.torch_ops().segment_attention(values, logits, ptr, eid, state, cv, cl, threshold, call or 0)

@@ -1,4 +1,5 @@
-"""Build libnbx.so for gfx950 with hipcc (in-tree: <package>/lib/libnbx.so).
+"""Build libnbx.so for gfx950 with hipcc (in-tree: <package>/lib/libnbx.so), and the torch operators over it
+(csrc/block_ops_torch.cpp -> lib/nbx_torch.so) with the host compiler.
 
     python <package>/build.py [--jobs 8] [--verbose]
 """
@@ -50,6 +51,24 @@ def _needs(obj: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+TORCH_SRC = os.path.join(CSRC, "block_ops_torch.cpp")
+TORCH_LIB = os.path.join(OUT_DIR, "nbx_torch.so")
+
+
+def _torch_command():
+    """The host compiler's command for lib/nbx_torch.so (HIP's headers for the stream type only)."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            *(a for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                          "/opt/rocm/include", sysconfig.get_paths()["include"]) for a in ("-isystem", d)),
+            TORCH_SRC, "-o", TORCH_LIB, f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_hip", "-ltorch_cpu",
+            "-ltorch_python", "-ltorch"]
+
+
 def build(jobs: int = 8, verbose: bool = False, force: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
     hipcc = _hipcc()
@@ -62,12 +81,15 @@ def build(jobs: int = 8, verbose: bool = False, force: bool = False) -> str:
         if force or _needs(o, [s] + headers):
             cmds.append([hipcc, *FLAGS, *FILE_FLAGS.get(os.path.basename(s), []), "-c", s, "-o", o])
 
+    if not _TAG and (force or _needs(TORCH_LIB, [TORCH_SRC, os.path.join(HERE, "..", "include", "nbx.h")])):
+        cmds.append(_torch_command())
+
     def run(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f"hipcc failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         return r.stderr
 
     with cf.ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
@@ -75,7 +97,7 @@ def build(jobs: int = 8, verbose: bool = False, force: bool = False) -> str:
             if verbose and err:
                 print(err, file=sys.stderr)
     _keep_device_asm()
-    if cmds or not os.path.exists(LIB) or _needs(LIB, objs):
+    if any(c[0] == hipcc for c in cmds) or not os.path.exists(LIB) or _needs(LIB, objs):
         # librccl.so.1: csrc/comm.hip (under PyTorch the loader reuses torch's copy, same soname)
         run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", LIB, *objs, "-L/opt/rocm/lib", "-lrccl"])
     check_isa()
