@@ -683,6 +683,8 @@ def train_loop(a, world, device, P, model, forward, target, model_size):
         P.allreduce_gradients(params)
         torch.nn.utils.clip_grad_norm_(params, 1.0, foreach=True)
         opt.step()
+        if getattr(model, "block_rng", None) is not None:
+            model.block_rng.advance()        # on the device: every replay draws anew
         return loss
 
     # roofline: every GEMM launch of one eager step, event-timed on the launch stream
@@ -821,6 +823,7 @@ def bench_ponita_train(a, rank, world, device, P):
     B, N = a.batch or 64, NBODY
     torch.manual_seed(0)
     model = PO.PONITA_NBODY(**PONITA_TRAIN).to(device).train()
+    model.fused_residual = a.block_ops
     model.model.materialize()
     loc, vel, mass = initial_states(B, N, rank * B)
     rng = np.random.default_rng(200 + rank)
@@ -991,6 +994,9 @@ def bench_eqv2_train(a, rank, world, device, P):
     B, N = a.batch or 64, NBODY
     torch.manual_seed(0)
     model = EquiformerV2_nbody(**EQV2_C4).to(device).train()
+    if a.block_ops:
+        from nbody_amd.block_ops import CounterRNG
+        model.block_rng = CounterRNG(rank, device)
     loc, vel, mass = initial_states(B, N, rank * B)
     rng = np.random.default_rng(300 + rank)
     t = lambda x: torch.tensor(x, dtype=torch.float32, device=device)
@@ -1202,6 +1208,9 @@ def main():
                     help="C2: self-feed steps of the torch CPU restatement timed for cpu_baseline")
     ap.add_argument("--eager", action="store_true",
                     help="egnn_mc_train / segnn_train: run the step eagerly (no HIP graph)")
+    ap.add_argument("--block-ops", action="store_true",
+                    help="eqv2_train / ponita_train: the blocks' residual adds, norms, dropouts and attention as "
+                         "block operators (nbody_amd.block_ops) instead of torch glue")
     ap.add_argument("--deterministic-bn", action="store_true",
                     help="segnn: fixed-order BatchNorm sums (bit-reproducible) instead of fp64 atomics")
     ap.add_argument("--bn-mode", default="batch", choices=["batch", "sync", "running"],

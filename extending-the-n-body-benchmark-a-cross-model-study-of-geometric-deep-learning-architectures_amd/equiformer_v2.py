@@ -226,6 +226,10 @@ class EquiformerV2_nbody(nn.Module):
     EquiformerV2 section), the composed one (eqv2_train.py) every single-resolution lmax <= 6
     including the constructor default lmax 6 / mmax 2."""
 
+    # a block_ops.CounterRNG: the training composition's residual adds, norms, dropouts and attention run as
+    # block operators with counter-based draws (eqv2_train.py); None: torch's RNG, as the reference
+    block_rng = None
+
     def __init__(self, device=None, use_pbc=False, regress_forces=True, otf_graph=True, max_neighbors=5,
                  max_radius=4096, max_num_elements=90, num_layers=12, attn_hidden_channels=128, sphere_channels=128,
                  num_heads=8, attn_alpha_channels=32, attn_value_channels=16, ffn_hidden_channels=512,

@@ -19,6 +19,12 @@ reference's forward uses:
 * gathers x[edge_index[0 / 1]], embedding lookups and the aggregation = ``segnn_train._GatherFn`` /
   ``_SegSumFn`` over CSR tables (no atomics).
 
+With ``model.block_rng`` set to a ``block_ops.CounterRNG`` the residual adds (with drop path, projection
+dropout and the norm behind them) and the attention (softmax, alpha dropout, weighted sum over the edges) run
+as block operators (block_ops.py): the dropouts draw from the counter, no mask is stored, and a captured step
+draws anew when it ends with ``model.block_rng.advance()``.  None (the default): the operators above with
+torch's RNG, as the reference.
+
 Edge frames come from ``nbx_eqv2_train_edges`` / ``nbx_eqv2_edges`` (the inference path's frames and
 gauge draws).  Without autograd the same composition is the inference forward of the configurations
 the fused kernels do not cover (EquiformerV2_nbody.forward / rollout).
@@ -32,6 +38,7 @@ import torch
 
 from . import _lib, so3
 from .ponita_train import _LayerNormFn, linear
+from .block_ops import segment_attention, sh_residual_norm
 from .segnn_train import Graph, _GatherFn, _SegSumFn, _at, _dp, _st, colsum, gemm_grouped
 
 _f32 = torch.float32
@@ -649,6 +656,14 @@ class _Step:
         mask = torch.nn.functional.dropout(x.new_ones(x.shape[0], 1, x.shape[2]), p, True)
         return x * mask
 
+    def residual(self, x, y, norm):
+        """x + proj_drop(drop_path(y)) and its rms norm in one pass (block_ops.sh_residual_norm)."""
+        m = self.m
+        on = self.training
+        return sh_residual_norm(x, y, _f(norm.affine_weight), _f(norm.affine_bias), eps=norm.eps,
+                                path_p=m.drop_path_rate if on else 0.0, path_group=self.N,
+                                channel_p=m.proj_drop if on else 0.0, rng=m.block_rng)
+
     # ---------------------------------------------------------------- layers
     def attention(self, A, x, cout):
         """SO2EquivariantGraphAttention (transformer_block.py:226-370) of x [V][9][C] -> [V][9][cout]."""
@@ -671,10 +686,16 @@ class _Step:
                                A.alpha_norm.eps)
         a = act(a, _lib.ACT_SLRELU).view(E, nh, na)
         logit = (a * _f(A.alpha_dot)).sum(-1)
+        nr, nf = self.lay.n_red, self.lay.n_full
+        if m.block_rng is not None:
+            # the weights are per (edge, head) and the rotation back acts on coefficients alone, so they may
+            # follow it: softmax, dropout and the weighted sum over a node's edges in one pass
+            rot = self.rotate_inv(msg).view(E, nf, nh, nv)
+            agg = segment_attention(rot, logit, g.dptr, g.deid, p=A.alpha_drop if self.training else 0.0, rng=m.block_rng)
+            return self.so3_linear(A.proj, agg.view(V, nf, nh * nv))
         alpha = _SoftmaxFn.apply(logit, g)
         if self.training and A.alpha_drop > 0.0:   # the module's own rate: the force block's is 0
             alpha = torch.nn.functional.dropout(alpha, A.alpha_drop, True)    # (equiformer_v2_nbody.py:362)
-        nr, nf = self.lay.n_red, self.lay.n_full
         msg = (msg.view(E, nr, nh, nv) * alpha[:, None, :, None]).reshape(E, nr, nh * nv)
         rot = self.rotate_inv(msg)
         agg = _SegSumFn.apply(rot.reshape(E, nf * nh * nv), g.dst, g.dptr, g.deid, V).view(V, nf, nh * nv)
@@ -716,6 +737,13 @@ def train_forward(model, pos, vel, charges, B, N, gauge=None, seed=0, frame=0):
     x0 = gather(_f(m.sphere_embedding.weight), st.gn, "s")                               # [V][C]
     xv = linear(vel, m.velocity_embedding.weight, m.velocity_embedding.bias).view(V, 3, C)
     x = torch.cat([x0[:, None], xv, x0.new_zeros(V, st.lay.n_full - 4, C)], 1) + st.edge_degree()
+    if m.block_rng is not None:
+        z = st.rms_norm(m.blocks[0].norm_1 if len(m.blocks) else m.norm, x)
+        for blk, after in zip(m.blocks, [b.norm_1 for b in m.blocks[1:]] + [m.norm]):
+            y, z = st.residual(x, st.attention(blk.ga, z, C), blk.norm_2)
+            x, z = st.residual(y, st.ffn(blk.ffn, z), after)
+        pred = st.attention(m.force_block, z, 2)
+        return pred[:, 1:4, :2].transpose(1, 2).reshape(V, 6)
     for blk in m.blocks:
         y = st.proj_drop(st.drop_path(st.attention(blk.ga, st.rms_norm(blk.norm_1, x), C))) + x
         x = st.proj_drop(st.drop_path(st.ffn(blk.ffn, st.rms_norm(blk.norm_2, y)))) + y

@@ -164,6 +164,9 @@ class PonitaFiberBundle(nn.Module):
 class PONITA_NBODY(nn.Module):
     """ponita_nbody.py:9-116.  ``forward(graph) -> [B*N, 6]`` (pos_dt | vel)."""
 
+    # True: the training composition's layer scale + residual add as one operator (block_ops.residual_norm)
+    fused_residual = False
+
     def __init__(self, lr=1e-3, weight_decay=1e-5, warmup=10, layer_scale=1e-6, train_augm=False, hidden_dim=64,
                  layers=4, radius=None, num_ori=20, basis_dim=128, degree=3, widening_factor=4,
                  multiple_readouts=True, in_channels_scalar=1, in_channels_vec=1, out_channels_scalar=0,

@@ -13,7 +13,9 @@ tree:
 * FiberBundleConv (nn/conv.py:103-133): the spatial message over the destination CSR (``_MessageFn``;
   backward over the source CSR, no atomics) and the depth-wise fibre convolution + bias
   (``_FiberFn``);
-* LayerNorm (``_LayerNormFn``).
+* LayerNorm (``_LayerNormFn``);
+* with ``module.fused_residual`` (default False: two torch launches) the layer scale and the residual add in
+  one pass (``block_ops.residual_norm``), in the backward too.
 
 Invariants / polynomial features / the lifted input are data (no gradient), computed once per step
 by ``nbx_ponita_train_featurize``; the two basis MLPs run once per step and their outputs are shared
@@ -28,6 +30,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .block_ops import residual_norm
 from .segnn_train import Graph, colsum, gemm, gemm_batched, gemm_grouped, _at, _dp, _st, _ws
 
 _f32 = torch.float32
@@ -227,9 +230,12 @@ def train_forward(module, pos, vel, mass, edge_index):
                                layer.norm.eps)
         y = linear(y, layer.linear_1.weight, layer.linear_1.bias, GELU)
         y = linear(y, layer.linear_2.weight, layer.linear_2.bias)
-        if layer.layer_scale is not None:
-            y = layer.layer_scale.to(_f32) * y
-        h = y + h
+        if module.fused_residual:
+            h, _ = residual_norm(h, y, gate=None if layer.layer_scale is None else layer.layer_scale.to(_f32))
+        else:
+            if layer.layer_scale is not None:
+                y = layer.layer_scale.to(_f32) * y
+            h = y + h
         if ro is not None:
             readouts.append(linear(h, ro.weight, ro.bias))
     readout = sum(readouts) / len(readouts)
