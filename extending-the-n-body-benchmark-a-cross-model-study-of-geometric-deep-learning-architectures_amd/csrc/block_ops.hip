@@ -58,23 +58,30 @@ __global__ __launch_bounds__(256) void dropout_flat_kernel(int64_t total, uint32
 }
 
 // Row form (entries of S C elements sharing draws): a block takes 256 chunks of eight elements, of one
-// entry or of several.  CHANNEL keeps the entry's mask as bits in LDS, one Philox block for eight channels,
-// shared by the S rows.
+// entry or of several.  CHANNEL keeps the mask of the block's channels as bits in LDS, one Philox block for
+// eight channels, shared by the S rows: all of a short row's, or the window of 2048 channels (wrapping at C)
+// that a part of a long row touches.
+constexpr int CHANNEL_WINDOW = 2048 / 8 + 2;
+
 template <typename T, bool CHANNEL>
 __global__ __launch_bounds__(256) void dropout_rows_kernel(int64_t n, int64_t RS, int64_t C, int64_t group, int cpr,
                                                            int rpb, int64_t segs, uint32_t threshold, float scale,
                                                            const int64_t* __restrict__ rng, uint32_t call,
                                                            int64_t* __restrict__ used, const T* __restrict__ X,
                                                            T* __restrict__ Y) {
-    extern __shared__ uint8_t mask[];
+    __shared__ uint8_t mask[CHANNEL ? CHANNEL_WINDOW : 1];
     note_used(used, rng);
     const DrawKey key = draw_key(rng, call);
     const int64_t row0 = blockIdx.x / segs * rpb, seg = blockIdx.x % segs;
     const int64_t Cq = (C + 7) >> 3;
+    const int64_t first = rpb > 1 ? 0 : seg * 2048 % C >> 3;             // the window's first byte
+    const int per = (int)(Cq < CHANNEL_WINDOW ? Cq : CHANNEL_WINDOW);   // bytes per entry
     if (CHANNEL) {
-        const int64_t rows = std::min<int64_t>(rpb, n - row0);
-        for (int64_t k = threadIdx.x; k < rows * Cq; k += 256)
-            mask[k] = (uint8_t)keep_bits(key, (uint64_t)(row0 * Cq + k), threshold);
+        const int rows = (int)std::min<int64_t>(rpb, n - row0);
+        for (int k = threadIdx.x; k < rows * per; k += 256) {
+            const int64_t q = first + k % per;
+            mask[k] = (uint8_t)keep_bits(key, (uint64_t)((row0 + k / per) * Cq + (q < Cq ? q : q - Cq)), threshold);
+        }
         __syncthreads();
     }
     const int lr = rpb > 1 ? (int)threadIdx.x / cpr : 0;
@@ -85,11 +92,12 @@ __global__ __launch_bounds__(256) void dropout_rows_kernel(int64_t n, int64_t RS
     float v[8];
     load8n(X + at, cnt, v);
     if (CHANNEL) {
-        const uint8_t* mk = mask + lr * Cq;
+        const uint8_t* mk = mask + lr * per;
         int64_t c = f0 % C;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            v[i] = (mk[c >> 3] >> (c & 7) & 1) ? v[i] * scale : 0.f;
+            const int64_t q = (c >> 3) - first;
+            v[i] = (mk[q < 0 ? q + Cq : q] >> (c & 7) & 1) ? v[i] * scale : 0.f;
             c = c + 1 == C ? 0 : c + 1;
         }
     } else {
@@ -905,15 +913,13 @@ extern "C" int nbx_dropout(int32_t dtype, int32_t per, int64_t n, int64_t S, int
                                rng, call, used, (const T*)X, (T*)Y);
         } else {
             const bool channel = per == NBX_DROP_CHANNEL;
-            const int64_t chunks = ceil_div(RS, 8), Cq = ceil_div(C, 8);
-            NBX_CHECK_ARG(!channel || Cq <= 65536, "nbx_dropout: need C <= 2^19 for one draw per channel");
+            const int64_t chunks = ceil_div(RS, 8);
             int rpb = chunks <= 128 ? (int)(256 / chunks) : 1;
             const int64_t segs = rpb > 1 ? 1 : ceil_div(chunks, 256), blocks = ceil_div(n, rpb) * segs;
             NBX_CHECK_ARG(grid_ok(blocks, 256), "nbx_dropout: too many elements");
             const int cpr = rpb > 1 ? (int)chunks : 256;
             if (channel)
-                hipLaunchKernelGGL((dropout_rows_kernel<T, true>), dim3((unsigned)blocks), dim3(256),
-                                   (size_t)(rpb * Cq), st, n, RS, C, group, cpr, rpb, segs, threshold, scale, rng, call,
+                hipLaunchKernelGGL((dropout_rows_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, n, RS, C, group, cpr, rpb, segs, threshold, scale, rng, call,
                                    used, (const T*)X, (T*)Y);
             else
                 hipLaunchKernelGGL((dropout_rows_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, st, n, RS, C,

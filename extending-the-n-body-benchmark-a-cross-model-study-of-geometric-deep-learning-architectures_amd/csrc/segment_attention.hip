@@ -375,7 +375,7 @@ __global__ __launch_bounds__(256) void segment_attention_chunk_kernel(nbx_segmen
             weighted_rows<T, VW>(acc, i0 + el, i1, p.EL, [&](int i) { return sW[i * H + head]; },
                                  [&](int i) { return (const T*)a.values + (int64_t)sE[i] * RL + (int64_t)f * VW; });
         if (p.EL > 1) join_groups<VW>(acc, red, p.RV, p.EL);
-        const bool before = a.ptr[v] < p0, after = a.ptr[v + 1] > p0 + cnt;
+        const bool before = a.ptr[v] < p0, after = std::min<int64_t>(a.E, a.ptr[v + 1]) > p0 + cnt;
         if (before || after) {
             const int64_t slot = 2 * c + (before ? 0 : 1);
             if (on && el == 0)
@@ -573,7 +573,7 @@ __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment
         for (int i = i0 + (t & 7); i < i1; i += 8) d += sA[i * H + h] * sD[i * H + h];
         d = sum8(d);
         if (v < 0) continue;
-        const bool before = a.ptr[v] < p0, after = a.ptr[v + 1] > p0 + cnt;
+        const bool before = a.ptr[v] < p0, after = std::min<int64_t>(a.E, a.ptr[v + 1]) > p0 + cnt;
         if ((before || after) && (t & 7) == 0) share[(2 * (int64_t)blockIdx.x + (before ? 0 : 1)) * H + h] = d;
         for (int i = i0 + (t & 7); i < i1; i += 8) {
             const float al = sA[i * H + h], dp = sD[i * H + h];

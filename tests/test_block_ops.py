@@ -227,7 +227,7 @@ def test_other_abi_refusals():
     drop = lambda **k: L.nbx_dropout(*{**dict(dtype=0, per=0, n=4, S=1, C=1, group=1, threshold=10, rng=8, call=0,   # noqa: E731
                                               used=None, X=8, Y=8, stream=None), **k}.values())
     for kw in (dict(dtype=3), dict(per=3), dict(n=-1), dict(group=0), dict(threshold=65536), dict(X=None), dict(rng=None),
-               dict(n=2 ** 41), dict(per=2, C=2 ** 20), dict(n=2 ** 39)):
+               dict(n=2 ** 41), dict(n=2 ** 39)):
         assert drop(**kw) == 1, kw
     assert drop(n=0) == 0
     sh = lib.ShResidualNormArgs(V=3, path_group=1, lmax=7, C=8, weight=8)

@@ -36,7 +36,9 @@ def _bits(a, b):
     ((1,), "element", 1), ((7, 3), "element", 1), ((33, 129), "element", 1), ((5, 4, 3, 8), "element", 1),
     ((1, 1), "group", 1), ((13, 9, 8), "group", 5), ((40, 7), "group", 3), ((6, 3000), "group", 2), ((9,), "group", 2),
     ((1, 1), "channel", 1), ((11, 9, 16), "channel", 1), ((7, 4, 61), "channel", 1), ((3, 700), "channel", 1),
-    ((2, 3, 2, 5), "channel", 1), ((3, 5, 1000), "channel", 1), ((4, 300, 9), "channel", 1)])
+    ((2, 3, 2, 5), "channel", 1), ((3, 5, 1000), "channel", 1), ((4, 300, 9), "channel", 1),
+    ((2, 3, 2047), "channel", 1), ((2, 1, 2048), "channel", 1), ((1, 3, 2049), "channel", 1), ((2, 2, 5001), "channel", 1),
+    ((1, 40, 2070), "channel", 1), ((1, 700000), "channel", 1)])
 def test_dropout(rng, dtype, shape, per, group):
     r = _rand(1)
     x, dy = r(*shape).to(dtype), r(*shape).to(dtype)
@@ -377,6 +379,38 @@ def test_attention_edges_in_no_list(hip_device, rng, lengths):
     _, dv, dl = _attention_case(hip_device, rng, lengths, 2, 2, 4, F32, F32, 0.2, extra=17)
     rest = eid[int(ptr[-1]):].long()
     assert not dv[rest].any() and not dl[rest].any()
+
+
+@pytest.mark.parametrize("lengths", [[5, 3], [70, 60]])
+def test_attention_entries_out_of_range(hip_device, lengths):
+    """An eid entry outside [0, E) counts as masked; a list is cut at E."""
+    ptr, eid = _lists(lengths, 0)
+    E = len(eid)
+    r = _rand(3)
+    v, l, dout = r(E, 1, 2, 4), r(E, 2), r(2, 1, 2, 4)
+    gone = eid[1].long().item()
+    masked = l.clone()
+    masked[gone] = -math.inf
+    ref = O.segment_attention(v, masked, ptr, eid, torch.ones(E, 2, dtype=torch.bool), 0.0, dout)
+    bad, long = eid.clone(), ptr.clone()
+    bad[1] = E + 7 if lengths[0] == 5 else -3
+    long[-1] = E + 100
+    vd, ld = v.to(hip_device).requires_grad_(), l.to(hip_device).requires_grad_()
+    out = B.segment_attention(vd, ld, long.to(hip_device), bad.to(hip_device))
+    O.within(out, ref["out"], "out")
+    dv, dl = torch.autograd.grad(out, (vd, ld), dout.to(hip_device))
+    rest = torch.arange(E) != gone                    # the edge that no list names is not written
+    for t, n in ((dv, "dvalues"), (dl, "dlogits")):
+        O.within(t[rest.to(hip_device)], O.B(ref[n].val[rest], ref[n].err[rest]), n)
+
+
+def test_library_refusals_reach_python(hip_device):
+    from nbody_amd._lib import NbxError
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=hip_device)                # noqa: E731
+    with pytest.raises(NbxError, match="H <= 64"):
+        B.segment_attention(torch.zeros(1, 1, 65, 4, device=hip_device), torch.zeros(1, 65, device=hip_device), i32(0, 1), i32(0))
+    with pytest.raises(NbxError, match="H D"):
+        B.segment_attention(torch.zeros(1, 1, 2, 1001, device=hip_device), torch.zeros(1, 2, device=hip_device), i32(0, 1), i32(0))
 
 
 def test_attention_empty(hip_device):
