@@ -65,7 +65,7 @@ def _torch_command():
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
             *(a for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                           "/opt/rocm/include", sysconfig.get_paths()["include"]) for a in ("-isystem", d)),
-            TORCH_SRC, "-o", TORCH_LIB, f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_hip", "-ltorch_cpu",
+            TORCH_SRC, "-o", TORCH_LIB, f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",
             "-ltorch_python", "-ltorch"]
 
 

@@ -5,6 +5,7 @@
 // Built by build.py with the host compiler.  Entry points are handed over by address, so this file's calls go
 // to the library that the package has loaded.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -67,11 +68,18 @@ T* ptr(const Tensor& t) {
 Tensor value_or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
-Tensor empty_if(bool wanted, const Tensor& like) { return wanted && like.defined() ? at::empty_like(like) : Tensor(); }
-Tensor used_state(const Tensor& state) { return state.defined() ? at::empty_like(state) : Tensor(); }
 
-Tensor workspace(size_t bytes, const Tensor& like) {
-    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+// A new contiguous tensor, from the allocator at once: the dispatcher's way to it takes as long again, and on
+// autograd's thread a pass allocates up to nine.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& on) {
+    return Tensor(at::detail::empty_cuda(sizes, type, on.device(), std::nullopt));
+}
+Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t); }
+Tensor empty_if(bool wanted, const Tensor& like) { return wanted && like.defined() ? fresh_like(like) : Tensor(); }
+Tensor used_state(const Tensor& state) { return state.defined() ? fresh_like(state) : Tensor(); }
+
+Tensor workspace(size_t bytes, const Tensor& on) {
+    return bytes ? fresh({(int64_t)bytes}, at::kByte, on) : Tensor();
 }
 
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
@@ -87,7 +95,7 @@ struct DropoutHow {
 };
 
 Tensor run_dropout(const Tensor& x, const DropoutHow& h, const Tensor& state, const Tensor& used) {
-    Tensor y = at::empty_like(x);
+    Tensor y = fresh_like(x);
     c10::DeviceGuard guard(x.device());
     check(entries.dropout((int32_t)h.dtype, (int32_t)h.per, h.n, h.S, h.C, h.group, (uint32_t)h.threshold,
                           ptr<int64_t>(state), (uint32_t)h.call, ptr<int64_t>(used), x.data_ptr(), y.data_ptr(),
@@ -98,7 +106,7 @@ Tensor run_dropout(const Tensor& x, const DropoutHow& h, const Tensor& state, co
 
 struct DropoutFn : torch::autograd::Function<DropoutFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& state, const DropoutHow& h) {
-        Tensor used = at::empty_like(state);
+        Tensor used = fresh_like(state);
         Tensor y = run_dropout(x, h, state, used);
         ctx->save_for_backward({used});
         ctx->saved_data["how"] = std::vector<int64_t>{h.dtype, h.per, h.n, h.S, h.C, h.group, h.threshold, h.call};
@@ -153,8 +161,8 @@ void set_params(ResidualArgs& a, const Tensor& gate, const Tensor& post_w, const
 
 std::pair<Tensor, Tensor> run_residual(ResidualArgs a, const Tensor& x, const Tensor& y, const Tensor& state,
                                        const Tensor& used, const Tensor& stats) {
-    Tensor h = at::empty(x.sizes(), x.options()), z;
-    if (a.pre_w) z = at::empty(y.sizes(), y.options());
+    Tensor h = fresh_like(x), z;
+    if (a.pre_w) z = fresh_like(y);
     a.x = x.data_ptr();
     a.y = y.data_ptr();
     a.rng = ptr<int64_t>(state);
@@ -176,7 +184,7 @@ struct ResidualFn : torch::autograd::Function<ResidualFn> {
                      pre_w = value_or_none(pre_w_), pre_b = value_or_none(pre_b_), state = value_or_none(state_);
         const bool norms = post_w.defined() || pre_w.defined();
         Tensor used = used_state(state), stats;
-        if (norms) stats = at::empty({4, a.rows}, x.options().dtype(at::kFloat));
+        if (norms) stats = fresh({4, a.rows}, at::kFloat, x);
         ctx->saved_data["how"] = bytes_of(a);
         set_params(a, gate, post_w, post_b, pre_w, pre_b);
         auto [h, z] = run_residual(a, x, y, state, used, stats);
@@ -203,8 +211,8 @@ struct ResidualFn : torch::autograd::Function<ResidualFn> {
         set_params(a, s[2], s[3], s[4], s[5], s[6]);
         const auto shape = ctx->saved_data["x"].toIntVector();
         static const at::ScalarType types[] = {at::kFloat, at::kBFloat16, at::kHalf};
-        if (ctx->needs_input_grad(0)) out[0] = at::empty(shape, any.options().dtype(types[a.x_dtype]));
-        if (ctx->needs_input_grad(1)) out[1] = at::empty(shape, any.options().dtype(types[a.y_dtype]));
+        if (ctx->needs_input_grad(0)) out[0] = fresh(shape, types[a.x_dtype], any);
+        if (ctx->needs_input_grad(1)) out[1] = fresh(shape, types[a.y_dtype], any);
         // without dz nothing reaches the norm behind the sum: its parameters' gradients are 0
         for (int i = 2, edge = 2; i < 7; ++i)   // an absent input has no edge
             if (s[i].defined()) out[i] = empty_if(ctx->needs_input_grad(edge++), s[i]);
@@ -270,7 +278,7 @@ using ShArgs = nbx_sh_residual_norm_args;
 
 std::pair<Tensor, Tensor> run_sh(ShArgs a, const Tensor& x, const Tensor& y, const Tensor& weight, const Tensor& bias,
                                  const Tensor& state, const Tensor& used, const Tensor& stats) {
-    Tensor h = at::empty_like(x), z = at::empty_like(x);
+    Tensor h = fresh_like(x), z = fresh_like(x);
     a.x = x.data_ptr();
     a.y = y.data_ptr();
     a.weight = weight.data_ptr();
@@ -289,7 +297,7 @@ struct ShFn : torch::autograd::Function<ShFn> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& y, const Tensor& weight,
                                  const Tensor& bias, const OptTensor& state_, const ShArgs& a) {
         const Tensor state = value_or_none(state_);
-        Tensor used = used_state(state), stats = at::empty({2, a.V}, x.options().dtype(at::kFloat));
+        Tensor used = used_state(state), stats = fresh({2, a.V}, at::kFloat, x);
         ctx->saved_data["how"] = bytes_of(a);
         auto [h, z] = run_sh(a, x, y, weight, bias, state, used, stats);
         ctx->save_for_backward({h, weight, bias, used, stats});
@@ -360,7 +368,7 @@ void set_lists(AttentionArgs& a, const Tensor& values, const Tensor& logits, con
 
 Tensor run_attention(AttentionArgs a, const Tensor& values, const Tensor& logits, const Tensor& lists, const Tensor& eid,
                      const Tensor& state, const Tensor& used, const Tensor& stats) {
-    Tensor out = at::empty({a.V, a.K, a.H, a.D}, values.options());
+    Tensor out = fresh({a.V, a.K, a.H, a.D}, values.scalar_type(), values);
     set_lists(a, values, logits, lists, eid);
     a.rng = ptr<int64_t>(state);
     a.used = ptr<int64_t>(used);
@@ -378,7 +386,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& values, const Tensor& logits, const Tensor& lists,
                           const Tensor& eid, const OptTensor& state_, const AttentionArgs& a) {
         const Tensor state = value_or_none(state_);
-        Tensor used = used_state(state), stats = at::empty({2, a.V, a.H}, values.options().dtype(at::kFloat));
+        Tensor used = used_state(state), stats = fresh({2, a.V, a.H}, at::kFloat, values);
         ctx->saved_data["how"] = bytes_of(a);
         Tensor out = run_attention(a, values, logits, lists, eid, state, used, stats);
         ctx->save_for_backward({values, logits, lists, eid, used, stats});
