@@ -474,7 +474,7 @@ __global__ __launch_bounds__(256) void segment_attention_join_kernel(nbx_segment
 template <typename T, int VW>
 __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment_attention_args a, SaPlan p, float keep,
                                                                      float* __restrict__ wa, float* __restrict__ wd,
-                                                                     float* __restrict__ share) {
+                                                                     float* __restrict__ share, int2* __restrict__ ends) {
     extern __shared__ float lds[];
     const int H = a.H, t = threadIdx.x;
     float* sA = lds;                       // [eb][H] alpha
@@ -555,6 +555,7 @@ __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment
         }
     }
     if (!a.dlogits) return;
+    if (t == 0) ends[blockIdx.x] = make_int2(sV[0], sV[cnt - 1]);
     __syncthreads();
     // red: a position's entries are rows of `per` per head
     const int per = a.D / VW / p.grp, rows = p.entries / (cols / p.grp);
@@ -591,18 +592,17 @@ __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment
 __global__ __launch_bounds__(256) void segment_attention_dlogits_kernel(nbx_segment_attention_args a, SaPlan p,
                                                                         const float* __restrict__ wa,
                                                                         const float* __restrict__ wd,
-                                                                        const float* __restrict__ share) {
+                                                                        const float* __restrict__ share,
+                                                                        const int2* __restrict__ ends) {
     __shared__ float red[256];
-    __shared__ int sV[64];
     const int t = threadIdx.x, H = a.H;
     const int64_t p0 = blockIdx.x * (int64_t)p.eb;
     const int cnt = (int)std::min<int64_t>(p.eb, a.E - p0);
-    if (t < 64) nodes_of_positions(a.ptr, a.V, p0, cnt, sV);
-    __syncthreads();
+    const int2 ends_here = ends[blockIdx.x];   // the nodes of the block's first and last position
     const int hs = 256 / H, h = t % H, r = t / H;
     for (int side = 0; side < 2; ++side) {
-        const int v = side ? sV[cnt - 1] : sV[0];
-        if (v < 0 || (side && v == sV[0])) continue;
+        const int v = side ? ends_here.y : ends_here.x;
+        if (v < 0 || (side && v == ends_here.x)) continue;
         const int64_t q0 = std::max(0, a.ptr[v]), q1 = std::min<int64_t>(a.E, a.ptr[v + 1]);
         if (q0 >= p0 && q1 <= p0 + cnt) continue;
         const int64_t b0 = q0 / p.eb, b1 = (q1 - 1) / p.eb;
@@ -700,7 +700,7 @@ int with_values(const nbx_segment_attention_args& a, F&& f) {
 }
 
 size_t workspace_need(const nbx_segment_attention_args& a, bool backward) {
-    if (backward) return a.dlogits ? (size_t)2 * (a.E + backward_plan(a).nc) * a.H * sizeof(float) : 0;
+    if (backward) return a.dlogits ? (size_t)2 * ((a.E + backward_plan(a).nc) * a.H + backward_plan(a).nc) * sizeof(float) : 0;
     const SaPlan p = forward_plan(a);
     return p.chunked ? (size_t)2 * p.nc * (a.K * a.H * a.D + 2 * a.H) * sizeof(float) : 0;
 }
@@ -773,7 +773,8 @@ extern "C" int nbx_segment_attention_backward(const nbx_segment_attention_args* 
     NBX_CHECK_ARG(p.nc * p.T < ((int64_t)1 << 32), "nbx_segment_attention_backward: too many edges");
     hipStream_t st = (hipStream_t)stream;
     const float keep = keep_scale(a->threshold);
-    float* wa = (float*)a->workspace;
+    int2* ends = (int2*)a->workspace;
+    float* wa = (float*)(ends + p.nc);
     float* wd = wa + a->E * a->H;
     float* share = wd + a->E * a->H;
     if (int rc = with_values(*a, [&](auto t, auto vw) -> int {
@@ -781,13 +782,14 @@ extern "C" int nbx_segment_attention_backward(const nbx_segment_attention_args* 
             constexpr int VW = decltype(vw)::value;
             const size_t lds = (size_t)(3 * p.eb * a->H + p.eb * p.entries + 196) * 4;
             hipLaunchKernelGGL((segment_attention_bwd_kernel<T, VW>), dim3((unsigned)p.nc), dim3(p.T), lds, st, *a, p, keep,
-                               wa, wd, share);
+                               wa, wd, share, ends);
             NBX_LAUNCH_CHECK("segment_attention_bwd");
             return NBX_OK;
         }))
         return rc;
     if (a->dlogits) {
-        hipLaunchKernelGGL(segment_attention_dlogits_kernel, dim3((unsigned)p.nc), dim3(256), 0, st, *a, p, wa, wd, share);
+        hipLaunchKernelGGL(segment_attention_dlogits_kernel, dim3((unsigned)p.nc), dim3(256), 0, st, *a, p, wa, wd,
+                           share, ends);
         NBX_LAUNCH_CHECK("segment_attention_dlogits");
     }
     return NBX_OK;
