@@ -39,7 +39,9 @@ __device__ __forceinline__ void note_used(int64_t* used, const int64_t* rng) {
 }
 
 // ======================================================================== dropout
-// Flat form: thread t owns elements 8 t .. 8 t + 7, which are exactly one Philox block's draws.
+// Flat form: thread t owns elements 8 t .. 8 t + 7, which are exactly one Philox block's draws (16 bits a draw:
+// with 32 the generator's 20 wide multiplies per four elements would take longer than 16-bit elements' way
+// through HBM).  33.5M bf16 elements: 24 us, 134 MB at 5.5 TB/s (partly from the last-level cache).
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_flat_kernel(int64_t total, uint32_t threshold, float scale,
                                                            const int64_t* __restrict__ rng, uint32_t call,
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(256) void dropout_flat_kernel(int64_t total, uint32
 // Row form (entries of S C elements sharing draws): a block takes 256 chunks of eight elements, of one
 // entry or of several.  CHANNEL keeps the mask of the block's channels as bits in LDS, one Philox block for
 // eight channels, shared by the S rows: all of a short row's, or the window of 2048 channels (wrapping at C)
-// that a part of a long row touches.
+// that a part of a long row touches.  8M fp32 elements: 13.5 us, 64 MB at 4.8 TB/s.
 constexpr int CHANNEL_WINDOW = 2048 / 8 + 2;
 
 template <typename T, bool CHANNEL>
@@ -161,7 +163,9 @@ __device__ __forceinline__ uint32_t row_keep(const Draws& d, int64_t row, int la
     return keep_bits(d.key, (uint64_t)(row * d.Cq + lane), d.threshold);
 }
 
-// Forward: one row per 16 / 64 lanes or per block.
+// Forward: one row per 16 / 64 lanes or per block; the draws are formed while the row is on its way.  16384 rows
+// of 2048 bf16 columns with both norms, gate and draws: 65 us, 268 MB at 4.1 TB/s (a copy: 4.8).  Several rows
+// per block with the next one prefetched take 70 us: twice the registers, half the waves.
 template <typename TX, typename TY, int W>
 __global__ __launch_bounds__(W ? 256 : 1024) void residual_norm_kernel(nbx_residual_norm_args a, float keep) {
     __shared__ float red[4][16];
@@ -229,6 +233,9 @@ struct RowPlan {
 
 RowPlan row_plan(int64_t rows, int64_t C, int64_t gate_groups) {
     RowPlan p = {};
+    // 16 lanes a row up to 128 columns, a wave up to 512, then waves (forward + backward, fp32, 16384 x 128: 42 us by
+    // 16 lanes, 65 by waves; 8192 x 256: 48.5 by waves, 51.6 by blocks; 8192 x 512: 53.8 / 55.1); past 2048 columns
+    // a block has one row and up to 16 waves, with the registers that leaves
     p.W = C <= 128 ? 16 : C <= 512 ? 64 : C <= 2048 ? 0 : -1;
     p.nw = (int)ceil_div(C, 512);
     p.rpb = p.W > 0 ? 256 / p.W : std::max(1, 4 / p.nw);
@@ -257,6 +264,9 @@ RowPlan row_plan(int64_t rows, int64_t C, int64_t gate_groups) {
 // or WHOLE) has the gate inside: SUM_A = sum of dn yhat, SUM_B = sum of dn, dn = du gate.
 enum { SUM_A, SUM_B, SUM_PRE_W, SUM_PRE_B, SUMS };
 
+// The backward pass reads y, h, dh and dz once: statistics come from the forward pass, xhat from the stored h (in
+// 16 bits that is one rounding more than the forward pass had; gradients of a 16-bit type are rounded as much
+// again).  The same 16384 x 2048 bf16 block: 94 us, 403 MB at 4.3 TB/s, and 11 us for the sums.
 template <typename TX, typename TY>
 struct RowIn {   // a row's eight columns as loaded, one row ahead of their use
     Raw8<TX> dh, h;
@@ -469,9 +479,10 @@ __global__ __launch_bounds__(W >= 0 ? 256 : 1024, W >= 0 ? 3 : 1) void residual_
     }
 }
 
-// Column sums of the partial rows.  The first jobs * ceil(C / 64) blocks: a parameter over all blocks (dpost_*
-// with each block's gate row put back), 64 columns x 16 waves, each wave every 16th row, combined in order.
-// Then gate group after group over its cpg blocks: the same, or (cpg <= 16) a thread per column.
+// Column sums of the partial rows.  The first jobs * ceil(C / 32) blocks: a parameter over all blocks (dpost_*
+// with each block's gate row put back), 32 columns x 32 slots, each slot every 32nd row, combined in order.
+// Then gate group after group over its cpg blocks: the same, or (cpg <= 16) a thread per column: 64 groups of
+// 12 partial rows of 2048 columns take 14.2 us so, 16.9 with slots.
 enum { OUT_POST_W, OUT_POST_B, OUT_PRE_W, OUT_PRE_B, OUTS };
 struct FinalSums {
     void* out[OUTS];
@@ -488,14 +499,14 @@ __device__ __forceinline__ float load1p(const void* p, int dtype, int64_t at) {
 
 __global__ __launch_bounds__(1024) void residual_norm_sums_kernel(FinalSums f, int64_t nblocks, int64_t cpg, int64_t C,
                                                                   const float* __restrict__ part) {
-    __shared__ float red[2][16][64];
-    const int tiles = (int)((C + 63) / 64), job = (int)blockIdx.x / tiles;
+    __shared__ float red[2][32][33];
+    const int tiles = (int)((C + 31) / 32), job = (int)blockIdx.x / tiles;
     const bool gates = job >= f.jobs, thread_per_column = gates && cpg <= 16;
     const int gtiles = cpg <= 16 ? (int)((C + 1023) / 1024) : tiles, gb = (int)blockIdx.x - f.jobs * tiles;
-    const int lane = threadIdx.x & 63, w = thread_per_column ? 0 : threadIdx.x >> 6;
+    const int lane = threadIdx.x & 31, w = thread_per_column ? 0 : threadIdx.x >> 5;
     const int64_t c = thread_per_column ? gb % gtiles * (int64_t)1024 + threadIdx.x
-                                        : (gates ? gb % gtiles : (int)blockIdx.x % tiles) * (int64_t)64 + lane;
-    const int k = gates ? SUM_A : f.job[job], step = thread_per_column ? 1 : 16;
+                                        : (gates ? gb % gtiles : (int)blockIdx.x % tiles) * (int64_t)32 + lane;
+    const int k = gates ? SUM_A : f.job[job], step = thread_per_column ? 1 : 32;
     const int64_t g = gates ? gb / gtiles : 0;
     const int nb = (int)(gates ? cpg : nblocks);
     const float* p = part + ((int64_t)k * nblocks + g * cpg) * C + c;
@@ -510,12 +521,15 @@ __global__ __launch_bounds__(1024) void residual_norm_sums_kernel(FinalSums f, i
             if (f.dtype == NBX_F32) with_gate((const float*)f.gate);
             else if (f.dtype == NBX_BF16) with_gate((const bf16*)f.gate);
             else with_gate((const f16*)f.gate);
+        } else if (both) {
+#pragma unroll 8
+            for (int b = w; b < nb; b += step) {
+                s += p[b * C];
+                s2 += p[(nblocks + b) * C];
+            }
         } else {
 #pragma unroll 8
             for (int b = w; b < nb; b += step) s += p[b * C];
-            if (both)
-#pragma unroll 8
-                for (int b = w; b < nb; b += step) s2 += p[(nblocks + b) * C];
         }
     }
     if (!thread_per_column) {
@@ -525,7 +539,7 @@ __global__ __launch_bounds__(1024) void residual_norm_sums_kernel(FinalSums f, i
         if (w) return;
         s = s2 = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < 32; ++i) {
             s += red[0][i][lane];
             s2 += red[1][i][lane];
         }
@@ -571,7 +585,8 @@ int with_types(const nbx_residual_norm_args& a, F&& f) {
 // A node's (lmax+1)^2 rows of C channels are cut into chunks of eight channels of one row (the last of a row may
 // be shorter), kept in the registers of TPN threads: 64 (four nodes per block) or the block; thread t holds
 // chunks t, t + TPN, .. (NJ of them).  The l = 0 row is chunks 0 .. C/8 - 1, all in the first wave, so its
-// centring needs no barrier: one block-wide sum per direction is left.
+// centring needs no barrier: one block-wide sum per direction is left.  2560 nodes of lmax 6, 128 channels, fp32:
+// forward 59 us (257 MB at 4.3 TB/s), backward 71 us (321 MB at 4.5 TB/s) and 4 us for the sums.
 constexpr int SH_MAXC = 512;
 constexpr int SH_LDS_HEAD = 64 + 2 * 4 * SH_MAXC / 8 / 4;   // floats before the rows in the backward pass's LDS
 
@@ -579,12 +594,14 @@ struct ShPlan {
     int S, cpr, chunks, tpn, nj, npb, threads;   // cpr: chunks per row; npb: nodes in flight per block
 };
 
-ShPlan sh_plan(int lmax, int C) {
+ShPlan sh_plan(int64_t V, int lmax, int C) {
     ShPlan p = {};
     p.S = (lmax + 1) * (lmax + 1);
     p.cpr = (C + 7) / 8;
     p.chunks = p.S * p.cpr;
-    if (p.chunks <= 128) {
+    // a wave per node where nodes are many and small; else a block (forward + backward of lmax 2, 64 channels: 320
+    // nodes 16.9 us by waves, 14.7 by blocks; 1024: 18.8 / 18.2; 2048: 24.9 / 25.9; 8192: 47 / 68)
+    if (p.chunks <= 128 && V >= 2048) {
         p.tpn = 64;
         p.nj = p.chunks <= 64 ? 1 : 2;
         p.npb = 4;
@@ -814,23 +831,23 @@ __global__ __launch_bounds__(SUB ? 256 : 1024) void sh_residual_norm_bwd_kernel(
     }
 }
 
-// dweight [lmax+1][C] | dbias [C] from the units' partial rows: 64 columns x 16 waves in a fixed order
+// dweight [lmax+1][C] | dbias [C] from the units' partial rows: 32 columns x 32 slots in a fixed order
 __global__ __launch_bounds__(1024) void sh_residual_sums_kernel(nbx_sh_residual_norm_args a, int64_t nunits,
                                                                 const float* __restrict__ part) {
-    __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    __shared__ float red[32][33];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t ld = (int64_t)(a.lmax + 2) * a.C;
-    const int64_t c = blockIdx.x * (int64_t)64 + lane;
+    const int64_t c = blockIdx.x * (int64_t)32 + lane;
     float s = 0.f;
     if (c < ld)
 #pragma unroll 8
-        for (int64_t u = w; u < nunits; u += 16) s += part[u * ld + c];
+        for (int64_t u = w; u < nunits; u += 32) s += part[u * ld + c];
     red[w][lane] = s;
     __syncthreads();
     if (w == 0 && c < ld) {
         float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t += red[i][lane];
+        for (int i = 0; i < 32; ++i) t += red[i][lane];
         const int64_t nw = ld - a.C;
         if (c < nw) {
             if (a.dweight) store1p(a.dweight, a.param_dtype, c, t);
@@ -997,8 +1014,8 @@ extern "C" int nbx_residual_norm_backward(const nbx_residual_norm_args* a, void*
                    a->param_dtype, 0, {}};
     for (int k = 0; k < OUTS; ++k)
         if (f.out[k]) f.job[f.jobs++] = k;
-    const int64_t blocks = f.jobs * ceil_div(C, 64) +
-                           (a->dgate && !own ? a->gate_groups * ceil_div(C, p.cpg <= 16 ? 1024 : 64) : 0);
+    const int64_t blocks = f.jobs * ceil_div(C, 32) +
+                           (a->dgate && !own ? a->gate_groups * ceil_div(C, p.cpg <= 16 ? 1024 : 32) : 0);
     if (blocks) {
         hipLaunchKernelGGL(residual_norm_sums_kernel, dim3((unsigned)blocks), dim3(1024), 0, st, f, p.nblocks, p.cpg, C,
                            part);
@@ -1011,7 +1028,7 @@ extern "C" int nbx_sh_residual_norm(const nbx_sh_residual_norm_args* a, void* st
     if (int rc = sh_check(a, "nbx_sh_residual_norm")) return rc;
     if (a->V == 0) return NBX_OK;
     NBX_CHECK_ARG(a->x && a->y && a->bias && a->h && a->z, "nbx_sh_residual_norm: null operand");
-    const ShPlan p = sh_plan(a->lmax, a->C);
+    const ShPlan p = sh_plan(a->V, a->lmax, a->C);
     NBX_CHECK_ARG(grid_ok(ceil_div(a->V, p.npb), p.threads), "nbx_sh_residual_norm: too many nodes");
     if (int rc = with_type(a->dtype, [&](auto t) { return sh_launch<false, decltype(t)>(*a, p, 0, nullptr, (hipStream_t)stream); }))
         return rc;
@@ -1022,7 +1039,7 @@ extern "C" int nbx_sh_residual_norm(const nbx_sh_residual_norm_args* a, void* st
 extern "C" int nbx_sh_residual_norm_backward_workspace_bytes(const nbx_sh_residual_norm_args* a, size_t* bytes) {
     if (int rc = sh_check(a, "nbx_sh_residual_norm_backward_workspace_bytes")) return rc;
     NBX_CHECK_ARG(bytes, "nbx_sh_residual_norm_backward_workspace_bytes: null result");
-    const ShPlan p = sh_plan(a->lmax, a->C);
+    const ShPlan p = sh_plan(a->V, a->lmax, a->C);
     *bytes = a->V ? sh_workspace(p, a->V, a->lmax, a->C) : 0;
     return NBX_OK;
 }
@@ -1031,7 +1048,7 @@ extern "C" int nbx_sh_residual_norm_backward(const nbx_sh_residual_norm_args* a,
     if (int rc = sh_check(a, "nbx_sh_residual_norm_backward")) return rc;
     NBX_CHECK_ARG(a->V >= 1, "nbx_sh_residual_norm_backward: need a node");
     NBX_CHECK_ARG(a->stats && (!a->dz || a->h), "nbx_sh_residual_norm_backward: null operand");
-    const ShPlan p = sh_plan(a->lmax, a->C);
+    const ShPlan p = sh_plan(a->V, a->lmax, a->C);
     const int64_t units = sh_units(p, a->V);
     const bool sums = a->dweight || a->dbias;
     if (sums && !(a->workspace && a->workspace_bytes >= sh_workspace(p, a->V, a->lmax, a->C))) {
@@ -1043,7 +1060,7 @@ extern "C" int nbx_sh_residual_norm_backward(const nbx_sh_residual_norm_args* a,
     if (int rc = with_type(a->dtype, [&](auto t) { return sh_launch<true, decltype(t)>(*a, p, units, part, st); })) return rc;
     NBX_LAUNCH_CHECK("sh_residual_norm_bwd");
     if (sums) {
-        hipLaunchKernelGGL(sh_residual_sums_kernel, dim3((unsigned)ceil_div((a->lmax + 2) * a->C, 64)), dim3(1024), 0, st,
+        hipLaunchKernelGGL(sh_residual_sums_kernel, dim3((unsigned)ceil_div((a->lmax + 2) * a->C, 32)), dim3(1024), 0, st,
                            *a, units, part);
         NBX_LAUNCH_CHECK("sh_residual_sums");
     }

@@ -71,7 +71,7 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 
 struct SaPlan {
     int T, RV, EL, slices;    // threads, vectors per row, edges side by side, blocks per row
-    int RB, spb;              // join: vectors of a row per block; list form: slices per block
+    int RB, spb, tile;        // join: vectors of a row per block; list form: slices per block, edges at a time
     int eb, TP, grp, entries; // backward: positions per block, threads that work, lanes of a head that shuffle,
                               // what they leave per position
     int chunked;
@@ -177,20 +177,20 @@ __device__ __forceinline__ void join_groups(float (&acc)[VW], float* red, int RV
 }
 
 // ======================================================================== forward, list form
-// A block per node and `spb` slices of T vectors of its row.  A list of up to 64 edges has its weights formed
+// A block per node and `spb` slices of T vectors of its row.  A list of up to `tile` edges has its weights formed
 // once for all slices, while the first slice's values are on their way; the next slice's are loaded before
-// this one's result is stored.
+// this one's result is stored.  640 nodes of 4 edges, rows of 49 x 8 x 16 fp32: 18 us, 80 MB at 4.4 TB/s.
 template <typename T, int VW>
 __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment_attention_args a, SaPlan p, float keep) {
     extern __shared__ float lds[];
     const int H = a.H, t = threadIdx.x;
-    float* sW = lds;                       // [TILE][H] logits, then weights
-    float* sP = sW + TILE * H;             // [TILE][H] exp(l - m)
-    float* sM = sP + TILE * H;             // [H] running maximum
+    float* sW = lds;                       // [tile][H] logits, then weights
+    float* sM = sW + p.tile * H;           // [H] running maximum
     float* sR = sM + H;                    // [H] factor of what is summed so far
     float* sS = sR + H;                    // [H] running sum
     float* red = sS + H;                   // [T VW]
-    int* sE = reinterpret_cast<int*>(red + p.T * VW);   // [TILE]
+    int* sE = reinterpret_cast<int*>(red + p.T * VW);   // [tile]
+    uint8_t* sK = reinterpret_cast<uint8_t*>(sE + p.tile);   // [tile][H]
     note_used(a);
     const DrawKey key = a.threshold ? draw_key(a.rng, a.call) : DrawKey{0, 0, 0, 0};
     const int64_t v = blockIdx.x;
@@ -214,26 +214,27 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
         for (int i = t; i < cnt * H; i += p.T) {
             const int e = sE[i / H];
             sW[i] = e < 0 ? -INFINITY : load_logit(a, (int64_t)e * H + i % H);
+            sK[i] = !a.threshold || keep_one(key, (uint64_t)(int64_t)e * H + i % H, a.threshold);
         }
         __syncthreads();
-        if (t < H) {
-            float m = sM[t];
-            for (int i = 0; i < cnt; ++i) m = fmaxf(m, sW[i * H + t]);
-            sR[t] = sM[t] == -INFINITY ? 0.f : __expf(sM[t] - m);
-            sM[t] = m;
+        for (int h = t >> 3; h < H; h += p.T >> 3) {   // 8 lanes per head
+            float m = -INFINITY, s = 0.f;
+            for (int i = t & 7; i < cnt; i += 8) m = fmaxf(m, sW[i * H + h]);
+            const float m0 = sM[h], s0 = sS[h], m1 = fmaxf(m0, max8(m));
+            for (int i = t & 7; i < cnt; i += 8) {
+                const float w = weight_of(sW[i * H + h], finite_max(m1));
+                s += w;
+                sW[i * H + h] = sK[i * H + h] ? w : 0.f;
+            }
+            s = sum8(s);
+            if ((t & 7) == 0) {   // the 8 lanes have read what this replaces
+                const float r = m0 == -INFINITY ? 0.f : __expf(m0 - m1);
+                sR[h] = r;
+                sM[h] = m1;
+                sS[h] = s0 * r + s;
+            }
         }
         __syncthreads();
-        for (int i = t; i < cnt * H; i += p.T) {
-            const float w = weight_of(sW[i], finite_max(sM[i % H]));
-            sP[i] = w;
-            sW[i] = !a.threshold || keep_one(key, (uint64_t)(int64_t)sE[i / H] * H + i % H, a.threshold) ? w : 0.f;
-        }
-        __syncthreads();
-        if (t < H) {
-            float s = sS[t] * sR[t];
-            for (int i = 0; i < cnt; ++i) s += sP[i * H + t];
-            sS[t] = s;
-        }
     };
     auto finish = [&](float (&acc)[VW], int f, int head) {   // after a barrier that follows the sums
         if (is_on(f) && el == 0) {
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
         }
     };
     auto head_of = [&](int f) { return is_on(f) ? (f * VW / a.D) % H : 0; };
-    if (j1 - j0 <= TILE) {
+    if (j1 - j0 <= p.tile) {
         const int cnt = std::max(0, j1 - j0);
         RawV<T, VW> x[AHEAD];
         auto fetch = [&](int f) {
@@ -259,7 +260,6 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
             sS[t] = 0.f;
         }
         weigh(j0, cnt, [&] { fetch(column(s0)); });
-        __syncthreads();
         for (int s = s0; s < s1; ++s) {
             const int f = column(s), head = head_of(f);
             float acc[VW] = {};
@@ -287,8 +287,8 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
                 sM[t] = -INFINITY;
                 sS[t] = 0.f;
             }
-            for (int b = j0; b < j1; b += TILE) {
-                const int cnt = std::min(TILE, j1 - b);
+            for (int b = j0; b < j1; b += p.tile) {
+                const int cnt = std::min(p.tile, j1 - b);
                 weigh(b, cnt, [] {});
                 const float r = sR[head];
 #pragma unroll
@@ -309,6 +309,8 @@ __global__ __launch_bounds__(256) void segment_attention_list_kernel(nbx_segment
 }
 
 // ======================================================================== forward, chunk form
+// 60000 edges of 8 x 64 bf16 to 96 nodes: 19 us (61 MB at 3.2 TB/s: the searches, logits and softmax come before
+// the values) and 9.5 us for the join, whose longest list has 96 parts.
 // partial sums of the lists that cross chunk c's borders: slot 2 c = the list that began before it, slot
 // 2 c + 1 = the list that begins in it and goes on: acc [2 nc][RL] unnormalised, ms [2 nc][2][H] (max, sum)
 template <typename T, int VW>
@@ -470,7 +472,8 @@ __global__ __launch_bounds__(256) void segment_attention_join_kernel(nbx_segment
 // dl = a (dp - sum over the list of a dp).  A list that crosses the block's borders leaves its a, dp (per
 // position) and its share of the sum: slot 2 block = the list that began before, 2 block + 1 = the one that
 // goes on.  Threads: EL groups of RV, or (long rows) TP threads, a multiple of the H D / VW columns, over the
-// row in steps of TP: either way a thread stays with one head.
+// row in steps of TP: either way a thread stays with one head.  2560 edges of 49 x 8 x 16 fp32: 35.5 us (145 MB at
+// 4.1 TB/s) + 3.5; 60000 edges of 8 x 64 bf16: 30 us (123 MB at 4.1 TB/s) + 8 for the lists that cross.
 template <typename T, int VW>
 __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment_attention_args a, SaPlan p, float keep,
                                                                      float* __restrict__ wa, float* __restrict__ wd,
@@ -657,7 +660,15 @@ SaPlan forward_plan(const nbx_segment_attention_args& a) {
     p.RV = (int)(a.K * a.H * a.D / VW);
     p.EL = p.RV <= p.T ? p.T / p.RV : 1;
     p.slices = p.RV <= p.T ? 1 : (int)ceil_div(p.RV, p.T);
-    p.chunked = a.E >= 32 * a.V;
+    // The lists' lengths are on the device.  E a multiple of V is taken for lists of one length (a fully connected
+    // graph): the list form up to 128 edges (K 1, 8 heads of 16, fp32, both passes: 4096 x 7 37 us against 53 in
+    // chunks, 2048 x 15 31 / 43, 1040 x 64 40 / 43, 516 x 128 43 / 47).  Otherwise chunks, which do not wait for the
+    // longest list (ragged lists, 60000 edges to 3000 nodes: 61 us against 107 in list form, to 1000: 52 / 156;
+    // 20000 to 2000: 61 / 58), but for small graphs, where the list form's single launch counts.
+    p.chunked = a.V && a.E % a.V == 0 ? a.E > 128 * a.V : a.E > 1024;
+    // edges whose weights a list's block forms at once: 256 for long lists (60000 edges to 1000 nodes in list form:
+    // 127 us against 151 at 64), 64 where lists are short or heads many, for the LDS
+    p.tile = a.E <= 8 * a.V || a.H > 32 ? TILE : 4 * TILE;
     // about 1024 blocks or more: 640 nodes of 7 slices take 24.4 us at one slice per block, 20.3 at two, 18.1 at
     // four, 19.2 at seven
     p.spb = (int)ceil_div(p.slices, std::min<int64_t>(p.slices, std::max<int64_t>(1, ceil_div(1024, std::max<int64_t>(1, a.V)))));
@@ -676,10 +687,15 @@ SaPlan backward_plan(const nbx_segment_attention_args& a) {
     p.grp = g <= 64 && (g & (g - 1)) == 0 ? g : 1;
     p.entries = std::min(p.RV, p.TP) / p.grp;
     // positions per block: enough blocks for the chip first, then few (each has its searches and sums), within
-    // 48 KB of LDS
+    // 48 KB of LDS: 60000 edges of 8 x 64 bf16 take 46 us at 16, 40 at 32, 38 at 64; long rows (2560 edges of 49 x 8
+    // x 16 fp32) 40 us at 2, 38 at 4, 48 at 8, 77 at 16
     p.eb = p.RV <= p.T ? TILE : 4;
     while (p.eb > 4 && (a.E < 768 * (int64_t)p.eb || p.eb * (p.entries + 3 * a.H) > 12288)) p.eb /= 2;
     p.eb = std::max(p.eb, std::min(p.EL, TILE));
+    // lists of one length (a fully connected graph): whole lists per block, so that none crosses
+    const int64_t d = a.V && a.E % a.V == 0 ? a.E / a.V : 0;
+    if (d >= 1 && d <= p.eb) p.eb = (int)(p.eb / d * d);
+    else if (d > p.eb && d <= std::min(2 * p.eb, TILE) && d * (p.entries + 3 * a.H) <= 12288) p.eb = (int)d;
     p.nc = ceil_div(a.E, p.eb);
     return p;
 }
@@ -733,7 +749,7 @@ extern "C" int nbx_segment_attention(const nbx_segment_attention_args* a, void* 
         using T = decltype(t);
         constexpr int VW = decltype(vw)::value;
         if (!p.chunked) {
-            const size_t lds = (size_t)(2 * TILE * a->H + 3 * a->H + p.T * VW + TILE) * 4;
+            const size_t lds = (size_t)(p.tile * a->H + 3 * a->H + p.T * VW + p.tile) * 4 + p.tile * a->H;
             hipLaunchKernelGGL((segment_attention_list_kernel<T, VW>), dim3((unsigned)a->V, (unsigned)ceil_div(p.slices, p.spb)),
                                dim3(p.T), lds, st, *a, p, keep);
             NBX_LAUNCH_CHECK("segment_attention_list");
