@@ -236,7 +236,7 @@ RowPlan row_plan(int64_t rows, int64_t C, int64_t gate_groups) {
     // 16 lanes a row up to 128 columns, a wave up to 512, then waves (forward + backward, fp32, 16384 x 128: 42 us by
     // 16 lanes, 65 by waves; 8192 x 256: 48.5 by waves, 51.6 by blocks; 8192 x 512: 53.8 / 55.1); past 2048 columns
     // a block has one row and up to 16 waves, with the registers that leaves
-    p.W = C <= 128 ? 16 : C <= 512 ? 64 : C <= 2048 ? 0 : -1;
+    p.W = C <= 128 ? 16 : C <= 512 ? 64 : C <= 2048 ? 0 : C <= 4096 ? -1 : -2;
     p.nw = (int)ceil_div(C, 512);
     p.rpb = p.W > 0 ? 256 / p.W : std::max(1, 4 / p.nw);
     p.threads = p.W > 0 ? 256 : p.rpb * p.nw * 64;
@@ -264,12 +264,12 @@ RowPlan row_plan(int64_t rows, int64_t C, int64_t gate_groups) {
 // or WHOLE) has the gate inside: SUM_A = sum of dn yhat, SUM_B = sum of dn, dn = du gate.
 enum { SUM_A, SUM_B, SUM_PRE_W, SUM_PRE_B, SUMS };
 
-// The backward pass reads y, h, dh and dz once: statistics come from the forward pass, xhat from the stored h (in
-// 16 bits that is one rounding more than the forward pass had; gradients of a 16-bit type are rounded as much
-// again).  The same 16384 x 2048 bf16 block: 94 us, 403 MB at 4.3 TB/s, and 11 us for the sums.
+// The backward pass reads y, h, dh and dz once; statistics come from the forward pass.  A 16-bit h has lost what
+// xhat needs (the weight gradients would be off by its rounding again), so there x is read in its place and h
+// is formed again from x and y.  The same 16384 x 2048 bf16 block: 94 us, 403 MB at 4.3 TB/s, and 11 us for the sums.
 template <typename TX, typename TY>
 struct RowIn {   // a row's eight columns as loaded, one row ahead of their use
-    Raw8<TX> dh, h;
+    Raw8<TX> dh, h;   // h: x where h is formed again
     Raw8<TY> dz, y;
     float mu1, rs1, mu2, rs2;
     int64_t r;
@@ -277,7 +277,7 @@ struct RowIn {   // a row's eight columns as loaded, one row ahead of their use
 };
 
 template <typename TX, typename TY, int W, bool NORM, bool OWN>
-__global__ __launch_bounds__(W >= 0 ? 256 : 1024, W >= 0 ? 3 : 1) void residual_norm_bwd_kernel(nbx_residual_norm_args a, RowPlan p,
+__global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1) void residual_norm_bwd_kernel(nbx_residual_norm_args a, RowPlan p,
                                                                                     float keep,
                                                                                     float* __restrict__ part) {
     __shared__ float red[4][16][2];
@@ -315,13 +315,14 @@ __global__ __launch_bounds__(W >= 0 ? 256 : 1024, W >= 0 ? 3 : 1) void residual_
     if (a.threshold) d.key = draw_key(a.rng, a.call);
     const float s = a.scale * keep, invC = 1.0f / (float)C;
     const bool rowgate = OWN && !p.whole, post = NORM && a.post_w, pre = NORM && a.pre_w && a.dz;
-    const bool need_y = post || a.dgate;
+    constexpr bool AGAIN = sizeof(TX) == 2;
+    const bool need_y = post || a.dgate || (AGAIN && pre);
     float acc[SUMS][8] = {}, ag[OWN ? 8 : 1] = {};
-    float pw[8], pb[OWN ? 8 : 1] = {}, qw[8], gt[8];
+    float pw[8], pb[OWN || (AGAIN && NORM) ? 8 : 1] = {}, qw[8], gt[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) gt[i] = 1.f;
     if (post) load8p(a.post_w, a.param_dtype, c0, cn, pw);
-    if constexpr (OWN)
+    if constexpr (OWN || (AGAIN && NORM))
         if (post && a.post_b) load8p(a.post_b, a.param_dtype, c0, cn, pb);
     if (pre) load8p(a.pre_w, a.param_dtype, c0, cn, qw);
     // the slot's rows: first, past the last, step; all slots of a block run `iters` rows
@@ -340,9 +341,12 @@ __global__ __launch_bounds__(W >= 0 ? 256 : 1024, W >= 0 ? 3 : 1) void residual_
         iters = (p.cs + p.rpb - 1) / p.rpb;
         if constexpr (!OWN) {
             if (a.gate) load8p(a.gate, a.param_dtype, g * a.C + c0, cn, gt);
-            if (post)   // the norm's weight and the gate act on the same values
+            if (post)   // the norm's weight (and, for h again, its bias) and the gate act on the same values
 #pragma unroll
-                for (int i = 0; i < 8; ++i) gt[i] *= i < cn ? pw[i] : 0.f;
+                for (int i = 0; i < 8; ++i) {
+                    if constexpr (AGAIN && NORM) pb[i] *= gt[i];
+                    gt[i] *= i < cn ? pw[i] : 0.f;
+                }
         }
     }
     using In = RowIn<TX, TY>;
@@ -353,7 +357,8 @@ __global__ __launch_bounds__(W >= 0 ? 256 : 1024, W >= 0 ? 3 : 1) void residual_
         fetch8n((const TX*)a.dh + row + (uint32_t)c0, a.dh ? in.n : 0, in.dh);
         if (pre) {
             fetch8n((const TY*)a.dz + row + (uint32_t)c0, in.n, in.dz);
-            fetch8n((const TX*)a.h + row + (uint32_t)c0, in.n, in.h);
+            if constexpr (AGAIN) fetch8n((const TX*)a.x + in.r * a.ldx + (uint32_t)c0, in.n, in.h);
+            else fetch8n((const TX*)a.h + row + (uint32_t)c0, in.n, in.h);
             in.mu2 = a.stats[2 * a.rows + in.r];
             in.rs2 = a.stats[3 * a.rows + in.r];
         }
@@ -375,14 +380,30 @@ __global__ __launch_bounds__(W >= 0 ? 256 : 1024, W >= 0 ? 3 : 1) void residual_
             else if (left == 0) load8p(a.gate, a.param_dtype, in.r / p.rpg * a.C + c0, n, gt);
         }
         float t[8], v[8], e[8];
+        const uint32_t m = row_keep(d, in.r, lane);
         unpack8(in.dh, t);
         if (pre) {
-            unpack8(in.dz, e);
             unpack8(in.h, v);
+            if constexpr (AGAIN) {
+                float u[8];
+                unpack8(in.y, u);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (post) {
+                        u[k] = (u[k] - in.mu1) * in.rs1;
+                        // gt holds the gate times the weight (OWN: the gate alone)
+                        if constexpr (NORM) u[k] = OWN ? (u[k] * pw[k] + pb[k]) * gt[k] : u[k] * gt[k] + pb[k];
+                    } else {
+                        u[k] *= gt[k];
+                    }
+                    v[k] += (m >> k & 1) && k < n ? s * u[k] : 0.f;
+                }
+            }
+            unpack8(in.dz, e);
             float s1 = 0.f, s2 = 0.f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                v[k] = (v[k] - in.mu2) * in.rs2;   // from h as it is stored
+                v[k] = (v[k] - in.mu2) * in.rs2;
                 acc[SUM_PRE_W][k] += e[k] * v[k];  // past the row e is 0
                 acc[SUM_PRE_B][k] += e[k];
                 e[k] *= k < n ? qw[k] : 0.f;
@@ -396,7 +417,6 @@ __global__ __launch_bounds__(W >= 0 ? 256 : 1024, W >= 0 ? 3 : 1) void residual_
             for (int k = 0; k < 8; ++k) t[k] += in.rs2 * (e[k] - s1 - v[k] * s2);
         }
         if (a.dx) store8n((TX*)a.dx + row + (uint32_t)c0, n, t);
-        const uint32_t m = row_keep(d, in.r, lane);
 #pragma unroll
         for (int k = 0; k < 8; ++k) t[k] = (m >> k & 1) && k < n ? s * t[k] : 0.f;
         if (need_y) {
@@ -739,6 +759,7 @@ __global__ __launch_bounds__(SUB ? 256 : 1024) void sh_residual_norm_bwd_kernel(
     const int t = SUB ? (int)threadIdx.x & 63 : (int)threadIdx.x, sub = SUB ? (int)threadIdx.x >> 6 : 0;
     const int64_t unit = SUB ? blockIdx.x * (int64_t)4 + sub : blockIdx.x;
     const int C = a.C;
+    constexpr bool AGAIN = sizeof(T) == 2;   // a 16-bit h has lost what the norm's gradient needs: x + k y again
     const float k = (a.path_threshold ? k1 : 1.f) * (a.channel_threshold ? k2 : 1.f);
     DrawKey key = {0, 0, 0, 0};
     if (a.path_threshold | a.channel_threshold) key = draw_key(a.rng, a.call);
@@ -769,15 +790,25 @@ __global__ __launch_bounds__(SUB ? 256 : 1024) void sh_residual_norm_bwd_kernel(
         const float m0 = a.stats[v], rs = a.stats[a.V + v];
         float g[NJ][8], hc[NJ][8], dh[NJ][8];
         float dot = 0.f, sg = 0.f;
+        uint32_t path = 0xFFu;
+        if (a.path_threshold)
+            path = keep_one(key, (uint64_t)(v / a.path_group), a.path_threshold) ? 0xFFu : 0u;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int n = q[j].n;
             load8n((const T*)a.dz + base + q[j].at, a.dz ? n : 0, g[j]);
-            load8n((const T*)a.h + base + q[j].at, a.dz ? n : 0, hc[j]);
+            load8n((const T*)(AGAIN ? a.x : a.h) + base + q[j].at, a.dz ? n : 0, hc[j]);
             load8n((const T*)a.dh + base + q[j].at, a.dh ? n : 0, dh[j]);
         }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
+            if constexpr (AGAIN) {
+                const uint32_t m = a.channel_threshold ? path & bt[q[j].c8] : path;
+                float y[8];
+                load8n((const T*)a.y + base + q[j].at, a.dz ? q[j].n : 0, y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) hc[j][e] += (m >> e & 1) ? k * y[e] : 0.f;
+            }
             if (j == 0 && q[0].first) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -797,9 +828,6 @@ __global__ __launch_bounds__(SUB ? 256 : 1024) void sh_residual_norm_bwd_kernel(
         dot = node_sum<SUB>(dot, red, slot) / (float)C;
         // the centred row sums to 0, so only g is left of the l = 0 row's mean
         const float dm = t < 64 ? lanes_sum<64>(sg) / (float)C : 0.f;
-        uint32_t path = 0xFFu;
-        if (a.path_threshold)
-            path = keep_one(key, (uint64_t)(v / a.path_group), a.path_threshold) ? 0xFFu : 0u;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const uint32_t m = a.channel_threshold ? path & bt[q[j].c8] : path;
@@ -978,7 +1006,8 @@ extern "C" int nbx_residual_norm_backward(const nbx_residual_norm_args* a, void*
     if (int rc = residual_check(a, "nbx_residual_norm_backward")) return rc;
     NBX_CHECK_ARG(a->rows >= 1, "nbx_residual_norm_backward: need a row");
     NBX_CHECK_ARG((!a->post_w && !a->dgate) || a->y, "nbx_residual_norm_backward: null y");
-    NBX_CHECK_ARG(!a->pre_w || !a->dz || a->h, "nbx_residual_norm_backward: null h");
+    const bool again = a->x_dtype != NBX_F32;   // h is formed again from x and y
+    NBX_CHECK_ARG(!a->pre_w || !a->dz || (again ? a->x && a->y : a->h != nullptr), "nbx_residual_norm_backward: null h");
     NBX_CHECK_ARG((!a->pre_w && !a->post_w) || a->stats, "nbx_residual_norm_backward: null stats");
     NBX_CHECK_ARG((!a->dgate || a->gate) && ((!a->dpost_w && !a->dpost_b) || a->post_w) &&
                       ((!a->dpre_w && !a->dpre_b) || a->pre_w),
@@ -1004,7 +1033,8 @@ extern "C" int nbx_residual_norm_backward(const nbx_residual_norm_args* a, void*
                             : (own ? residual_norm_bwd_kernel<TX, TY, W, false, true> : residual_norm_bwd_kernel<TX, TY, W, false, false>);
             };
             auto k = p.W == 16 ? pick(std::integral_constant<int, 16>{}) : p.W == 64 ? pick(std::integral_constant<int, 64>{})
-                   : p.W == 0 ? pick(std::integral_constant<int, 0>{}) : pick(std::integral_constant<int, -1>{});
+                   : p.W == 0 ? pick(std::integral_constant<int, 0>{}) : p.W == -1 ? pick(std::integral_constant<int, -1>{})
+                                                                                                : pick(std::integral_constant<int, -2>{});
             hipLaunchKernelGGL(k, dim3((unsigned)p.nblocks), dim3(p.threads), 0, st, *a, p, keep, part);
             NBX_LAUNCH_CHECK("residual_norm_bwd");
             return NBX_OK;
@@ -1047,7 +1077,8 @@ extern "C" int nbx_sh_residual_norm_backward_workspace_bytes(const nbx_sh_residu
 extern "C" int nbx_sh_residual_norm_backward(const nbx_sh_residual_norm_args* a, void* stream) {
     if (int rc = sh_check(a, "nbx_sh_residual_norm_backward")) return rc;
     NBX_CHECK_ARG(a->V >= 1, "nbx_sh_residual_norm_backward: need a node");
-    NBX_CHECK_ARG(a->stats && (!a->dz || a->h), "nbx_sh_residual_norm_backward: null operand");
+    NBX_CHECK_ARG(a->stats && (!a->dz || (a->dtype == NBX_F32 ? a->h != nullptr : a->x && a->y)),
+                  "nbx_sh_residual_norm_backward: null operand");
     const ShPlan p = sh_plan(a->V, a->lmax, a->C);
     const int64_t units = sh_units(p, a->V);
     const bool sums = a->dweight || a->dbias;

@@ -188,9 +188,10 @@ struct ResidualFn : torch::autograd::Function<ResidualFn> {
         ctx->saved_data["how"] = bytes_of(a);
         set_params(a, gate, post_w, post_b, pre_w, pre_b);
         auto [h, z] = run_residual(a, x, y, state, used, stats);
-        // y is read again for its norm and the gate's gradient only, h for the norm behind it
-        const bool keep_y = post_w.defined() || (gate.defined() && gate.requires_grad());
-        ctx->save_for_backward({keep_y ? y : Tensor(), z.defined() ? h : Tensor(), gate, post_w, post_b, pre_w, pre_b, used,
+        // y is read again for its norm and the gate's gradient; for the norm behind the sum h, or in 16 bits x and y
+        const bool again = z.defined() && a.x_dtype != NBX_F32;
+        const bool keep_y = again || post_w.defined() || (gate.defined() && gate.requires_grad());
+        ctx->save_for_backward({keep_y ? y : Tensor(), again ? x : z.defined() ? h : Tensor(), gate, post_w, post_b, pre_w, pre_b, used,
                                 stats});
         ctx->saved_data["x"] = x.sizes().vec();
         ctx->set_materialize_grads(false);
@@ -204,8 +205,12 @@ struct ResidualFn : torch::autograd::Function<ResidualFn> {
         if (!dh.defined() && !dz.defined()) return out;
         auto a = args_of<ResidualArgs>(ctx);
         const auto s = ctx->get_saved_variables();
-        const Tensor &used = s[7], &stats = s[8], h = dense(s[1]);
-        Tensor y = s[0];
+        const Tensor &used = s[7], &stats = s[8];
+        Tensor y = s[0], h = s[1], x;
+        if (h.defined() && a.x_dtype != NBX_F32) {
+            std::tie(x, a.ldx) = rows_of(h, a.C);
+            h = Tensor();
+        }
         if (y.defined()) std::tie(y, a.ldy) = rows_of(y, a.C);   // saved-tensor hooks may give other strides
         const Tensor& any = dh.defined() ? dh : dz;
         set_params(a, s[2], s[3], s[4], s[5], s[6]);
@@ -216,6 +221,7 @@ struct ResidualFn : torch::autograd::Function<ResidualFn> {
         // without dz nothing reaches the norm behind the sum: its parameters' gradients are 0
         for (int i = 2, edge = 2; i < 7; ++i)   // an absent input has no edge
             if (s[i].defined()) out[i] = empty_if(ctx->needs_input_grad(edge++), s[i]);
+        a.x = ptr(x);
         a.y = ptr(y);
         a.h = ptr(h);
         a.rng = ptr<int64_t>(used);
@@ -300,7 +306,8 @@ struct ShFn : torch::autograd::Function<ShFn> {
         Tensor used = used_state(state), stats = fresh({2, a.V}, at::kFloat, x);
         ctx->saved_data["how"] = bytes_of(a);
         auto [h, z] = run_sh(a, x, y, weight, bias, state, used, stats);
-        ctx->save_for_backward({h, weight, bias, used, stats});
+        const bool again = a.dtype != NBX_F32;   // the backward pass forms h again from x and y
+        ctx->save_for_backward({again ? x : h, weight, bias, used, stats, again ? y : Tensor()});
         ctx->set_materialize_grads(false);
         return {h, z};
     }
@@ -312,7 +319,9 @@ struct ShFn : torch::autograd::Function<ShFn> {
         auto a = args_of<ShArgs>(ctx);
         const auto s = ctx->get_saved_variables();
         for (int i = 0; i < 4; ++i) out[i] = empty_if(ctx->needs_input_grad(i), s[i < 2 ? 0 : i - 1]);
-        a.h = ptr(s[0]);
+        if (a.dtype != NBX_F32) a.x = ptr(s[0]);
+        else a.h = ptr(s[0]);
+        a.y = ptr(s[5]);
         a.weight = ptr(s[1]);
         a.bias = ptr(s[2]);
         a.rng = ptr<int64_t>(s[3]);

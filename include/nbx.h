@@ -961,7 +961,8 @@ int nbx_dropout(int32_t dtype, int32_t per, int64_t n, int64_t S, int64_t C, int
  * *_b NULL: no bias; gate NULL: none, else [gate_groups][C], one row for each rows / gate_groups consecutive
  * rows.  Draws: group 0: draw = row Cp + column (Cp = C rounded up to 8); group r > 0: one for each r rows.
  * stats (fp32 [4][rows]: mean and 1/sqrt(.. + eps) of the y norm, then of the h norm; NULL: not kept) is what
- * the backward call reads next to y and h.  x and y rows are ldx / ldy elements apart; everything else is
+ * the backward call reads next to y (for post_w and dgate) and, for pre_w, h in fp32 or x and y in 16 bits (a 16-bit
+ * h has lost what the norm's gradient needs; it is formed again).  x and y rows are ldx / ldy elements apart; everything else is
  * contiguous. */
 typedef struct nbx_residual_norm_args {
     int64_t rows, C, ldx, ldy, gate_groups, group;
@@ -988,7 +989,8 @@ int nbx_residual_norm_backward(const nbx_residual_norm_args* a, void* stream);
  * (lmax <= 6, C <= 512): h = x + k1 k2 y, z = norm(h; weight [lmax+1][C], bias [C]).  k1: one draw for each
  * path_group consecutive nodes (path_threshold, call); k2: one for each (node, channel), draw = node Cp + c
  * (channel_threshold, call + 1).  x, y, h, z and gradients in dtype, weight / bias in param_dtype (fp32 or
- * dtype); stats fp32 [2][V] = (l = 0 mean, scale).  All contiguous. */
+ * dtype); stats fp32 [2][V] = (l = 0 mean, scale).  The backward call reads h in fp32, x and y in 16 bits.  All
+ * contiguous. */
 typedef struct nbx_sh_residual_norm_args {
     int64_t V, path_group;
     int32_t lmax, C, dtype, param_dtype;

@@ -196,10 +196,8 @@ def residual_norm(x, y, gate, post, pre, kind, eps, scale, k, p, dh=None, dz=Non
     t = B(dh) if dh is not None else B(torch.zeros(R, C))
     if pre is not None:
         dzb = B(dz) if dz is not None else B(torch.zeros(R, C))
-        # the backward pass forms xhat from h as it is stored: (h (1 + d) - mu) r
-        stored = B(hhat.val, hhat.err + out["h"].err * (rh.val + rh.err))
-        t = t + _norm_back(dzb * B(pre[0]), stored, rh, kind)
-        out["dpre_w"], out["dpre_b"] = (dzb * stored).sum(0), dzb.sum(0)
+        t = t + _norm_back(dzb * B(pre[0]), hhat, rh, kind)
+        out["dpre_w"], out["dpre_b"] = (dzb * hhat).sum(0), dzb.sum(0)
     out["dx"] = t.rounded(x.dtype)
     du = (t * drop).where(k)
     if gate is not None:
@@ -235,10 +233,9 @@ def sh_residual_norm(x, y, w, b, eps, k, factor, dh=None, dz=None):
     if dh is None and dz is None:
         return out
     dzb = B(dz) if dz is not None else B(torch.zeros(V, S, C))
-    hs = B(hc.val, hc.err + out["h"].err)          # from h as it is stored
     g = dzb * wd
-    coef = (g * hs).sum((1, 2), True) * r * r * r * (1.0 / C)
-    t = g * r - hs * bal * coef
+    coef = (g * hc).sum((1, 2), True) * r * r * r * (1.0 / C)
+    t = g * r - hc * bal * coef
     # the mean of the l = 0 row of t: the centred row's share is 0 up to its rounding
     m = t[:, :1].mean(-1, True)
     t = t - B(torch.where(first, m.val, 0.0), torch.where(first, m.err, 0.0))
@@ -246,7 +243,7 @@ def sh_residual_norm(x, y, w, b, eps, k, factor, dh=None, dz=None):
         t = t + B(dh)
     out["dx"] = t.rounded(x.dtype)
     out["dy"] = (t * f).where(k).rounded(y.dtype)
-    rows = (dzb * hs * r).sum(0)
+    rows = (dzb * hc * r).sum(0)
     out["dw"] = B(torch.zeros(L + 1, C, dtype=torch.float64).index_add_(0, deg, rows.val),
                   torch.zeros(L + 1, C, dtype=torch.float64).index_add_(0, deg, rows.err + 13 * EPS * rows.val.abs())).rounded(w.dtype)
     out["db"] = dzb[:, 0].sum(0).rounded(b.dtype)
