@@ -244,8 +244,9 @@ RowPlan row_plan(int64_t rows, int64_t C, int64_t gate_groups) {
     p.rpg = rows / groups;
     // up to 768 blocks, three on each CU at its 168 registers; each leaves one partial row per sum, read once
     // more.  16384 rows of 2048 bf16 columns, kernel + sums: 109 + 10 us at 512 blocks, 94 + 14 at 768, 110 + 18
-    // at 1024 (149 + 19 at four blocks to a CU: the registers spill)
-    const int64_t chunk = std::max<int64_t>(p.rpb, ceil_div(rows, 768));
+    // at 1024 (149 + 19 at four blocks to a CU: the registers spill).  Rows of more than 2048 columns have one block
+    // to a CU: 4096 rows of 8192, 180 + 14 us at 256 blocks, 191 + 23 at 512, 217 + 31 at 768
+    const int64_t chunk = std::max<int64_t>(p.rpb, ceil_div(rows, p.W >= 0 ? 768 : 256));
     p.whole = p.rpg < chunk && groups > 1;
     if (p.whole) {
         p.gps = std::max<int64_t>(1, chunk / p.rpb / p.rpg);
@@ -266,7 +267,7 @@ enum { SUM_A, SUM_B, SUM_PRE_W, SUM_PRE_B, SUMS };
 
 // The backward pass reads y, h, dh and dz once; statistics come from the forward pass.  A 16-bit h has lost what
 // xhat needs (the weight gradients would be off by its rounding again), so there x is read in its place and h
-// is formed again from x and y.  The same 16384 x 2048 bf16 block: 94 us, 403 MB at 4.3 TB/s, and 11 us for the sums.
+// is formed again from x and y.  The same 16384 x 2048 bf16 block: 100 us, 403 MB at 4.0 TB/s, and 11 us for the sums.
 template <typename TX, typename TY>
 struct RowIn {   // a row's eight columns as loaded, one row ahead of their use
     Raw8<TX> dh, h;   // h: x where h is formed again
@@ -316,6 +317,9 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
     const float s = a.scale * keep, invC = 1.0f / (float)C;
     const bool rowgate = OWN && !p.whole, post = NORM && a.post_w, pre = NORM && a.pre_w && a.dz;
     constexpr bool AGAIN = sizeof(TX) == 2;
+    // at 16 waves a block (128 registers a thread) no row is fetched ahead and the weights are read per row: 4096 rows
+    // of 8192 bf16 columns 217 us, fetched ahead with spills 264 (fp32: 225 / 350)
+    constexpr bool LEAN = W == -2;
     const bool need_y = post || a.dgate || (AGAIN && pre);
     float acc[SUMS][8] = {}, ag[OWN ? 8 : 1] = {};
     float pw[8], pb[OWN || (AGAIN && NORM) ? 8 : 1] = {}, qw[8], gt[8];
@@ -324,7 +328,7 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
     if (post) load8p(a.post_w, a.param_dtype, c0, cn, pw);
     if constexpr (OWN || (AGAIN && NORM))
         if (post && a.post_b) load8p(a.post_b, a.param_dtype, c0, cn, pb);
-    if (pre) load8p(a.pre_w, a.param_dtype, c0, cn, qw);
+    if (pre && !LEAN) load8p(a.pre_w, a.param_dtype, c0, cn, qw);
     // the slot's rows: first, past the last, step; all slots of a block run `iters` rows
     int64_t r0, r1, step, iters, left = 0;
     if (p.whole) {
@@ -369,10 +373,16 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
         }
     };
     In in;
-    fetch(r0, in);
+    if (!LEAN) fetch(r0, in);
     for (int64_t i = 0; i < iters; ++i) {
         In next;
-        if (i + 1 < iters) fetch(r0 + (i + 1) * step, next);
+        if constexpr (LEAN) {
+            asm volatile("" ::: "memory");   // what is read per row is not kept in registers over the rows
+            fetch(r0 + i * step, in);
+            if (pre) load8p(a.pre_w, a.param_dtype, c0, cn, qw);
+        } else if (i + 1 < iters) {
+            fetch(r0 + (i + 1) * step, next);
+        }
         const int n = in.n;
         const int64_t row = in.r * a.C;
         if constexpr (OWN) {
@@ -474,7 +484,7 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
                 store8p(a.dgate, a.param_dtype, in.r / p.rpg * a.C + c0, n, g);
             }
         }
-        in = next;
+        if constexpr (!LEAN) in = next;
     }
     // one partial row per block and sum: part[sum][block][C]
 #pragma unroll
