@@ -53,9 +53,9 @@ __global__ __launch_bounds__(256) void dropout_flat_kernel(int64_t total, uint32
     const int n = (int)std::min<int64_t>(8, total - 8 * q);
     float v[8];
     load8n(X + 8 * q, n, v);
-    const uint32_t m = keep_bits(draw_key(rng, call), (uint64_t)q, threshold);
+    const Keep8 m = keep_eight(draw_key(rng, call), (uint64_t)q, threshold);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (m >> i & 1) ? v[i] * scale : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = m.k[i] ? v[i] * scale : 0.f;
     store8n(Y + 8 * q, n, v);
 }
 
@@ -141,10 +141,15 @@ __device__ __forceinline__ void row_stats(const float (&v)[8], int n, int C, int
         mu = row_sum<W>(s, red, slot) / (float)C;
     }
     float q = 0.f;
+    if (n == 8 || rms) {   // columns past the row are 0
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float d = i < n ? v[i] - mu : 0.f;
-        q += d * d;
+        for (int i = 0; i < 8; ++i) q += (v[i] - mu) * (v[i] - mu);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float d = i < n ? v[i] - mu : 0.f;
+            q += d * d;
+        }
     }
     rs = 1.0f / sqrtf(row_sum<W>(q, red, slot) / (float)C + eps);
 }
@@ -156,11 +161,11 @@ struct Draws {
     float scale;
 };
 
-// the keep bits of a row's eight columns at 8 lane
-__device__ __forceinline__ uint32_t row_keep(const Draws& d, int64_t row, int lane) {
-    if (d.threshold == 0) return 0xFFu;
-    if (d.group) return keep_one(d.key, (uint64_t)(row / d.group), d.threshold) ? 0xFFu : 0u;
-    return keep_bits(d.key, (uint64_t)(row * d.Cq + lane), d.threshold);
+// whether a row's eight columns at 8 lane are kept
+__device__ __forceinline__ Keep8 row_keep(const Draws& d, int64_t row, int lane) {
+    if (d.threshold == 0) return keep_all(true);
+    if (d.group) return keep_all(keep_one(d.key, (uint64_t)(row / d.group), d.threshold));
+    return keep_eight(d.key, (uint64_t)(row * d.Cq + lane), d.threshold);
 }
 
 // Forward: one row per 16 / 64 lanes or per block; the draws are formed while the row is on its way.  16384 rows
@@ -181,7 +186,7 @@ __global__ __launch_bounds__(W ? 256 : 1024) void residual_norm_kernel(nbx_resid
     Raw8<TY> ry;
     fetch8n((const TX*)a.x + r * a.ldx + c0, n, rx);
     fetch8n((const TY*)a.y + r * a.ldy + c0, n, ry);
-    const uint32_t m = row_keep(d, r, lane);   // while the rows are on their way
+    const Keep8 m = row_keep(d, r, lane);   // while the rows are on their way
     float x[8], u[8], w[8], b[8];
     unpack8(rx, x);
     unpack8(ry, u);
@@ -204,7 +209,7 @@ __global__ __launch_bounds__(W ? 256 : 1024) void residual_norm_kernel(nbx_resid
     }
     const float s = a.scale * keep;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] += (m >> i & 1) ? s * u[i] : 0.f;
+    for (int i = 0; i < 8; ++i) x[i] = fmaf(s, m.k[i] ? u[i] : 0.f, x[i]);
     store8n((TX*)a.h + r * a.C + c0, n, x);
     if (a.pre_w) {
         // z is the norm of the sum before h is rounded to its type: one rounding per result
@@ -349,27 +354,28 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     if constexpr (AGAIN && NORM) pb[i] *= gt[i];
-                    gt[i] *= i < cn ? pw[i] : 0.f;
+                    gt[i] *= pw[i];
                 }
         }
     }
     using In = RowIn<TX, TY>;
     auto fetch = [&](int64_t r, In& in) {
-        in.n = r < r1 ? cn : 0;
-        in.r = r < r1 ? r : 0;
+        const bool live = r < r1;   // else zeros, its statistics too: nothing of another row reaches the sums
+        in.n = live ? cn : 0;
+        in.r = live ? r : 0;
         const int64_t row = in.r * a.C;
         fetch8n((const TX*)a.dh + row + (uint32_t)c0, a.dh ? in.n : 0, in.dh);
         if (pre) {
             fetch8n((const TY*)a.dz + row + (uint32_t)c0, in.n, in.dz);
             if constexpr (AGAIN) fetch8n((const TX*)a.x + in.r * a.ldx + (uint32_t)c0, in.n, in.h);
             else fetch8n((const TX*)a.h + row + (uint32_t)c0, in.n, in.h);
-            in.mu2 = a.stats[2 * a.rows + in.r];
-            in.rs2 = a.stats[3 * a.rows + in.r];
+            in.mu2 = live ? a.stats[2 * a.rows + in.r] : 0.f;
+            in.rs2 = live ? a.stats[3 * a.rows + in.r] : 0.f;
         }
         if (need_y) fetch8n((const TY*)a.y + in.r * a.ldy + (uint32_t)c0, in.n, in.y);
         if (post) {
-            in.mu1 = a.stats[in.r];
-            in.rs1 = a.stats[a.rows + in.r];
+            in.mu1 = live ? a.stats[in.r] : 0.f;
+            in.rs1 = live ? a.stats[a.rows + in.r] : 0.f;
         }
     };
     In in;
@@ -390,7 +396,7 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
             else if (left == 0) load8p(a.gate, a.param_dtype, in.r / p.rpg * a.C + c0, n, gt);
         }
         float t[8], v[8], e[8];
-        const uint32_t m = row_keep(d, in.r, lane);
+        const Keep8 m = row_keep(d, in.r, lane);
         unpack8(in.dh, t);
         if (pre) {
             unpack8(in.h, v);
@@ -406,7 +412,7 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
                     } else {
                         u[k] *= gt[k];
                     }
-                    v[k] += (m >> k & 1) && k < n ? s * u[k] : 0.f;
+                    v[k] = fmaf(s, m.k[k] ? u[k] : 0.f, v[k]);
                 }
             }
             unpack8(in.dz, e);
@@ -416,7 +422,7 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
                 v[k] = (v[k] - in.mu2) * in.rs2;
                 acc[SUM_PRE_W][k] += e[k] * v[k];  // past the row e is 0
                 acc[SUM_PRE_B][k] += e[k];
-                e[k] *= k < n ? qw[k] : 0.f;
+                e[k] *= qw[k];   // 0 past the row, as every weight below
                 s1 += e[k];
                 s2 += e[k] * v[k];
             }
@@ -428,7 +434,7 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
         }
         if (a.dx) store8n((TX*)a.dx + row + (uint32_t)c0, n, t);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) t[k] = (m >> k & 1) && k < n ? s * t[k] : 0.f;
+        for (int k = 0; k < 8; ++k) t[k] = m.k[k] ? s * t[k] : 0.f;
         if (need_y) {
             unpack8(in.y, v);
             if (post)
@@ -440,7 +446,7 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const float u = post ? v[k] * pw[k] + pb[k] : v[k];
-                    e[k] = (m >> k & 1) ? t[k] * u : 0.f;   // a dropped place counts 0 whatever it held
+                    e[k] = m.k[k] ? t[k] * u : 0.f;   // a dropped place counts 0 whatever it held
                     ag[k] += e[k];
                 }
                 if (rowgate) store8p(a.dgate, a.param_dtype, row + (uint32_t)c0, n, e);
@@ -451,7 +457,7 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
         if (post || (!OWN && a.dgate))
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                acc[SUM_A][k] += (m >> k & 1) ? t[k] * v[k] : 0.f;
+                acc[SUM_A][k] = fmaf(t[k], m.k[k] ? v[k] : 0.f, acc[SUM_A][k]);
                 acc[SUM_B][k] += t[k];
             }
         if constexpr (!OWN)
@@ -461,7 +467,7 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
             float s1 = 0.f, s2 = 0.f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                if constexpr (OWN) t[k] *= k < n ? pw[k] : 0.f;
+                if constexpr (OWN) t[k] *= pw[k];
                 s1 += t[k];
                 s2 += t[k] * v[k];
             }

@@ -44,6 +44,28 @@ __device__ __forceinline__ uint32_t keep_bits(const DrawKey& key, uint64_t q, ui
     return m;
 }
 
+// The same as eight truth values (lane masks in scalar registers: one select per use).
+struct Keep8 {
+    bool k[8];
+};
+__device__ __forceinline__ Keep8 keep_all(bool k) {
+    Keep8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.k[i] = k;
+    return r;
+}
+__device__ __forceinline__ Keep8 keep_eight(const DrawKey& key, uint64_t q, uint32_t threshold) {
+    const uint4 w = draw_block(key, q);
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    Keep8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r.k[2 * i] = (v[i] & 0xFFFFu) >= threshold;
+        r.k[2 * i + 1] = (v[i] >> 16) >= threshold;
+    }
+    return r;
+}
+
 __device__ __forceinline__ bool keep_one(const DrawKey& key, uint64_t draw, uint32_t threshold) {
     return keep_bits(key, draw >> 3, threshold) >> (draw & 7) & 1;
 }

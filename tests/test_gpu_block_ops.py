@@ -187,6 +187,20 @@ def test_residual_dropped_places_hold_anything(hip_device, rng):
     assert torch.equal(dg.cpu(), 2 * k.float().sum(0))
 
 
+@pytest.mark.parametrize("R,C,gates", [(50, 40, 5), (50, 40, 10), (21, 600, 3), (7, 2100, 7), (100, 300, 4)])
+def test_residual_bad_row_stays_in_its_group(hip_device, R, C, gates):
+    """A row of NaN reaches its own results and its gate group's gradient, no other's."""
+    r = _rand(2)
+    x, y = r(R, C), r(R, C)
+    y[0, 0] = math.nan
+    ins = [t.to(hip_device).requires_grad_() for t in (x, y, 1 + 0.1 * r(gates, C), 1 + 0.1 * r(C), 1 + 0.1 * r(C))]
+    h, z = B.residual_norm(ins[0], ins[1], gate=ins[2], post=(ins[3], None), pre=(ins[4], None), norm="layer")
+    dx, dy, dg = torch.autograd.grad((h, z), ins[:3], (torch.ones_like(h), r(R, C).to(hip_device)))
+    for t in (h, z, dx, dy):
+        assert torch.isnan(t[0]).any() and torch.isfinite(t[1:]).all()
+    assert torch.isnan(dg[0]).all() and torch.isfinite(dg[1:]).all()
+
+
 def test_residual_empty(hip_device):
     w = torch.ones(8, device=hip_device)
     h, z = B.residual_norm(torch.empty(0, 8, device=hip_device), torch.empty(0, 8, device=hip_device), pre=(w, None))
