@@ -169,7 +169,7 @@ __device__ __forceinline__ Keep8 row_keep(const Draws& d, int64_t row, int lane)
 }
 
 // Forward: one row per 16 / 64 lanes or per block; the draws are formed while the row is on its way.  16384 rows
-// of 2048 bf16 columns with both norms, gate and draws: 65 us, 268 MB at 4.1 TB/s (a copy: 4.8).  Several rows
+// of 2048 bf16 columns with both norms, gate and draws: 64 us, 268 MB at 4.2 TB/s (a copy: 4.8).  Several rows
 // per block with the next one prefetched take 70 us: twice the registers, half the waves.
 template <typename TX, typename TY, int W>
 __global__ __launch_bounds__(W ? 256 : 1024) void residual_norm_kernel(nbx_residual_norm_args a, float keep) {
@@ -272,7 +272,7 @@ enum { SUM_A, SUM_B, SUM_PRE_W, SUM_PRE_B, SUMS };
 
 // The backward pass reads y, h, dh and dz once; statistics come from the forward pass.  A 16-bit h has lost what
 // xhat needs (the weight gradients would be off by its rounding again), so there x is read in its place and h
-// is formed again from x and y.  The same 16384 x 2048 bf16 block: 100 us, 403 MB at 4.0 TB/s, and 11 us for the sums.
+// is formed again from x and y.  The same 16384 x 2048 bf16 block: 96 us, 403 MB at 4.2 TB/s, and 9.5 us for the sums.
 template <typename TX, typename TY>
 struct RowIn {   // a row's eight columns as loaded, one row ahead of their use
     Raw8<TX> dh, h;   // h: x where h is formed again
@@ -518,7 +518,7 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
 // Column sums of the partial rows.  The first jobs * ceil(C / 32) blocks: a parameter over all blocks (dpost_*
 // with each block's gate row put back), 32 columns x 32 slots, each slot every 32nd row, combined in order.
 // Then gate group after group over its cpg blocks: the same, or (cpg <= 16) a thread per column: 64 groups of
-// 12 partial rows of 2048 columns take 14.2 us so, 16.9 with slots.
+// 12 partial rows of 2048 columns, with two parameters: 15.6 us so, 18.3 with slots.
 enum { OUT_POST_W, OUT_POST_B, OUT_PRE_W, OUT_PRE_B, OUTS };
 struct FinalSums {
     void* out[OUTS];
@@ -622,7 +622,7 @@ int with_types(const nbx_residual_norm_args& a, F&& f) {
 // be shorter), kept in the registers of TPN threads: 64 (four nodes per block) or the block; thread t holds
 // chunks t, t + TPN, .. (NJ of them).  The l = 0 row is chunks 0 .. C/8 - 1, all in the first wave, so its
 // centring needs no barrier: one block-wide sum per direction is left.  2560 nodes of lmax 6, 128 channels, fp32:
-// forward 59 us (257 MB at 4.3 TB/s), backward 71 us (321 MB at 4.5 TB/s) and 4 us for the sums.
+// forward 60 us (257 MB at 4.3 TB/s), backward 67 us (321 MB at 4.8 TB/s) and 4 us for the sums.
 constexpr int SH_MAXC = 512;
 constexpr int SH_LDS_HEAD = 64 + 2 * 4 * SH_MAXC / 8 / 4;   // floats before the rows in the backward pass's LDS
 
