@@ -114,7 +114,7 @@ __device__ __forceinline__ void nodes_of_positions(const int32_t* __restrict__ p
         if (lane >= m) v = std::max(v, left);
     }
     const int64_t p = p0 + lane;
-    sV[lane] = lane < cnt && p >= ptr[v] && p < ptr[v + 1] ? v : -1;
+    sV[lane] = V > 0 && lane < cnt && p >= ptr[v] && p < ptr[v + 1] ? v : -1;   // V = 0: ptr has one entry
 }
 
 // The lists that have positions in a block: sP[j] = first position of the j-th, sP[lists] = cnt; returns how
@@ -777,8 +777,8 @@ extern "C" int nbx_segment_attention(const nbx_segment_attention_args* a, void* 
 
 extern "C" int nbx_segment_attention_backward(const nbx_segment_attention_args* a, void* stream) {
     if (int rc = sa_check(a, "nbx_segment_attention_backward")) return rc;
-    if (a->V == 0 || a->E == 0 || (!a->dvalues && !a->dlogits)) return NBX_OK;
-    NBX_CHECK_ARG(a->ptr && a->eid && a->values && a->logits && a->stats && a->dout,
+    if (a->E == 0 || (!a->dvalues && !a->dlogits)) return NBX_OK;   // without a node the gradients are 0
+    NBX_CHECK_ARG(a->ptr && a->eid && a->values && a->logits && (a->V == 0 || (a->stats && a->dout)),
                   "nbx_segment_attention_backward: null operand");
     const size_t need = workspace_need(*a, true);
     if (need && !(a->workspace && a->workspace_bytes >= need)) {

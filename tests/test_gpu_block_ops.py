@@ -436,6 +436,19 @@ def test_attention_empty(hip_device):
     assert out.shape == (0, 2, 2, 4)
 
 
+@pytest.mark.parametrize("E", [1, 300])
+def test_attention_without_nodes(hip_device, rng, E):
+    """No node at all: every edge is in no list, its gradients are 0."""
+    values = torch.ones(E, 2, 2, 4, device=hip_device, requires_grad=True)
+    logits = torch.ones(E, 2, device=hip_device, requires_grad=True)
+    eid = torch.arange(E, dtype=torch.int32, device=hip_device)
+    del_me = [torch.full((E, 2, 2, 4), 7.0, device=hip_device), torch.full((E, 2), 7.0, device=hip_device)]
+    del del_me   # what the gradients' memory may hold beforehand
+    out = B.segment_attention(values, logits, torch.zeros(1, dtype=torch.int32, device=hip_device), eid, p=0.3, rng=rng, call=1)
+    dv, dl = torch.autograd.grad(out, (values, logits), torch.empty_like(out))
+    assert out.shape == (0, 2, 2, 4) and not dv.any() and not dl.any()
+
+
 # ------------------------------------------------------------------------------------------------ across the operators
 def _block(x, params, ptr, eid, rng, step_calls=True):
     """A block as the framework's training paths use the operators: attention over edges, gated residual with
