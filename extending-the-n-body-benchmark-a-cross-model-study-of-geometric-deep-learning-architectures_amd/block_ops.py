@@ -134,6 +134,16 @@ def dropout(x, p, rng=None, *, call=None, per="element", group=1):
 
 
 # ---------------------------------------------------------------------------------------------- residual + norms
+def _consecutive(gate, y):
+    """Whether a gate row belongs to consecutive rows of y: one or two axes, or y's axes from the front, then ones."""
+    if gate.dim() <= 2:
+        return True
+    same = 0
+    while same < gate.dim() - 1 and gate.shape[:same + 1] == y.shape[:same + 1]:
+        same += 1
+    return gate.dim() == y.dim() and all(s == 1 for s in gate.shape[same:-1])
+
+
 def residual_norm(x, y, *, gate=None, scale=1.0, post=None, pre=None, norm="rms", eps=1e-5, p=0.0, group=0, rng=None,
                   call=None):
     """The residual stream after a block: ``h = x + scale * dropout(gate * u)`` with ``u = y`` or, with ``post``
@@ -142,7 +152,8 @@ def residual_norm(x, y, *, gate=None, scale=1.0, post=None, pre=None, norm="rms"
 
     x (the stream) and y (the block's output) [..., C] of one shape, C <= 8192; y of x's type, or of 16 bits
     under a float32 stream.  norm = "rms" or "layer" (biased variance), for both places.  gate: [C] (layer
-    scale), [G, C] (one row for each rows / G consecutive rows) or y's shape.  gate and the norms' parameters
+    scale), [G, C] (one row for each rows / G consecutive rows, whatever y's axes are), y's shape, or y's leading axes
+    followed by ones ([B, 1, C] for y [B, N, C]).  gate and the norms' parameters
     are all float32 or all of y's type; their gradients are column sums in float32, rounded once.  p: drop rate
     of every element, or with group > 0 of whole groups of that many consecutive rows."""
     if norm not in _NORM:
@@ -169,8 +180,9 @@ def residual_norm(x, y, *, gate=None, scale=1.0, post=None, pre=None, norm="rms"
         if t is not None and t.shape != (C,):
             raise ValueError(f"a norm's parameters must be [{C}], got {list(t.shape)}")
     if gate is not None and (gate.dim() < 1 or gate.shape[-1] != C or (rows and gate.numel() == 0)
-                             or rows % max(gate.numel() // C, 1)):
-        raise ValueError(f"gate {list(gate.shape)} must be [C], [G, C] with G dividing the {rows} rows, or y's shape")
+                             or rows % max(gate.numel() // C, 1) or not _consecutive(gate, y)):
+        raise ValueError(f"gate {list(gate.shape)} must be [C], [G, C] with G dividing the {rows} rows, y's leading axes "
+                         f"followed by ones, or y's shape {list(y.shape)}")
     if int(group) < 0:
         raise ValueError(f"group must be at least 0, got {group}")
     dev = _device(x, y, *params)

@@ -134,6 +134,16 @@ def test_residual_refusals(kw, err):
         B.residual_norm(kw.pop("x"), kw.pop("y"), **kw)
 
 
+@pytest.mark.parametrize("shape,ok", [
+    ((6,), True), ((2, 6), True), ((10, 6), True), ((2, 5, 6), True), ((2, 1, 6), True), ((1, 1, 6), True),
+    ((1, 5, 6), False), ((1, 2, 6), False), ((5, 2, 6), False), ((1, 2, 1, 6), False)])
+def test_residual_gate_shapes(shape, ok):
+    """A gate whose rows broadcasting would repeat is refused: its rows are for consecutive rows of y.  What is
+    allowed gets as far as the device check."""
+    with pytest.raises(lib.NbxError if ok else ValueError, match="HIP device" if ok else "gate"):
+        B.residual_norm(_t(2, 5, 6), _t(2, 5, 6), gate=_t(*shape))
+
+
 @pytest.mark.parametrize("kw,err", [
     (dict(x=_t(3, 5, 8), y=_t(3, 5, 8)), ValueError), (dict(x=_t(3, 64, 8), y=_t(3, 64, 8)), ValueError),
     (dict(x=_t(3, 4, 513), y=_t(3, 4, 513)), ValueError), (dict(x=_t(3, 32), y=_t(3, 32)), ValueError),
