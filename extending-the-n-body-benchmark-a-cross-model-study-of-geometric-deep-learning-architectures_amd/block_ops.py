@@ -102,6 +102,14 @@ def _device(*tensors):
     return dev
 
 
+def _with_parameters(t, *params):
+    """An empty tensor with the parameters (None entries are skipped) in its graph."""
+    for p in params:
+        if p is not None:
+            t = t + p.flatten()[:1].sum().to(t.dtype)
+    return t
+
+
 def _dtype(t, what):
     code = _CODE.get(t.dtype)
     if code is None:
@@ -189,8 +197,9 @@ def residual_norm(x, y, *, gate=None, scale=1.0, post=None, pre=None, norm="rms"
     state = None
     if threshold:
         state, call = _draws(rng, call, 1, dev)
-    if rows == 0:
-        return x + y, (y * pre_w.to(y.dtype) if pre_w is not None else None)
+    if rows == 0:   # empty results that know their parameters: gradients of 0
+        h = x + _with_parameters(y, gate, post_w, post_b)
+        return h, (_with_parameters(h.to(y.dtype), pre_w, pre_b) if pre_w is not None else None)
     return _lib.torch_ops().residual_norm(x, y, gate, post_w, post_b, pre_w, pre_b, state, cx, cy, cp, _NORM[norm], eps,
                                           scale, threshold, int(group), call or 0)
 
@@ -224,7 +233,8 @@ def sh_residual_norm(x, y, weight, bias, *, eps=1e-5, path_p=0.0, path_group=1, 
     if t1 or t2:
         state, call = _draws(rng, call, 2, dev)
     if V == 0:
-        return x + y, y * bias.to(y.dtype)
+        h = x + y
+        return h, _with_parameters(h, weight, bias)
     return _lib.torch_ops().sh_residual_norm(x, y, weight, bias, state, lmax, code, cp, eps, t1, int(path_group), t2,
                                              call or 0)
 

@@ -205,6 +205,12 @@ def test_residual_empty(hip_device):
     w = torch.ones(8, device=hip_device)
     h, z = B.residual_norm(torch.empty(0, 8, device=hip_device), torch.empty(0, 8, device=hip_device), pre=(w, None))
     assert h.shape == z.shape == (0, 8)
+    ins = [torch.zeros(s, device=hip_device, dtype=d, requires_grad=True)
+           for s, d in (((0, 8), F32), ((0, 8), BF16), ((3, 8), F32), *[((8,), F32)] * 4)]
+    h, z = B.residual_norm(ins[0], ins[1], gate=ins[2], post=(ins[3], ins[4]), pre=(ins[5], ins[6]))
+    assert h.dtype == F32 and z.dtype == BF16
+    for g, t in zip(torch.autograd.grad((h, z), ins, (torch.empty_like(h), torch.empty_like(z))), ins):
+        assert g.shape == t.shape and not g.any()
 
 
 def test_residual_far_rows(hip_device):
@@ -289,6 +295,10 @@ def test_sh_partial_gradients_and_empty(hip_device):
     assert _bits(torch.autograd.grad(B.sh_residual_norm(*ins)[0], ins[0], dh)[0], dh)
     h, z = B.sh_residual_norm(torch.empty(0, 4, 9, device=hip_device), torch.empty(0, 4, 9, device=hip_device), w, b)
     assert h.shape == z.shape == (0, 4, 9)
+    ins = [torch.zeros(s, device=hip_device, requires_grad=True) for s in ((0, 4, 9), (0, 4, 9), (2, 9), (9,))]
+    h, z = B.sh_residual_norm(*ins)
+    for g, t in zip(torch.autograd.grad((h, z), ins, (torch.empty_like(h), torch.empty_like(z))), ins):
+        assert g.shape == t.shape and not g.any()
 
 
 # ------------------------------------------------------------------------------------------------ segment attention
