@@ -42,7 +42,12 @@ class CounterRNG:
         self._next = 0
 
     def take(self, calls=1):
-        """The number of the step's next call (of ``calls`` consecutive ones)."""
+        """The number of the step's next call (of ``calls`` consecutive ones).  Refused inside a backward pass:
+        a forward that is run again there (activation checkpointing) has to draw as it did, so give its operators
+        ``call`` explicitly and advance after the backward pass."""
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("the next call's number was asked for inside a backward pass: a recomputed forward "
+                               "needs an explicit call")
         c = self._next
         self._next += calls
         return c

@@ -743,6 +743,7 @@ extern "C" int nbx_segment_attention(const nbx_segment_attention_args* a, void* 
         return NBX_E_WORKSPACE;
     }
     const SaPlan p = forward_plan(*a);
+    NBX_CHECK_ARG(!p.chunked || p.nc * p.T < ((int64_t)1 << 32), "nbx_segment_attention: too many edges");
     hipStream_t st = (hipStream_t)stream;
     const float keep = keep_scale(a->threshold);
     return with_values(*a, [&](auto t, auto vw) -> int {

@@ -7,6 +7,7 @@ import subprocess
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import nbody_amd._lib as lib
 import nbody_amd.block_ops as B
@@ -274,3 +275,18 @@ def test_struct_layouts(tmp_path, name, mirror):
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [ctypes.sizeof(mirror)] + [getattr(mirror, f).offset for f in fields]
+
+
+def test_next_call_is_refused_in_a_backward_pass():
+    """A forward that runs again in the backward pass (activation checkpointing) must not draw anew."""
+    rng = B.CounterRNG(0, "cpu")
+    taken = []
+
+    def body(x):
+        taken.append(rng.take())
+        return x * x
+    x = torch.ones(3, requires_grad=True)
+    y = torch.utils.checkpoint.checkpoint(body, x, use_reentrant=False)
+    with pytest.raises(RuntimeError, match="explicit call"):
+        y.sum().backward()
+    assert taken == [0] and rng.take() == 1

@@ -6,6 +6,7 @@ import math
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import nbody_amd.block_ops as B
 from oracle import block_ops as O
@@ -528,6 +529,21 @@ def test_backward_draws_what_the_forward_drew(hip_device):
     rng.advance()
     (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
     assert torch.equal(dx, y.detach())
+
+
+def test_recomputed_forward_draws_the_same(hip_device):
+    """Activation checkpointing with explicit call numbers."""
+    rng = B.CounterRNG(1, hip_device)
+    r = _rand(3)
+    x, w = (r(*s).to(hip_device).requires_grad_() for s in ((70, 33), (33,)))
+
+    def body(x, w):
+        y = B.dropout(x * x, 0.3, rng, call=4)
+        return B.residual_norm(x, y, pre=(w, None), p=0.2, rng=rng, call=5)
+    g = r(70, 33).to(hip_device)
+    plain = torch.autograd.grad(body(x, w), (x, w), (g, g))
+    again = torch.autograd.grad(torch.utils.checkpoint.checkpoint(body, x, w, use_reentrant=False), (x, w), (g, g))
+    assert _bits(plain[0], again[0]) and _bits(plain[1], again[1])
 
 
 def test_graph_capture_replays_new_draws(hip_device):
