@@ -1,4 +1,5 @@
-"""The block operators' larger forms on the device: attention in chunks (lists that cross blocks).  Each test first asserts that its
+"""The block operators' larger forms on the device: attention in chunks (lists that cross blocks), residual rows
+dealt to a block in turn, wide rows, many nodes of spherical-harmonics features.  Each test first asserts that its
 sizes take the form it is about, so that a changed rule cannot leave the form untested.  Tolerances as in
 test_gpu_block_ops.py: the oracle's running error bounds."""
 import ctypes
@@ -10,8 +11,8 @@ import torch
 import nbody_amd._lib as lib
 import nbody_amd.block_ops as B
 from oracle import block_ops as O
-from test_gpu_block_ops import (BF16, F16, F32, CALL, SEED, STEP, _attention_case, _lists, _rand,
-                                rng)  # noqa: F401  (rng: a fixture)
+from test_gpu_block_ops import (BF16, F16, F32, CALL, SEED, STEP, _attention_case, _lists, _rand, _residual_case,
+                                _sh_case, rng)  # noqa: F401  (rng: a fixture)
 
 import numpy as np
 
@@ -148,3 +149,110 @@ def test_chunk_form_entries_out_of_range(hip_device):
     rest[gone] = False
     for t, n in ((dv, "dvalues"), (dl, "dlogits")):
         O.within(t[rest.to(hip_device)], O.B(ref[n].val[rest], ref[n].err[rest]), n)
+
+
+# ------------------------------------------------------------------------------------------------ rows in turn
+def _rows_in_turn(R, C, gates, slots):
+    """Whether a row slot of the backward pass has several rows, from its partial rows (four per block)."""
+    a = lib.ResidualNormArgs(rows=R, C=C, ldx=C, ldy=C, gate=8 if gates else None, gate_groups=gates)
+    n = lib.c_sz()
+    lib.check(lib.lib().nbx_residual_norm_backward_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "workspace")
+    return R > n.value // (16 * C) * slots
+
+
+SIXTEEN, MIXED, ALL32 = (BF16, BF16, BF16), (F32, F16, F32), (F32, F32, F32)
+
+
+# slots: row slots of a block (16 lanes a row up to 128 columns, a wave up to 512, then whole waves).  Gates: one
+# for all rows, groups longer and shorter than a block's share (several whole groups a slot among them), a gate a row
+@pytest.mark.parametrize("R,C,gates,slots", [
+    (13001, 24, 1, 16), (13001, 24, 13001, 16), (13000, 24, 2, 16), (52000, 24, 26000, 16),
+    (3500, 200, 1, 4), (3500, 200, 3500, 4), (3500, 200, 5, 4), (16000, 136, 8000, 4),
+    (4001, 520, 0, 2), (4000, 520, 4, 2), (4000, 520, 1000, 2), (6400, 520, 3200, 2),
+    (1700, 1100, 1, 1), (1700, 1100, 850, 1), (1700, 1100, 1700, 1), (3400, 1100, 1700, 1)])
+@pytest.mark.parametrize("types", [ALL32, SIXTEEN, MIXED], ids=["f32", "bf16", "f16_in_f32"])
+def test_residual_rows_in_turn(hip_device, rng, R, C, gates, slots, types):   # noqa: F811
+    assert _rows_in_turn(R, C, gates, slots)
+    _residual_case(hip_device, rng, R, C, "layer" if C % 8 else "rms", *types, gates, True, True, True, 0.1, 0)
+
+
+@pytest.mark.parametrize("R,C,gates", [(600, 2100, 1), (600, 2100, 2), (600, 2100, 300), (600, 2100, 600), (520, 4096, 1),
+                                       (600, 4200, 1), (600, 4200, 2), (600, 4200, 300), (600, 4200, 600), (300, 8191, 0),
+                                       (300, 8192, 1)])
+@pytest.mark.parametrize("types", [ALL32, SIXTEEN, MIXED], ids=["f32", "bf16", "f16_in_f32"])
+def test_residual_wide_rows_in_turn(hip_device, rng, R, C, gates, types):     # noqa: F811
+    """Rows of eight and of sixteen waves, several to a block."""
+    assert _rows_in_turn(R, C, gates, 1)
+    _residual_case(hip_device, rng, R, C, "layer", *types, gates, True, True, True, 0.1, 7 if C % 8 else 0)
+
+
+@pytest.mark.parametrize("post,pre", [(False, True), (True, False), (False, False)])
+@pytest.mark.parametrize("R,C,gates", [(3500, 200, 5), (1700, 1100, 850), (600, 2100, 600), (600, 4200, 2)])
+def test_residual_rows_in_turn_parts(hip_device, rng, R, C, gates, post, pre):   # noqa: F811
+    _residual_case(hip_device, rng, R, C, "rms", *SIXTEEN, gates, post, pre, False, 0.2, 0)
+
+
+@pytest.mark.parametrize("R,C,gates,slots", [
+    (13001, 32, 1, 16), (13000, 32, 26, 16), (13001, 32, 13001, 16), (52000, 32, 26000, 16), (3500, 256, 5, 4),
+    (16000, 256, 8000, 4), (4000, 1024, 4, 2), (4000, 1024, 1000, 2), (600, 2048, 1, 0), (1700, 2048, 850, 1),
+    (600, 4096, 2, 1), (600, 4096, 300, 1), (600, 8192, 2, 1), (600, 8192, 300, 1), (600, 8192, 600, 1)])
+@pytest.mark.parametrize("xt,yt", [(F32, F32), (BF16, BF16), (F32, F16)])
+def test_residual_sums_over_rows_are_exact(hip_device, R, C, gates, slots, xt, yt):
+    """Inputs whose every intermediate is a multiple of 2^-2 / C: the normed rows are +-1 (RMS norm of +-1 and of
+    +-2 gate, eps 0), gates 1 and 2, gradients -1, 0, 1.  Sums over the rows are below 2^10, so that float32
+    holds them exactly in any order, and a row that is lost, doubled or in another group shows."""
+    assert not slots or _rows_in_turn(R, C, gates, slots)
+    g = torch.Generator().manual_seed(R + C)
+    sign = lambda *s: 2.0 * torch.randint(0, 2, s, generator=g) - 1                              # noqa: E731
+    unit = lambda *s: torch.randint(-1, 2, s, generator=g).float()                               # noqa: E731
+    x, y, one = torch.zeros(R, C, dtype=xt), sign(R, C).to(yt), torch.ones(C)
+    gate = (1.0 + torch.arange(gates) % 2)[:, None].expand(gates, C).contiguous()
+    dh, dz = unit(R, C).to(xt), unit(R, C).to(yt)
+    ref = O.residual_norm(x, y, gate, (one, one * 0), (one, one * 0), "rms", 0.0, 2.0, torch.ones(R, C, dtype=torch.bool),
+                          0.0, dh, dz)
+    ins = [t.to(hip_device).requires_grad_() for t in (gate, one, one * 0, one, one * 0)]
+    h, z = B.residual_norm(x.to(hip_device), y.to(hip_device), gate=ins[0], scale=2.0, post=(ins[1], ins[2]),
+                           pre=(ins[3], ins[4]), eps=0.0)
+    got = torch.autograd.grad((h, z), ins, (dh.to(hip_device), dz.to(hip_device)))
+    for n, t in zip(("dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b"), got):
+        assert torch.equal(t.double().cpu(), ref[n].val), n
+
+
+# ------------------------------------------------------------------------------------------------ many nodes
+@pytest.mark.parametrize("V,lmax,C", [(2501, 2, 64), (2050, 1, 9), (4099, 0, 40), (2049, 3, 61)])
+@pytest.mark.parametrize("dtype,pt", [(F32, F32), (BF16, BF16), (F16, F32)])
+def test_sh_waves_per_node(hip_device, rng, V, lmax, C, dtype, pt):           # noqa: F811
+    """A wave per node (one or two chunks a lane), nodes that are no multiple of a block's four, several a wave."""
+    assert V >= 2048 and V % 4 and (lmax + 1) ** 2 * -(-C // 8) <= 128
+    _sh_case(hip_device, rng, V, lmax, C, dtype, pt, 0.2, 5, 0.1)
+
+
+@pytest.mark.parametrize("V,lmax,C", [(700, 3, 80), (1100, 2, 250)])
+@pytest.mark.parametrize("dtype,pt", [(BF16, F32), (F16, F16)])
+def test_sh_nodes_in_turn(hip_device, rng, V, lmax, C, dtype, pt):            # noqa: F811
+    """A block per node, several nodes in turn, in 16 bits."""
+    assert V > 512 and (lmax + 1) ** 2 * -(-C // 8) > 128
+    _sh_case(hip_device, rng, V, lmax, C, dtype, pt, 0.2, 5, 0.1)
+
+
+@pytest.mark.parametrize("V,lmax,C", [(2501, 2, 64), (4099, 0, 40), (2049, 3, 16), (700, 3, 80), (1100, 6, 128)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sh_sums_over_nodes(hip_device, V, lmax, C, dtype):
+    """Normed features of +-1 (up to the rounding of the degrees' balance: 32 half steps at most) and gradients of -1,
+    0, 1: the bias gradient is exact and a lost or doubled node is 1 in the weight's."""
+    g = torch.Generator().manual_seed(V)
+    S = (lmax + 1) ** 2
+    y = 2.0 * torch.randint(0, 2, (V, S, C), generator=g) - 1
+    half = 2.0 * (torch.arange(C) % 2) - 1                       # the l = 0 row has no mean
+    y[:, 0] = torch.stack([half[torch.randperm(C, generator=g)] for _ in range(V)])
+    dz = torch.randint(-1, 2, (V, S, C), generator=g).float()
+    w, b = (t.to(hip_device).requires_grad_() for t in (torch.ones(lmax + 1, C), torch.zeros(C)))
+    x, y, dz = (t.to(dtype) for t in (torch.zeros(V, S, C), y, dz))
+    _, z = B.sh_residual_norm(x.to(hip_device), y.to(hip_device), w, b, eps=0.0)
+    dw, db = torch.autograd.grad(z, (w, b), dz.to(hip_device))
+    assert torch.equal(db.cpu(), dz[:, 0].float().sum(0))
+    deg = torch.tensor([l for l in range(lmax + 1) for _ in range(2 * l + 1)])
+    want = torch.zeros(lmax + 1, C, dtype=torch.float64).index_add_(0, deg, (dz.double() * y.double()).sum(0))
+    # 32 half steps of each term, and one per addition (fewer than 128 deep: nodes in turn, slots, degree)
+    off = (dw.double().cpu() - want).abs()
+    assert float(off.max()) <= 160 * 2.0 ** -24 * V * (2 * lmax + 1) < 0.2, float(off.max())
