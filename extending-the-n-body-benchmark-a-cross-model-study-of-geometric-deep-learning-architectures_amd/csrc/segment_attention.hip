@@ -6,7 +6,8 @@
 //   * chunk form, for long lists: a block per 64 positions of the CSR, whatever nodes they belong to; a list
 //     that crosses a chunk's border leaves partial sums with their own maximum, joined by a second launch.
 // Backward: a block per few positions forms dvalues, the weights' gradient and, for lists that lie within
-// the block, the softmax's own gradient; a second launch finishes the lists that cross blocks.
+// the block, the softmax's own gradient; a second launch finishes the lists that cross blocks and the edges that
+// no list entry names.
 #include <algorithm>
 #include <type_traits>
 
@@ -477,7 +478,8 @@ __global__ __launch_bounds__(256) void segment_attention_join_kernel(nbx_segment
 template <typename T, int VW>
 __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment_attention_args a, SaPlan p, float keep,
                                                                      float* __restrict__ wa, float* __restrict__ wd,
-                                                                     float* __restrict__ share, int2* __restrict__ ends) {
+                                                                     float* __restrict__ share, int2* __restrict__ ends,
+                                                                     int32_t* __restrict__ named) {
     extern __shared__ float lds[];
     const int H = a.H, t = threadIdx.x;
     float* sA = lds;                       // [eb][H] alpha
@@ -498,6 +500,7 @@ __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment
     } else if (t < 64 + cnt) {
         const int e = a.eid[p0 + t - 64];
         sE[t - 64] = e >= 0 && e < a.E ? e : -1;
+        if (e >= 0 && e < a.E) named[e] = (int32_t)(p0 + t - 64);
     }
     __syncthreads();
     for (int i = t; i < cnt * H; i += p.T) {
@@ -591,17 +594,40 @@ __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment
     }
 }
 
-// finishes the lists that cross the block's borders: at most one that began before it and one that goes on
-__global__ __launch_bounds__(256) void segment_attention_dlogits_kernel(nbx_segment_attention_args a, SaPlan p,
-                                                                        const float* __restrict__ wa,
-                                                                        const float* __restrict__ wd,
-                                                                        const float* __restrict__ share,
-                                                                        const int2* __restrict__ ends) {
+// Finishes the lists that cross the block's borders: at most one that began before it and one that goes on.  And
+// the edges [p0, p0 + cnt) that no entry of eid names get gradients of 0: edge e is named iff eid[named[e]] = e,
+// whatever named[e] held before, so `named` needs no clearing.
+__global__ __launch_bounds__(256) void segment_attention_finish_kernel(nbx_segment_attention_args a, SaPlan p,
+                                                                       const float* __restrict__ wa,
+                                                                       const float* __restrict__ wd,
+                                                                       const float* __restrict__ share,
+                                                                       const int2* __restrict__ ends,
+                                                                       const int32_t* __restrict__ named) {
     __shared__ float red[256];
+    __shared__ uint64_t sMissing;
     const int t = threadIdx.x, H = a.H;
     const int64_t p0 = blockIdx.x * (int64_t)p.eb;
     const int cnt = (int)std::min<int64_t>(p.eb, a.E - p0);
-    const int2 ends_here = ends[blockIdx.x];   // the nodes of the block's first and last position
+    int2 ends_here = make_int2(-1, -1);   // the nodes of the block's first and last position
+    if (a.dlogits) ends_here = ends[blockIdx.x];
+    if (t < 64) {
+        bool missing = false;
+        if (t < cnt) {
+            const int32_t at = named[p0 + t];
+            missing = at < 0 || at >= a.E || a.eid[at] != p0 + t;
+        }
+        const uint64_t m = __ballot(missing);
+        if (t == 0) sMissing = m;
+    }
+    __syncthreads();
+    const int64_t halves = (int64_t)a.K * H * a.D * (a.v_dtype == NBX_F32 ? 2 : 1);   // 16-bit units of a row
+    for (uint64_t m = sMissing; m; m &= m - 1) {
+        const int64_t e = p0 + __ffsll((unsigned long long)m) - 1;
+        if (a.dvalues)
+            for (int64_t i = t; i < halves; i += 256) ((uint16_t*)a.dvalues)[e * halves + i] = 0;
+        if (a.dlogits && t < H) store_dlogit(a, e * H + t, 0.f);
+    }
+    if (!a.dlogits) return;
     const int hs = 256 / H, h = t % H, r = t / H;
     for (int side = 0; side < 2; ++side) {
         const int v = side ? ends_here.y : ends_here.x;
@@ -716,7 +742,10 @@ int with_values(const nbx_segment_attention_args& a, F&& f) {
 }
 
 size_t workspace_need(const nbx_segment_attention_args& a, bool backward) {
-    if (backward) return a.dlogits ? (size_t)2 * ((a.E + backward_plan(a).nc) * a.H + backward_plan(a).nc) * sizeof(float) : 0;
+    if (backward) {
+        const int64_t nc = backward_plan(a).nc;
+        return (size_t)((a.dlogits ? 2 * ((a.E + nc) * a.H + nc) : 0) + a.E) * sizeof(float);
+    }
     const SaPlan p = forward_plan(a);
     return p.chunked ? (size_t)2 * p.nc * (a.K * a.H * a.D + 2 * a.H) * sizeof(float) : 0;
 }
@@ -790,24 +819,23 @@ extern "C" int nbx_segment_attention_backward(const nbx_segment_attention_args* 
     NBX_CHECK_ARG(p.nc * p.T < ((int64_t)1 << 32), "nbx_segment_attention_backward: too many edges");
     hipStream_t st = (hipStream_t)stream;
     const float keep = keep_scale(a->threshold);
-    int2* ends = (int2*)a->workspace;
+    int2* ends = (int2*)a->workspace;   // ends, wa, wd and share only for dlogits
     float* wa = (float*)(ends + p.nc);
     float* wd = wa + a->E * a->H;
     float* share = wd + a->E * a->H;
+    int32_t* named = a->dlogits ? (int32_t*)(share + 2 * p.nc * a->H) : (int32_t*)a->workspace;
     if (int rc = with_values(*a, [&](auto t, auto vw) -> int {
             using T = decltype(t);
             constexpr int VW = decltype(vw)::value;
             const size_t lds = (size_t)(3 * p.eb * a->H + p.eb * p.entries + 196) * 4;
             hipLaunchKernelGGL((segment_attention_bwd_kernel<T, VW>), dim3((unsigned)p.nc), dim3(p.T), lds, st, *a, p, keep,
-                               wa, wd, share, ends);
+                               wa, wd, share, ends, named);
             NBX_LAUNCH_CHECK("segment_attention_bwd");
             return NBX_OK;
         }))
         return rc;
-    if (a->dlogits) {
-        hipLaunchKernelGGL(segment_attention_dlogits_kernel, dim3((unsigned)p.nc), dim3(256), 0, st, *a, p, wa, wd,
-                           share, ends);
-        NBX_LAUNCH_CHECK("segment_attention_dlogits");
-    }
+    hipLaunchKernelGGL(segment_attention_finish_kernel, dim3((unsigned)p.nc), dim3(256), 0, st, *a, p, wa, wd, share, ends,
+                       named);
+    NBX_LAUNCH_CHECK("segment_attention_finish");
     return NBX_OK;
 }

@@ -1016,8 +1016,8 @@ int nbx_sh_residual_norm_backward(const nbx_sh_residual_norm_args* a, void* stre
  * out[v][k][h][:] = sum over the list of w[e][h] values[e][k][h][:].  An empty list, or one whose logits are
  * all -inf, gives 0.  A weight that is exactly 0 (masked, dropped, underflown) reads nothing of its value.
  * Backward: dvalues, dlogits (NULL: not wanted); eid is a permutation of the edges, and those in no list
- * (positions from ptr[V] on) get gradients of 0.  An entry of eid outside [0, E) counts as masked (the edge that
- * is missing then gets no gradient), and lists end at E.
+ * (positions from ptr[V] on) get gradients of 0.  An entry of eid outside [0, E) counts as masked, an edge that no
+ * entry names gets gradients of 0 too, and lists end at E.
  * values / out in v_dtype, logits in l_dtype (fp32 or v_dtype); H <= 64, H D <= 4096 (1024 if D is no
  * multiple of 4), K H D < 2^20; stats fp32 [2][V][H] = (max, 1 / sum).  All contiguous.  workspace: forward and backward
  * ask their own size. */
