@@ -666,7 +666,8 @@ int vector_width(const nbx_segment_attention_args& a) {
 int sa_check(const nbx_segment_attention_args* a, const char* who) {
     NBX_CHECK_ARG(a, "%s: null arguments", who);
     const int64_t lim = (int64_t)1 << 31;
-    NBX_CHECK_ARG(a->V >= 0 && a->V < lim - 1 && a->E >= 0 && a->E < lim - TILE && a->K >= 1 && a->H >= 1 && a->D >= 1,
+    // a list is walked in steps of up to 4 TILE positions held in 32 bits: the step past the last has to fit
+    NBX_CHECK_ARG(a->V >= 0 && a->V < lim - 1 && a->E >= 0 && a->E < lim - 4 * TILE && a->K >= 1 && a->H >= 1 && a->D >= 1,
                   "%s: bad sizes", who);
     NBX_CHECK_ARG(dtype_ok(a->v_dtype) && (a->l_dtype == a->v_dtype || a->l_dtype == NBX_F32),
                   "%s: l_dtype must be fp32 or v_dtype", who);

@@ -1019,7 +1019,7 @@ int nbx_sh_residual_norm_backward(const nbx_sh_residual_norm_args* a, void* stre
  * (positions from ptr[V] on) get gradients of 0.  An entry of eid outside [0, E) counts as masked, an edge that no
  * entry names gets gradients of 0 too, and lists end at E.
  * values / out in v_dtype, logits in l_dtype (fp32 or v_dtype); H <= 64, H D <= 4096 (1024 if D is no
- * multiple of 4), K H D < 2^20; stats fp32 [2][V][H] = (max, 1 / sum).  All contiguous.  workspace: forward and backward
+ * multiple of 4), K H D < 2^20, V < 2^24, E < 2^31 - 256; stats fp32 [2][V][H] = (max, 1 / sum).  All contiguous.  workspace: forward and backward
  * ask their own size. */
 typedef struct nbx_segment_attention_args {
     int64_t V, E, K;

@@ -262,6 +262,17 @@ def test_other_abi_refusals():
     assert L.nbx_segment_attention_workspace_bytes(ctypes.byref(at), 1, ctypes.byref(n)) == 0 and n.value >= 4 * 2 * 4
 
 
+@pytest.mark.parametrize("V,E,ok", [(2 ** 24 - 1, 2 ** 31 - 257, True), (2 ** 24 - 1, 2 ** 31 - 256, False),
+                                    (2 ** 24 - 1, 128 * (2 ** 24 - 1), False), (1, 2 ** 31 - 65, False), (2 ** 24, 4, False)])
+def test_attention_largest_sizes(V, E, ok):
+    """The list form's steps of 256 positions are counted in 32 bits: the last one may not pass 2^31 (2^24 - 1 lists
+    of 128 edges would have).  What is allowed gets as far as the operand check."""
+    L = lib.lib()
+    at = lib.SegmentAttentionArgs(V=V, E=E, K=1, H=1, D=4)
+    assert L.nbx_segment_attention(ctypes.byref(at), None) == 1
+    assert (b"null operand" in L.nbx_last_error()) == ok
+
+
 @pytest.mark.parametrize("name,mirror", [("nbx_residual_norm_args", lib.ResidualNormArgs),
                                          ("nbx_sh_residual_norm_args", lib.ShResidualNormArgs),
                                          ("nbx_segment_attention_args", lib.SegmentAttentionArgs)])
