@@ -252,8 +252,9 @@ def segment_attention(values, logits, ptr, eid, *, p=0.0, rng=None, call=None):
     values [E, K, H, D] (K rows per edge that share the heads' weights), logits [E, H] float32 or of values'
     type; ptr int32 [V + 1] and eid int32 [E]: the edges by destination, eid a permutation of the edges
     (``segnn_train.Graph``'s dptr / deid).  A node without edges, or whose logits are all -inf, gets 0; edges
-    in no list (positions from ptr[V] on, or named by no entry of eid) get gradients of 0.  A weight that is exactly 0 reads nothing of its
-    value.  H <= 64 and H D <= 4096 (1024 if D is no multiple of 4)."""
+    in no list (positions from ptr[V] on, or named by no entry of eid) get gradients of 0.  A weight that is exactly
+    0 reads nothing of its value.  H <= 64, H D <= 4096 (1024 if D is no multiple of 4), K H D < 2^20, V < 2^24 and
+    E < 2^31 - 256."""
     threshold = _threshold(p)
     cv, cl = _dtype(values, "values"), _dtype(logits, "logits")
     if values.dim() != 4 or logits.shape != (values.shape[0], values.shape[2]):
