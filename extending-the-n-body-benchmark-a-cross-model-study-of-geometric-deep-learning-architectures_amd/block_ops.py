@@ -18,6 +18,8 @@ function of (seed, step, call, index) alone (Philox4x32-10), so a step can be re
 backward pass needs no mask.  The drop rate is resolved to 2^-16 and the scale is that of the resolved rate,
 so the mean is exact.  A dropped element is 0 whatever it held.
 
+First derivatives by backward passes only: ``create_graph`` and forward-mode (dual) tensors are refused.
+
 Like the framework's other operators these run on the HIP device only.
 """
 from __future__ import annotations

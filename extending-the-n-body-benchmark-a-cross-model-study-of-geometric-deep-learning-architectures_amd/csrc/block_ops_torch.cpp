@@ -82,7 +82,11 @@ Tensor workspace(size_t bytes, const Tensor& on) {
     return bytes ? fresh({(int64_t)bytes}, at::kByte, on) : Tensor();
 }
 
+// Whether the call is recorded.  A dual tensor (forward-mode derivatives) need not require a gradient, and its
+// tangent would be lost without a word: refused.
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->defined() && t->_fw_grad(0).defined()) fail("block operators have no forward-mode derivatives");
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor* t : ts)
         if (t->defined() && t->requires_grad()) return true;

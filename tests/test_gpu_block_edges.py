@@ -3,12 +3,46 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import nbody_amd.block_ops as B
 from oracle import block_ops as O
 from test_gpu_block_ops import BF16, F16, F32, _bits, _lists, _rand
 
 pytestmark = pytest.mark.gpu
+
+
+def _operators(dev):
+    """name -> (the operator as a function of its tensors, those tensors)."""
+    r = _rand(0)
+    t = lambda *s: r(*s).to(dev)                                                             # noqa: E731
+    rng = torch.tensor([5, 1], dtype=torch.int64, device=dev)
+    ptr, eid = (q.to(dev) for q in _lists([3, 0, 5], 1))
+    return {
+        "dropout": (lambda x: B.dropout(x, 0.3, rng, call=0), [t(6, 8)]),
+        "residual_norm": (lambda x, y, g, w, b, w2, b2: B.residual_norm(x, y, gate=g, post=(w, b), pre=(w2, b2)),
+                          [t(6, 8), t(6, 8), t(3, 8), t(8), t(8), t(8), t(8)]),
+        "sh_residual_norm": (B.sh_residual_norm, [t(6, 4, 8), t(6, 4, 8), t(2, 8), t(8)]),
+        "segment_attention": (lambda v, l: B.segment_attention(v, l, ptr, eid), [t(8, 3, 2, 4), t(8, 2)])}
+
+
+OPERATORS = ("dropout", "residual_norm", "sh_residual_norm", "segment_attention")
+
+
+# ------------------------------------------------------------------------------------------------ derivatives
+@pytest.mark.parametrize("name", OPERATORS)
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(hip_device, name, grad):
+    """A dual tensor in any place, recorded or not: its tangent would be lost."""
+    from nbody_amd._lib import NbxError
+    f, ins = _operators(hip_device)[name]
+    for i, t in enumerate(ins):
+        for mode in (torch.enable_grad, torch.no_grad):
+            with forward_ad.dual_level(), mode():
+                dual = forward_ad.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))
+                with pytest.raises(NbxError, match="forward-mode"):
+                    f(*ins[:i], dual, *ins[i + 1:])
+    f(*ins)                                            # plain tensors again
 
 
 # ------------------------------------------------------------------------------------------------ segment attention
