@@ -78,6 +78,21 @@ Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t)
 Tensor empty_if(bool wanted, const Tensor& like) { return wanted && like.defined() ? fresh_like(like) : Tensor(); }
 Tensor used_state(const Tensor& state) { return state.defined() ? fresh_like(state) : Tensor(); }
 
+constexpr at::ScalarType TYPES[] = {at::kFloat, at::kBFloat16, at::kHalf};   // NBX_F32, NBX_BF16, NBX_F16
+
+// A saved tensor as it was saved: hooks (torch.autograd.graph.saved_tensors_hooks) may give back any other.
+// Contiguous but for the residual rows, whose strides are asked for (rows_of).
+Tensor unchanged(const Tensor& t, int64_t numel, at::ScalarType type, const Tensor& on) {
+    if (t.defined() && (t.numel() != numel || t.scalar_type() != type || t.device() != on.device()))
+        fail("a saved tensor came back as another: " + std::to_string(t.numel()) + " x " + toString(t.scalar_type()) +
+             " on " + t.device().str() + ", saved were " + std::to_string(numel) + " x " + toString(type) + " on " +
+             on.device().str());
+    return t;
+}
+Tensor restored(const Tensor& t, int64_t numel, at::ScalarType type, const Tensor& on) {
+    return dense(unchanged(t, numel, type, on));
+}
+
 Tensor workspace(size_t bytes, const Tensor& on) {
     return bytes ? fresh({(int64_t)bytes}, at::kByte, on) : Tensor();
 }
@@ -120,7 +135,8 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
         first_derivatives_only();
         const auto v = ctx->saved_data["how"].toIntVector();
         const DropoutHow h{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-        return {run_dropout(dy[0].contiguous(), h, ctx->get_saved_variables()[0], Tensor()), Tensor(), Tensor()};
+        const Tensor used = restored(ctx->get_saved_variables()[0], 2, at::kLong, dy[0]);
+        return {run_dropout(dy[0].contiguous(), h, used, Tensor()), Tensor(), Tensor()};
     }
 };
 
@@ -150,7 +166,7 @@ using ResidualArgs = nbx_residual_norm_args;
 
 // (tensor, elements between its rows): strided rows are read in place, anything else is copied
 std::pair<Tensor, int64_t> rows_of(const Tensor& t, int64_t C) {
-    if (t.dim() == 2 && t.size(0) > 1 && t.stride(1) == 1 && t.stride(0) >= C) return {t, t.stride(0)};
+    if (t.dim() == 2 && t.size(0) > 1 && t.size(1) == C && t.stride(1) == 1 && t.stride(0) >= C) return {t, t.stride(0)};
     return {t.contiguous(), C};
 }
 
@@ -208,20 +224,22 @@ struct ResidualFn : torch::autograd::Function<ResidualFn> {
         const Tensor dh = dense(g[0]), dz = g.size() > 1 ? dense(g[1]) : Tensor();
         if (!dh.defined() && !dz.defined()) return out;
         auto a = args_of<ResidualArgs>(ctx);
-        const auto s = ctx->get_saved_variables();
-        const Tensor &used = s[7], &stats = s[8];
-        Tensor y = s[0], h = s[1], x;
+        auto s = ctx->get_saved_variables();
+        const Tensor& any = dh.defined() ? dh : dz;
+        const at::ScalarType param = TYPES[a.param_dtype];
+        for (int i = 2; i < 7; ++i) s[i] = restored(s[i], i == 2 ? a.gate_groups * a.C : a.C, param, any);
+        const Tensor used = restored(s[7], 2, at::kLong, any), stats = restored(s[8], 4 * a.rows, at::kFloat, any);
+        Tensor y = unchanged(s[0], a.rows * a.C, TYPES[a.y_dtype], any), h = unchanged(s[1], a.rows * a.C, TYPES[a.x_dtype], any), x;
         if (h.defined() && a.x_dtype != NBX_F32) {
             std::tie(x, a.ldx) = rows_of(h, a.C);
             h = Tensor();
         }
-        if (y.defined()) std::tie(y, a.ldy) = rows_of(y, a.C);   // saved-tensor hooks may give other strides
-        const Tensor& any = dh.defined() ? dh : dz;
+        h = dense(h);
+        if (y.defined()) std::tie(y, a.ldy) = rows_of(y, a.C);
         set_params(a, s[2], s[3], s[4], s[5], s[6]);
         const auto shape = ctx->saved_data["x"].toIntVector();
-        static const at::ScalarType types[] = {at::kFloat, at::kBFloat16, at::kHalf};
-        if (ctx->needs_input_grad(0)) out[0] = fresh(shape, types[a.x_dtype], any);
-        if (ctx->needs_input_grad(1)) out[1] = fresh(shape, types[a.y_dtype], any);
+        if (ctx->needs_input_grad(0)) out[0] = fresh(shape, TYPES[a.x_dtype], any);
+        if (ctx->needs_input_grad(1)) out[1] = fresh(shape, TYPES[a.y_dtype], any);
         // without dz nothing reaches the norm behind the sum: its parameters' gradients are 0
         for (int i = 2, edge = 2; i < 7; ++i)   // an absent input has no edge
             if (s[i].defined()) out[i] = empty_if(ctx->needs_input_grad(edge++), s[i]);
@@ -321,7 +339,12 @@ struct ShFn : torch::autograd::Function<ShFn> {
         const Tensor dh = dense(g[0]), dz = dense(g[1]);
         if (!dh.defined() && !dz.defined()) return out;
         auto a = args_of<ShArgs>(ctx);
-        const auto s = ctx->get_saved_variables();
+        auto s = ctx->get_saved_variables();
+        const Tensor& any = dh.defined() ? dh : dz;
+        const int64_t L = a.lmax + 1, sizes[] = {a.V * L * L * a.C, L * a.C, a.C, 2, 2 * a.V, a.V * L * L * a.C};
+        const at::ScalarType types[] = {TYPES[a.dtype], TYPES[a.param_dtype], TYPES[a.param_dtype], at::kLong, at::kFloat,
+                                        TYPES[a.dtype]};
+        for (int i = 0; i < 6; ++i) s[i] = restored(s[i], sizes[i], types[i], any);
         for (int i = 0; i < 4; ++i) out[i] = empty_if(ctx->needs_input_grad(i), s[i < 2 ? 0 : i - 1]);
         if (a.dtype != NBX_F32) a.x = ptr(s[0]);
         else a.h = ptr(s[0]);
@@ -409,8 +432,11 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
         first_derivatives_only();
         variable_list out(6);
         auto a = args_of<AttentionArgs>(ctx);
-        const auto s = ctx->get_saved_variables();
+        auto s = ctx->get_saved_variables();
         const Tensor dout = g[0].contiguous();
+        const int64_t sizes[] = {a.E * a.K * a.H * a.D, a.E * a.H, a.V + 1, a.E, 2, 2 * a.V * a.H};
+        const at::ScalarType types[] = {TYPES[a.v_dtype], TYPES[a.l_dtype], at::kInt, at::kInt, at::kLong, at::kFloat};
+        for (int i = 0; i < 6; ++i) s[i] = restored(s[i], sizes[i], types[i], dout);
         for (int i = 0; i < 2; ++i) out[i] = empty_if(ctx->needs_input_grad(i), s[i]);
         set_lists(a, s[0], s[1], s[2], s[3]);
         a.rng = ptr<int64_t>(s[4]);

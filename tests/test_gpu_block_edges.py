@@ -45,6 +45,51 @@ def test_forward_mode_is_refused(hip_device, name, grad):
     f(*ins)                                            # plain tensors again
 
 
+def _gradients(f, ins, seed=7):
+    outs = f(*ins)
+    outs = [o for o in (outs if isinstance(outs, tuple) else (outs,)) if o is not None]
+    r = _rand(seed)
+    return torch.autograd.grad(outs, ins, [r(*o.shape).to(o) for o in outs])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("name", OPERATORS)
+def test_saved_tensors_with_other_strides(hip_device, name, dtype):
+    """Hooks on saved tensors may give the values back in another order of memory."""
+    f, ins = _operators(hip_device)[name]
+    ins = [t.to(dtype).requires_grad_() for t in ins]
+    want = _gradients(f, ins)
+    turn = lambda t: t.transpose(0, -1).contiguous().transpose(0, -1) if t.dim() > 1 else t     # noqa: E731
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, turn):
+        got = _gradients(f, ins)
+    assert all(_bits(a, b) for a, b in zip(want, got))
+    with torch.autograd.graph.save_on_cpu():
+        got = _gradients(f, ins)
+    assert all(_bits(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_saved_tensors_of_another_kind_are_refused(hip_device, name):
+    """One saved tensor after the other comes back with another type, another size or from another device."""
+    from nbody_amd._lib import NbxError
+    f, ins = _operators(hip_device)[name]
+    ins = [t.requires_grad_() for t in ins]
+    for change in (lambda t: t.to(torch.float16), lambda t: t.flatten()[:-1], lambda t: t.cpu()):
+        seen = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: (seen.append(0), t)[1]):
+            _gradients(f, ins)
+        assert seen
+        for i in range(len(seen)):
+            at = []
+
+            def unpack(t, i=i, at=at, change=change):
+                at.append(0)
+                return change(t) if len(at) == i + 1 else t
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                with pytest.raises(NbxError, match="saved tensor"):
+                    _gradients(f, ins)
+
+
 # ------------------------------------------------------------------------------------------------ segment attention
 @pytest.mark.parametrize("lengths", [[5, 3], [70, 0, 60], [0, 64, 1, 63, 200, 500, 3, 270, 0]])
 @pytest.mark.parametrize("K,H,D,dtype", [(1, 2, 4, F32), (2, 3, 5, BF16), (1, 4, 64, F16), (49, 8, 16, F32)])
