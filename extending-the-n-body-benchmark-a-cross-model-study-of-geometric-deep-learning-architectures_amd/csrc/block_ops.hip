@@ -476,6 +476,9 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
             s2 *= invC;
 #pragma unroll
             for (int k = 0; k < 8; ++k) t[k] = in.rs1 * (t[k] - s1 - v[k] * s2);
+            if (d.group && !m.k[0])   // the row is dropped, whatever it held: not 0 times an infinity's norm
+#pragma unroll
+                for (int k = 0; k < 8; ++k) t[k] = 0.f;
         }
         if (a.dy) store8n((TY*)a.dy + row + (uint32_t)c0, n, t);
         if constexpr (OWN) {

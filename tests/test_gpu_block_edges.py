@@ -90,6 +90,36 @@ def test_saved_tensors_of_another_kind_are_refused(hip_device, name):
                     _gradients(f, ins)
 
 
+# ------------------------------------------------------------------------------------------------ residual + norms
+@pytest.mark.parametrize("C", [40, 300, 600, 2100, 4200])
+@pytest.mark.parametrize("types", [(F32, F32, F32), (BF16, BF16, BF16), (F32, F16, F32)], ids=["f32", "bf16", "f16_in_f32"])
+@pytest.mark.parametrize("norm,gates", [("rms", 0), ("layer", 1), ("layer", 4), ("rms", 24)])
+@pytest.mark.parametrize("pre", [False, True])
+def test_residual_dropped_rows_hold_anything(hip_device, C, types, norm, gates, pre):
+    """Rows of a dropped group may hold infinities and NaN before their norm: results and every gradient are those
+    of rows of zeros there."""
+    xt, yt, pt = types
+    r, dev, R = _rand(C), hip_device, 24
+    rng = torch.tensor([11, 2], dtype=torch.int64, device=dev)
+    kept = O.keep(11, 3, 2, torch.arange(R).numpy() // 2, 0.5)
+    assert 4 < int(kept.sum()) < 20
+    x, y, dh, dz = (r(R, C).to(dev, t) for t in (xt, yt, xt, yt))
+    gate = (1 + 0.3 * r(gates, C)).to(dev, pt) if gates else None
+    w, b, w2 = ((1 + 0.3 * r(C)).to(dev, pt) for _ in range(3))
+
+    def run(fill):
+        held = torch.where(kept.to(dev)[:, None], y, fill.to(dev, yt))
+        ins = [t.clone().requires_grad_() for t in (x, held, w, b) + ((w2,) if pre else ()) + ((gate,) if gates else ())]
+        h, z = B.residual_norm(ins[0], ins[1], gate=ins[-1] if gates else None, post=(ins[2], ins[3]),
+                               pre=(ins[4], None) if pre else None, norm=norm, p=0.5, group=2, rng=rng, call=3)
+        outs, grads = ((h, z), (dh, dz)) if pre else ((h,), (dh,))
+        return [t.detach() for t in outs] + list(torch.autograd.grad(outs, ins, grads))
+    want = run(torch.zeros(()))
+    for fill in (torch.tensor(math.inf), torch.tensor(math.nan), torch.tensor([math.inf, -math.inf, 1.0, math.nan] * (C // 4))):
+        for a, c in zip(want, run(fill)):
+            assert torch.isfinite(c).all() and torch.equal(a, c)
+
+
 # ------------------------------------------------------------------------------------------------ segment attention
 @pytest.mark.parametrize("lengths", [[5, 3], [70, 0, 60], [0, 64, 1, 63, 200, 500, 3, 270, 0]])
 @pytest.mark.parametrize("K,H,D,dtype", [(1, 2, 4, F32), (2, 3, 5, BF16), (1, 4, 64, F16), (49, 8, 16, F32)])
