@@ -24,6 +24,8 @@ Like the framework's other operators these run on the HIP device only.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -150,9 +152,12 @@ def dropout(x, p, rng=None, *, call=None, per="element", group=1):
 
 # ---------------------------------------------------------------------------------------------- residual + norms
 def _consecutive(gate, y):
-    """Whether a gate row belongs to consecutive rows of y: one or two axes, or y's axes from the front, then ones."""
+    """Whether a gate row belongs to consecutive rows of y: one or two axes, or y's axes from the front, then ones.
+    Not [N, C] for y [B, N, C], which broadcasting would repeat over B (unless N is B, or 1)."""
     if gate.dim() <= 2:
-        return True
+        lead = y.shape[:-1]
+        return (gate.dim() < 2 or len(lead) < 2 or gate.shape[0] != lead[-1]
+                or any(gate.shape[0] == math.prod(lead[:k]) for k in range(len(lead) + 1)))
     same = 0
     while same < gate.dim() - 1 and gate.shape[:same + 1] == y.shape[:same + 1]:
         same += 1
@@ -167,10 +172,11 @@ def residual_norm(x, y, *, gate=None, scale=1.0, post=None, pre=None, norm="rms"
 
     x (the stream) and y (the block's output) [..., C] of one shape, C <= 8192; y of x's type, or of 16 bits
     under a float32 stream.  norm = "rms" or "layer" (biased variance), for both places.  gate: [C] (layer
-    scale), [G, C] (one row for each rows / G consecutive rows, whatever y's axes are), y's shape, or y's leading axes
-    followed by ones ([B, 1, C] for y [B, N, C]).  gate and the norms' parameters
-    are all float32 or all of y's type; their gradients are column sums in float32, rounded once.  p: drop rate
-    of every element, or with group > 0 of whole groups of that many consecutive rows."""
+    scale), [G, C] (one row for each rows / G consecutive rows, whatever y's axes are; refused for y [.., N, C] with
+    G = N, which reads as a row for each N, unless G is also the product of y's first axes), y's shape, or y's
+    leading axes followed by ones ([B, 1, C] for y [B, N, C]).  gate and the norms' parameters are all float32 or
+    all of y's type; their gradients are column sums in float32, rounded once.  p: drop rate of every element, or
+    with group > 0 of whole groups of that many consecutive rows."""
     if norm not in _NORM:
         raise ValueError(f'norm must be "rms" or "layer", got {norm!r}')
     threshold = _threshold(p)
@@ -196,8 +202,9 @@ def residual_norm(x, y, *, gate=None, scale=1.0, post=None, pre=None, norm="rms"
             raise ValueError(f"a norm's parameters must be [{C}], got {list(t.shape)}")
     if gate is not None and (gate.dim() < 1 or gate.shape[-1] != C or (rows and gate.numel() == 0)
                              or rows % max(gate.numel() // C, 1) or not _consecutive(gate, y)):
-        raise ValueError(f"gate {list(gate.shape)} must be [C], [G, C] with G dividing the {rows} rows, y's leading axes "
-                         f"followed by ones, or y's shape {list(y.shape)}")
+        raise ValueError(f"gate {list(gate.shape)} must be [C], [G, C] with G dividing the {rows} rows (a row for "
+                         f"consecutive rows: broadcasting over y's first axes is not done), y's leading axes followed by "
+                         f"ones, or y's shape {list(y.shape)}")
     if int(group) < 0:
         raise ValueError(f"group must be at least 0, got {group}")
     dev = _device(x, y, *params)

@@ -145,6 +145,17 @@ def test_residual_gate_shapes(shape, ok):
         B.residual_norm(_t(2, 5, 6), _t(2, 5, 6), gate=_t(*shape))
 
 
+@pytest.mark.parametrize("y,gates,ok", [
+    ((2, 5, 6), 5, False), ((2, 5, 6), 1, True), ((2, 5, 6), 2, True), ((5, 5, 6), 5, True), ((1, 5, 6), 5, True),
+    ((2, 1, 6), 1, True), ((2, 4, 6), 4, False), ((2, 4, 6), 8, True), ((4, 10, 6), 20, True), ((2, 3, 5, 6), 5, False),
+    ((2, 3, 5, 6), 6, True), ((2, 3, 6, 6), 6, True), ((2, 3, 5, 6), 15, True), ((20, 6), 20, True), ((20, 6), 5, True)])
+def test_residual_gate_rows_are_not_broadcast(y, gates, ok):
+    """A gate [N, C] for y [B, N, C] reads as broadcasting, which is not what a [G, C] gate means: refused where the
+    two differ."""
+    with pytest.raises(lib.NbxError if ok else ValueError, match="HIP device" if ok else "broadcasting"):
+        B.residual_norm(_t(*y), _t(*y), gate=_t(gates, 6))
+
+
 @pytest.mark.parametrize("kw,err", [
     (dict(x=_t(3, 5, 8), y=_t(3, 5, 8)), ValueError), (dict(x=_t(3, 64, 8), y=_t(3, 64, 8)), ValueError),
     (dict(x=_t(3, 4, 513), y=_t(3, 4, 513)), ValueError), (dict(x=_t(3, 32), y=_t(3, 32)), ValueError),
