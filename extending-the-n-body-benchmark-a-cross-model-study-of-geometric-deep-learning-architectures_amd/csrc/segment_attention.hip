@@ -86,19 +86,27 @@ __device__ __forceinline__ void note_used(const nbx_segment_attention_args& a) {
     }
 }
 
-// sV[i], i < cnt <= 64: the node whose list holds position p0 + i (the last v with ptr[v] <= p0 + i), or -1 in
-// none.  One wave: a 64-way search for the first position, then the starts of the nodes after it are dropped
-// on their positions and spread to the right.
-__device__ __forceinline__ void nodes_of_positions(const int32_t* __restrict__ ptr, int64_t V, int64_t p0, int cnt,
-                                                   int* sV) {
-    const int lane = threadIdx.x & 63;
-    int64_t lo = 0, hi = V;
+// The last v of [lo, V) with ptr[v] <= p (lo if there is none): a 64-way search by one wave.
+__device__ __forceinline__ int64_t last_start(const int32_t* __restrict__ ptr, int64_t lo, int64_t V, int64_t p) {
+    int64_t hi = V;
     while (hi - lo > 1) {
-        const int64_t step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step;
-        const uint64_t below = __ballot(at < hi && ptr[std::min(at, V)] <= p0);
+        const int64_t step = (hi - lo + 63) >> 6, at = lo + ((threadIdx.x & 63) + 1) * step;
+        const uint64_t below = __ballot(at < hi && ptr[std::min(at, V)] <= p);
         lo += __popcll(below) * step;
         hi = std::min(hi, lo + step);
     }
+    return lo;
+}
+
+// sV[i], i < cnt <= 64: the node whose list holds position p0 + i (the last v with ptr[v] <= p0 + i), or -1 in
+// none.  One wave: a search for the first position, then the starts of the nodes after it are dropped on their
+// positions and spread to the right.  A run of empty nodes is searched for its last one, so that at most two steps
+// and a search go to each position, however many nodes start there (2^22 empty nodes between two lists, the backward
+// pass: 24 ms walked 64 at a time, 0.02 ms searched).
+__device__ __forceinline__ void nodes_of_positions(const int32_t* __restrict__ ptr, int64_t V, int64_t p0, int cnt,
+                                                   int* sV) {
+    const int lane = threadIdx.x & 63;
+    const int64_t lo = last_start(ptr, 0, V, p0);
     sV[lane] = lane == 0 ? (int)lo : -1;
     __threadfence_block();
     for (int64_t v = lo + 1; v < V; v += 64) {
@@ -106,6 +114,12 @@ __device__ __forceinline__ void nodes_of_positions(const int32_t* __restrict__ p
         const int64_t at = mine < V ? ptr[mine] - p0 : cnt;
         if (at > 0 && at < cnt) atomicMax(&sV[at], (int)mine);
         if (__ballot(at >= cnt)) break;   // starts ascend: the later ones lie behind the block
+        const int first = __builtin_amdgcn_readlane((int)at, 0);
+        if (first == __builtin_amdgcn_readlane((int)at, 63)) {   // 64 nodes at one position
+            v = last_start(ptr, v + 63, V, p0 + first);
+            if (lane == 0 && first > 0 && first < cnt) atomicMax(&sV[first], (int)v);
+            v -= 63;   // the loop's step goes on behind it
+        }
     }
     __threadfence_block();
     int v = sV[lane];

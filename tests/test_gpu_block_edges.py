@@ -7,7 +7,7 @@ import torch.autograd.forward_ad as forward_ad
 
 import nbody_amd.block_ops as B
 from oracle import block_ops as O
-from test_gpu_block_ops import BF16, F16, F32, _bits, _lists, _rand
+from test_gpu_block_ops import BF16, F16, F32, _attention_case, _bits, _lists, _rand, rng  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -147,3 +147,41 @@ def test_attention_edges_that_no_entry_names(hip_device, lengths, K, H, D, dtype
     for n, t in zip({"both": ("dvalues", "dlogits"), "values": ("dvalues",), "logits": ("dlogits",)}[needs], got):
         assert not t[gone.to(dev)].any(), n
         O.within(t, ref[n], n)
+
+
+@pytest.mark.parametrize("runs", [(62,), (63,), (64,), (65,), (127,), (128,), (129, 62, 190), (4000,), (63, 64, 65, 700)])
+@pytest.mark.parametrize("n", [3, 31, 300])
+def test_attention_runs_of_empty_nodes(hip_device, rng, runs, n):             # noqa: F811
+    """Many nodes that start at one position, inside a block of positions, at its ends and on either side."""
+    lengths = [n]
+    for i, k in enumerate(runs):
+        lengths += [0] * k + [n + i]
+    _attention_case(hip_device, rng, lengths, 1, 2, 4, F32, F32, 0.1)
+    _attention_case(hip_device, rng, [0] * runs[0] + lengths + [0] * runs[-1], 1, 2, 4, F32, F32, 0.1, extra=5)
+    if n == 300:   # in chunks
+        _attention_case(hip_device, rng, lengths + [700, 5] + [0] * runs[0] + [60], 1, 2, 4, F32, F32, 0.1)
+
+
+def test_attention_does_not_walk_empty_nodes(hip_device):
+    """2^22 empty nodes between two lists of one block: 65536 dependent loads if they were walked 64 at a time (tens of
+    milliseconds), a few if searched.  The best of five passes counts."""
+    V, E, dev = 1 << 22, 61, hip_device
+    ptr = torch.full((V + 1,), 30, dtype=torch.int32)
+    ptr[0], ptr[-1] = 0, E
+    r = _rand(1)
+    v, l = r(E, 1, 2, 4).to(dev).requires_grad_(), r(E, 2).to(dev).requires_grad_()
+    out = B.segment_attention(v, l, ptr.to(dev), torch.arange(E, dtype=torch.int32, device=dev))
+    assert not out[1:-1].any()
+    dout, times = torch.ones_like(out), []
+    for _ in range(5):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        got = torch.autograd.grad(out, (v, l), dout, retain_graph=True)
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+    ref = B.segment_attention(v, l, torch.tensor([0, 30, E], dtype=torch.int32, device=dev),
+                              torch.arange(E, dtype=torch.int32, device=dev))
+    want = torch.autograd.grad(ref, (v, l), torch.ones_like(ref))
+    assert all(_bits(p, q) for p, q in zip(got, want))
+    assert min(times) < 4.0, times
