@@ -250,7 +250,8 @@ RowPlan row_plan(int64_t rows, int64_t C, int64_t gate_groups) {
     // up to 768 blocks, three on each CU at its 168 registers; each leaves one partial row per sum, read once
     // more.  16384 rows of 2048 bf16 columns, kernel + sums: 109 + 10 us at 512 blocks, 94 + 14 at 768, 110 + 18
     // at 1024 (149 + 19 at four blocks to a CU: the registers spill).  Rows of more than 2048 columns have one block
-    // to a CU: 4096 rows of 8192, 180 + 14 us at 256 blocks, 191 + 23 at 512, 217 + 31 at 768
+    // to a CU: 4096 rows of 8192, fp32 188 + 11 us at 256 blocks, 200 + 15 at 512, 213 + 21 at 768 (bf16 223 + 11, 231 +
+    // 15, 260 + 22)
     const int64_t chunk = std::max<int64_t>(p.rpb, ceil_div(rows, p.W >= 0 ? 768 : 256));
     p.whole = p.rpg < chunk && groups > 1;
     if (p.whole) {
@@ -323,7 +324,8 @@ __global__ __launch_bounds__(W >= 0 ? 256 : W == -1 ? 512 : 1024, W >= 0 ? 3 : 1
     const bool rowgate = OWN && !p.whole, post = NORM && a.post_w, pre = NORM && a.pre_w && a.dz;
     constexpr bool AGAIN = sizeof(TX) == 2;
     // at 16 waves a block (128 registers a thread) no row is fetched ahead and the weights are read per row: 4096 rows
-    // of 8192 bf16 columns 217 us, fetched ahead with spills 264 (fp32: 225 / 350)
+    // of 8192 fp32 columns 188 us, fetched ahead with spills 304.  For 16-bit rows fetching ahead spills less, and is
+    // the faster since their norm gradients are formed from x and y (bf16: 189 us against 223 as it is here)
     constexpr bool LEAN = W == -2;
     const bool need_y = post || a.dgate || (AGAIN && pre);
     float acc[SUMS][8] = {}, ag[OWN ? 8 : 1] = {};

@@ -488,7 +488,8 @@ __global__ __launch_bounds__(256) void segment_attention_join_kernel(nbx_segment
 // position) and its share of the sum: slot 2 block = the list that began before, 2 block + 1 = the one that
 // goes on.  Threads: EL groups of RV, or (long rows) TP threads, a multiple of the H D / VW columns, over the
 // row in steps of TP: either way a thread stays with one head.  2560 edges of 49 x 8 x 16 fp32: 35.5 us (145 MB at
-// 4.1 TB/s) + 3.5; 60000 edges of 8 x 64 bf16: 30 us (123 MB at 4.1 TB/s) + 8 for the lists that cross.
+// 4.1 TB/s) + 4 for the second launch; 60000 edges of 8 x 64 bf16: 30 us (123 MB at 4.1 TB/s) + 9 (the check of
+// missing edges is about 1 of them; in it every block that a list crosses sums the shares of all the list's blocks).
 template <typename T, int VW>
 __global__ __launch_bounds__(1024) void segment_attention_bwd_kernel(nbx_segment_attention_args a, SaPlan p, float keep,
                                                                      float* __restrict__ wa, float* __restrict__ wd,
@@ -704,8 +705,10 @@ SaPlan forward_plan(const nbx_segment_attention_args& a) {
     // The lists' lengths are on the device.  E a multiple of V is taken for lists of one length (a fully connected
     // graph): the list form up to 128 edges (K 1, 8 heads of 16, fp32, both passes: 4096 x 7 37 us against 53 in
     // chunks, 2048 x 15 31 / 43, 1040 x 64 40 / 43, 516 x 128 43 / 47).  Otherwise chunks, which do not wait for the
-    // longest list (ragged lists, 60000 edges to 3000 nodes: 61 us against 107 in list form, to 1000: 52 / 156;
-    // 20000 to 2000: 61 / 58), but for small graphs, where the list form's single launch counts.
+    // longest list (ragged lists, 60001 edges to 3000 nodes: 61 us, to 1000: 52; 20001 to 2000: 56), but for small
+    // graphs, where the list form's single launch counts.  It is a guess: ragged lists whose E happens to be a multiple
+    // of V run the list form too, and wait for the longest list (60000 edges to 3000 nodes: 107 us, to 1000: 157; 20000
+    // to 2000: 60).
     p.chunked = a.V && a.E % a.V == 0 ? a.E > 128 * a.V : a.E > 1024;
     // edges whose weights a list's block forms at once: 256 for long lists (60000 edges to 1000 nodes in list form:
     // 127 us against 151 at 64), 64 where lists are short or heads many, for the LDS
@@ -728,7 +731,7 @@ SaPlan backward_plan(const nbx_segment_attention_args& a) {
     p.grp = g <= 64 && (g & (g - 1)) == 0 ? g : 1;
     p.entries = std::min(p.RV, p.TP) / p.grp;
     // positions per block: enough blocks for the chip first, then few (each has its searches and sums), within
-    // 48 KB of LDS: 60000 edges of 8 x 64 bf16 take 46 us at 16, 40 at 32, 38 at 64; long rows (2560 edges of 49 x 8
+    // 48 KB of LDS: 60000 edges of 8 x 64 bf16 take 49 us at 16, 42 at 32, 39 at 64; long rows (2560 edges of 49 x 8
     // x 16 fp32) 40 us at 2, 38 at 4, 48 at 8, 77 at 16
     p.eb = p.RV <= p.T ? TILE : 4;
     while (p.eb > 4 && (a.E < 768 * (int64_t)p.eb || p.eb * (p.entries + 3 * a.H) > 12288)) p.eb /= 2;
