@@ -273,7 +273,7 @@ enum { SUM_A, SUM_B, SUM_PRE_W, SUM_PRE_B, SUMS };
 
 // The backward pass reads y, h, dh and dz once; statistics come from the forward pass.  A 16-bit h has lost what
 // xhat needs (the weight gradients would be off by its rounding again), so there x is read in its place and h
-// is formed again from x and y.  The same 16384 x 2048 bf16 block: 96 us, 403 MB at 4.2 TB/s, and 9.5 us for the sums.
+// is formed again from x and y.  The same 16384 x 2048 bf16 block: 98 us, 403 MB at 4.1 TB/s, and 9.5 us for the sums.
 template <typename TX, typename TY>
 struct RowIn {   // a row's eight columns as loaded, one row ahead of their use
     Raw8<TX> dh, h;   // h: x where h is formed again
